@@ -225,6 +225,130 @@ TK_API cudaError_t tk_attention_forward_gqa_f16(const void* q, const void* k, co
                                                 int seq, int head_dim, float scale, int causal,
                                                 cudaStream_t stream);
 
+/* Attention forward for a language model's prompts, a further generalisation (no
+ * counterpart in the reference): score changes, masks, 16-bit outputs, strides.
+ *   s_ij = scale * q_i . k_j;  softcap > 0: s_ij = softcap * tanh(s_ij / softcap);
+ *   alibi_slopes (device, [heads_q]): s_ij -= alibi_slopes[h] * |pos_i - j|;
+ *   out_i = sum_j softmax_j(s_ij) v_j over the keys row i may see, and 0 where it may
+ *   see none.
+ * Q and out are [batch, heads_q, seq_q, head_dim], K and V [batch, heads_kv, seq_kv,
+ * head_dim]; query head h reads key head h / (heads_q / heads_kv). Row i stands at
+ * pos_i = i + seq_kv - seq_q (the queries are the last positions). Masks:
+ *   - causal (0 or 1): keys j <= pos_i. A row at a negative position sees none.
+ *   - prefix_lens (device int32, [batch], needs causal = 1): also keys
+ *     j < prefix_lens[b].
+ *   - doc_ids (device int32, contiguous [batch, seq_q], needs seq_q == seq_kv, not
+ *     with prefix_lens): only keys of the row's own document. Each maximal run of
+ *     equal ids is a document; a negative id is padding, which sees and is seen by
+ *     nothing, and whose K and V may hold anything (NaN included).
+ * Elements are binary16 (_f16) or bfloat16 (_bf16), out alike. Probabilities are
+ * rounded to that type before the PV product, everything between is FP32.
+ * head_dim in {16, 32, 64, 128}; seq_q, seq_kv >= 1; any finite scale; softcap >= 0
+ * (0: none).
+ * strides (host): 12 values in elements, (batch, head, row) of Q, K, V and out in
+ * turn, or NULL for contiguous tensors; the elements of a row are adjacent. Strides of
+ * dimensions larger than 1 must be positive, and out's rows must not share elements.
+ * Operands whose base or strides are not multiples of 16 bytes are first copied into
+ * stream-ordered scratch, which the documents' row intervals (8 bytes a row) and the
+ * work counter come from too. Except for padding, V must be finite: a masked key in a
+ * block of 128 that other rows see is multiplied by 0. */
+TK_API cudaError_t tk_attention_masked_f16(const void* q, const void* k, const void* v, void* out,
+                                           const int64_t* strides, int batch, int heads_q,
+                                           int heads_kv, int seq_q, int seq_kv, int head_dim,
+                                           float scale, float softcap, const float* alibi_slopes,
+                                           const int32_t* doc_ids, const int32_t* prefix_lens,
+                                           int causal, cudaStream_t stream);
+TK_API cudaError_t tk_attention_masked_bf16(const void* q, const void* k, const void* v, void* out,
+                                            const int64_t* strides, int batch, int heads_q,
+                                            int heads_kv, int seq_q, int seq_kv, int head_dim,
+                                            float scale, float softcap, const float* alibi_slopes,
+                                            const int32_t* doc_ids, const int32_t* prefix_lens,
+                                            int causal, cudaStream_t stream);
+
+/* ---- paged key/value cache in 8 bits (no counterpart in the reference) ---------------- */
+/* A cache has n_pages pages of page_size token places. k_cache and v_cache are
+ * [n_pages, heads_kv, page_size, head_dim] e4m3 bytes, k_scale and v_scale
+ * [n_pages, heads_kv] FP32: a byte stands for scale * e4m3. Slot s is place
+ * s % page_size of page s / page_size. A request's tokens lie, in order, in the
+ * pages of its row of the block table (int32 [n_requests, max_pages]). */
+
+/* Places for the new tokens of a step, from request lengths, on the GPU. Request r
+ * holds cached_lens[r] tokens and adds new_lens[r] (negative values count as 0).
+ *   - It is taken if new_lens[r] > 0, its row has room (max_pages), its tokens end
+ *     at or before max_tokens, and it needs no new page or the pages needed up to and
+ *     including it (in request order, requests that fail the other conditions not
+ *     counted) are at most *n_free.
+ *   - Page k of the call (k = 0, 1, ...) is free_pages[*n_free - 1 - k]; it is
+ *     entered into block_table (other entries stay as they are).
+ * Outputs: lens_out [n_requests] (tokens held afterwards; may be cached_lens itself),
+ * seq_lens [n_requests] (the same, but 0 for a request not taken: what the attention
+ * of this step sees), starts [n_requests + 1] (first token of each request in the
+ * packed order, by new_lens, taken or not), slots [max_tokens] (slot of each packed
+ * token; -1 for tokens of requests not taken, behind a negative table entry, and
+ * behind the last token), n_free_out (may be n_free). free_pages is not changed. To
+ * give pages back, a caller writes them at free_pages[*n_free ...] and raises *n_free.
+ * Any page_size >= 1; *n_free is taken as at most n_free_capacity. One launch, no scratch. */
+TK_API cudaError_t tk_kv_plan(const int32_t* cached_lens, const int32_t* new_lens, int n_requests,
+                              int page_size, int32_t* block_table, int max_pages,
+                              const int32_t* free_pages, int n_free_capacity, const int32_t* n_free,
+                              int32_t* lens_out, int32_t* seq_lens, int32_t* starts, int64_t* slots,
+                              int max_tokens, int32_t* n_free_out, cudaStream_t stream);
+
+/* Quantises new tokens into the cache. k and v hold n_tokens tokens of [heads_kv,
+ * head_dim] 16-bit elements (binary16 or bfloat16), k_stride and v_stride elements
+ * apart; token t goes to slots[t] (out of range: skipped). For each page and head that
+ * gets tokens:
+ *   scale = 2^e, the smallest with |x| <= 448 * 2^e for the new tokens' finite x, at
+ *   least 2^-100; if the page held tokens before (its first new place is not 0), not
+ *   below its scale, and where that grows the places before the first new one become
+ *   e4m3(old value * old scale / new scale);
+ *   new bytes = e4m3(x / scale), nearest even, infinities as 448, NaN as NaN.
+ * Tokens of one page must be adjacent, with consecutive slots, as tk_kv_plan gives
+ * them; what a page holds that is named in two separate stretches is not defined.
+ * Other places keep their bytes. head_dim 64 or 128, page_size 16, 32, 64 or 128; k, v
+ * and the caches 16-byte aligned, strides multiples of 8. One launch, no scratch. */
+TK_API cudaError_t tk_kv_append_e4m3_f16(const void* k, const void* v, int64_t k_stride,
+                                         int64_t v_stride, const int64_t* slots, int n_tokens,
+                                         int heads_kv, int head_dim, void* k_cache, void* v_cache,
+                                         float* k_scale, float* v_scale, int n_pages, int page_size,
+                                         cudaStream_t stream);
+TK_API cudaError_t tk_kv_append_e4m3_bf16(const void* k, const void* v, int64_t k_stride,
+                                          int64_t v_stride, const int64_t* slots, int n_tokens,
+                                          int heads_kv, int head_dim, void* k_cache, void* v_cache,
+                                          float* k_scale, float* v_scale, int n_pages, int page_size,
+                                          cudaStream_t stream);
+
+/* Attention of each request's newest tokens over its cached ones (which include them:
+ * append first). q and out hold n_tokens packed tokens of [heads_q, head_dim] 16-bit
+ * elements, q_stride and out_stride elements apart; tokens starts[r] .. starts[r + 1]
+ * are the last positions of request r, whose cache holds seq_lens[r] tokens. Query at
+ * position pos sees positions 0 .. pos. Scores as for tk_attention_masked (scale,
+ * softcap, alibi_slopes); the softmax is FP32, probabilities are rounded to binary16,
+ * and out has q's type. A row without a key (seq_lens[r] = 0, or all its pages outside
+ * [0, n_pages)) is 0; tokens of pages outside that range are as if they were not there;
+ * tokens behind starts[n_requests] are left as they were. Bytes behind a request's
+ * last token may hold anything.
+ * max_query_len: at least the largest number of query tokens of a request (rows past it
+ * are left as they were). max_seq_len only sets how the work is split and should be near
+ * the largest seq_lens; results are right for any. head_dim 64 or 128; page_size 16, 32,
+ * 64 or 128; q and out 16-byte aligned with strides that are multiples of 8, caches
+ * 32-byte aligned; n_requests * heads_kv * ceil(max_query_len * heads_q / heads_kv / 16)
+ * at most 2^24. Long contexts take scratch for their chunks' partial sums. */
+TK_API cudaError_t tk_attention_paged_e4m3_f16(
+    const void* q, int64_t q_stride, void* out, int64_t out_stride, int n_tokens, const void* k_cache,
+    const void* v_cache, const float* k_scale, const float* v_scale, int n_pages, int page_size,
+    const int32_t* block_table, int max_pages, const int32_t* seq_lens, const int32_t* starts,
+    int n_requests, int heads_q, int heads_kv, int head_dim, int max_query_len, int max_seq_len,
+    float scale, float softcap, const float* alibi_slopes, cudaStream_t stream);
+TK_API cudaError_t tk_attention_paged_e4m3_bf16(
+    const void* q, int64_t q_stride, void* out, int64_t out_stride, int n_tokens, const void* k_cache,
+    const void* v_cache, const float* k_scale, const float* v_scale, int n_pages, int page_size,
+    const int32_t* block_table, int max_pages, const int32_t* seq_lens, const int32_t* starts,
+    int n_requests, int heads_q, int heads_kv, int head_dim, int max_query_len, int max_seq_len,
+    float scale, float softcap, const float* alibi_slopes, cudaStream_t stream);
+
+/* ---- tuning switches ---------------------------------------------------------- */
+
 /* No counterpart in the reference (a tuning switch). GEMMs with m <= 64 (and no fused
  * epilogue) run on an operand-swapped kernel by default (1): C^T = B^T A^T, so the rows
  * of A become the tensor-core MMA's N dimension (16..64) and 128 columns of B its M;

@@ -1,0 +1,983 @@
+// attention_masked.cuh — attention forward under masks and score changes, on sm_100a:
+//
+//   s_ij = scale * q_i . k_j
+//   s_ij = softcap * tanh(s_ij / softcap)          if softcap > 0
+//   s_ij -= slope_h * |pos_i - j|                  if slopes are given
+//   o_i  = sum_j softmax_j(s_ij) v_j  over the keys row i may see; 0 if there are none
+//
+// pos_i = i + seq_kv - seq_q. Every mask offered here leaves each row ONE interval of
+// keys [lo_i, hi_i): causal [0, pos + 1), a prefix [0, max(pos + 1, prefix)), documents
+// the run of equal ids that holds the row (cut at pos + 1 if causal). So a block of
+// 128 keys is either outside the intervals of all rows of a tile (it is not loaded
+// and not multiplied), inside all of them (no mask is computed), or on an edge.
+//
+// The pipeline is that of attention.cuh: persistent CTAs, two 128-row query tiles each,
+// one TMA warp, one MMA-issuing thread, two softmax warpgroups, P written back over S
+// in tensor memory; see there for the tensor-memory map, the issue order and its
+// hazards. What differs:
+//  - each of the two tiles has its own range of key blocks, and the item's loads cover
+//    both;
+//  - binary16 or bfloat16 in and out, any strides of batch, head and row (4-D tensor maps);
+//  - the reference point of a row that has not met an allowed key stays -inf;
+//  - P is held as 2^(x - m + 7), so that binary16 keeps its 11 bits down to 2^-21 of
+//    the row's largest weight;
+//  - with documents, warp 10 zeroes the V rows of padding (negative ids) in shared
+//    memory before the PV product reads them: 0 * NaN would be NaN.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include <atomic>
+#include <climits>
+
+#include "attention.cuh"
+
+namespace tk {
+namespace masked {
+
+using attn::ex2;
+using attn::fma2;
+using attn::kBlockKV;
+using attn::kBlockQ;
+using attn::kKvSlots;
+using attn::kRegsControl;
+using attn::kRegsSoftmax;
+using attn::kThreads;
+using attn::kTmemCols;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLift = 7.0f;  // P <= 2^(8 + kLift) = 2^15 < 65504
+
+template <int kDPad, bool kBf16>
+struct Cfg : attn::Cfg<kDPad> {
+    static constexpr uint32_t kFormat = kBf16 ? (1u << 7) | (1u << 10) : 0u;  // A and B alike
+    static constexpr uint32_t kIdescS = attn::Cfg<kDPad>::kIdescS | kFormat;
+    static constexpr uint32_t kIdescO = attn::Cfg<kDPad>::kIdescO | kFormat;
+};
+
+struct Params {
+    int seq_q, seq_kv, head_dim;
+    int pairs;              // ceil(seq_q / 256)
+    int heads_q, heads_kv, group;
+    int num_items;          // batch * heads_q * pairs
+    int* next_item;         // zeroed counter, or null: item w -> CTA w % grid
+    int causal;
+    const int* prefix;      // [batch] or null
+    const int2* rows;       // documents: [batch, seq] (lo, hi) of each row, before the causal cut; or null
+    const int4* tiles;      // documents: [batch, 2 pairs] (lo, hi, holds padding, 0) of each 128 rows
+    float scale;            // of the raw product
+    float scale_log2;       // scale * log2(e)
+    float softcap;          // 0: none
+    const float* slopes;    // [heads_q] or null
+    uint16_t* out;
+    long long out_b, out_h, out_s;  // strides in elements
+    bool out_vec;           // 16-byte stores
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, uint32_t bar, int x, int y, int z, int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (kBf16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        return attn::pack_half2(lo, hi);
+    }
+}
+
+// ---- documents --------------------------------------------------------------------
+
+// For every position of a packed row: the run of equal ids that holds it (empty where
+// the id is negative). One CTA per batch row; 8 positions a thread, 8192 a step: a
+// running maximum of run starts going forward, a running minimum of run ends going
+// back. Then the intervals' hull for each 128 rows. Also zeroes the item counter.
+constexpr int kRunThreads = 1024;
+constexpr int kRunEach = 8;
+constexpr int kRunStep = kRunThreads * kRunEach;
+
+template <bool kMax>
+__device__ __forceinline__ int extreme(int a, int b) { return kMax ? max(a, b) : min(a, b); }
+
+// Exclusive running max (kMax, from thread 0 up) or min (from the last thread down) over
+// the CTA; `all` is the extreme of every thread's value.
+template <bool kMax>
+__device__ __forceinline__ int block_running(int v, int none, int* warp_values, int& all) {
+    const int lane = static_cast<int>(lane_id());
+    const int warp = static_cast<int>(threadIdx.x >> 5);
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int other = kMax ? __shfl_up_sync(0xffffffffu, x, o) : __shfl_down_sync(0xffffffffu, x, o);
+        if (kMax ? lane >= o : lane + o < 32) x = extreme<kMax>(x, other);
+    }
+    if (lane == (kMax ? 31 : 0)) warp_values[warp] = x;
+    int before = kMax ? __shfl_up_sync(0xffffffffu, x, 1) : __shfl_down_sync(0xffffffffu, x, 1);
+    if (lane == (kMax ? 0 : 31)) before = none;
+    __syncthreads();
+    int w = warp_values[lane];
+    int y = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int other = kMax ? __shfl_up_sync(0xffffffffu, y, o) : __shfl_down_sync(0xffffffffu, y, o);
+        if (kMax ? lane >= o : lane + o < 32) y = extreme<kMax>(y, other);
+    }
+    all = __shfl_sync(0xffffffffu, y, kMax ? 31 : 0);
+    int outer = __shfl_sync(0xffffffffu, y, kMax ? max(warp - 1, 0) : min(warp + 1, 31));
+    if (warp == (kMax ? 0 : 31)) outer = none;
+    __syncthreads();
+    return extreme<kMax>(before, outer);
+}
+
+__global__ void __launch_bounds__(kRunThreads) runs_kernel(const int* __restrict__ ids, int seq, int n_tiles, int causal,
+                                                           int2* rows, int4* tiles, int* next_item) {
+    __shared__ int warp_values[32];
+    const int tid = static_cast<int>(threadIdx.x);
+    ids += static_cast<long long>(blockIdx.x) * seq;
+    rows += static_cast<long long>(blockIdx.x) * seq;
+    tiles += static_cast<long long>(blockIdx.x) * n_tiles;
+    if (blockIdx.x == 0 && tid == 0 && next_item != nullptr) *next_item = 0;
+    int carry = 0;
+    for (int base = 0; base < seq; base += kRunStep) {
+        const int s0 = base + tid * kRunEach;
+        int id[kRunEach], before = s0 > 0 && s0 < seq ? ids[s0 - 1] : 0;
+        int last = -1;
+#pragma unroll
+        for (int i = 0; i < kRunEach; ++i) {
+            id[i] = s0 + i < seq ? ids[s0 + i] : -1;
+            if (s0 + i < seq && (s0 + i == 0 || id[i] != (i > 0 ? id[i - 1] : before))) last = s0 + i;
+        }
+        int all;
+        int start = max(block_running<true>(last, -1, warp_values, all), carry);
+#pragma unroll
+        for (int i = 0; i < kRunEach; ++i) {
+            if (s0 + i < seq) {
+                if (id[i] != (i > 0 ? id[i - 1] : before)) start = s0 + i;
+                rows[s0 + i].x = id[i] >= 0 ? start : 0;
+            }
+        }
+        carry = max(carry, all);
+    }
+    carry = seq;
+    for (int base = (seq - 1) / kRunStep * kRunStep; base >= 0; base -= kRunStep) {
+        const int s0 = base + tid * kRunEach;
+        int id[kRunEach];
+        const int after = s0 + kRunEach < seq ? ids[s0 + kRunEach] : 0;
+        int first = INT_MAX;  // smallest run end (exclusive) in these positions
+#pragma unroll
+        for (int i = kRunEach - 1; i >= 0; --i) {
+            id[i] = s0 + i < seq ? ids[s0 + i] : -1;
+            if (s0 + i < seq && (s0 + i == seq - 1 || id[i] != (i < kRunEach - 1 ? id[i + 1] : after))) first = s0 + i + 1;
+        }
+        int all;
+        int end = min(block_running<false>(first, INT_MAX, warp_values, all), carry);
+#pragma unroll
+        for (int i = kRunEach - 1; i >= 0; --i) {
+            if (s0 + i < seq) {
+                if (s0 + i == seq - 1 || id[i] != (i < kRunEach - 1 ? id[i + 1] : after)) end = s0 + i + 1;
+                rows[s0 + i].y = id[i] >= 0 ? end : 0;
+            }
+        }
+        carry = min(carry, all);
+    }
+    __syncthreads();
+    const int lane = static_cast<int>(lane_id());
+    for (int tile = tid >> 5; tile < n_tiles; tile += kRunThreads / 32) {
+        int lo = INT_MAX, hi = 0, pad = 0;
+#pragma unroll
+        for (int i = 0; i < kBlockQ / 32; ++i) {
+            const int s = tile * kBlockQ + i * 32 + lane;
+            if (s >= seq) continue;
+            const int2 r = rows[s];
+            if (r.x < r.y) {
+                lo = min(lo, r.x);
+                hi = max(hi, causal ? min(r.y, s + 1) : r.y);
+            } else {
+                pad = 1;
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            pad |= __shfl_xor_sync(0xffffffffu, pad, o);
+        }
+        if (lane == 0) tiles[tile] = make_int4(lo, hi, pad, 0);
+    }
+}
+
+// ---- work items ---------------------------------------------------------------------
+
+// One (batch, head) and two 128-row query tiles; within a (batch, head), later pairs
+// first (under a causal mask they see more keys). Tile g works on key blocks
+// [b0[g], b1[g]) (empty if b0 >= b1); the item's loads cover [jb, je).
+struct Item {
+    int batch, head, head_kv, q0;
+    int b0[2], b1[2];
+    int jb, je;
+};
+
+__device__ __forceinline__ Item make_item(int w, const Params& p) {
+    Item it;
+    const int pair = p.pairs - 1 - w % p.pairs;
+    const int bh = w / p.pairs;
+    it.batch = bh / p.heads_q;
+    it.head = bh % p.heads_q;
+    it.head_kv = it.head / p.group;
+    it.q0 = pair * 2 * kBlockQ;
+    it.jb = INT_MAX;
+    it.je = 0;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        const int r0 = it.q0 + g * kBlockQ;
+        int lo = 0, hi = 0;
+        if (r0 < p.seq_q) {
+            if (p.tiles != nullptr) {
+                const int4 t = __ldg(p.tiles + (static_cast<long long>(it.batch) * 2 * p.pairs + 2 * pair + g));
+                lo = t.x;
+                hi = t.y;
+            } else {
+                hi = p.seq_kv;
+                if (p.causal) {
+                    hi = min(r0 + kBlockQ, p.seq_q) + (p.seq_kv - p.seq_q);
+                    if (p.prefix != nullptr) hi = max(hi, __ldg(p.prefix + it.batch));
+                    hi = min(max(hi, 0), p.seq_kv);
+                }
+            }
+        }
+        it.b0[g] = lo < hi ? lo / kBlockKV : 0;
+        it.b1[g] = lo < hi ? (hi + kBlockKV - 1) / kBlockKV : 0;
+        if (it.b0[g] < it.b1[g]) {
+            it.jb = min(it.jb, it.b0[g]);
+            it.je = max(it.je, it.b1[g]);
+        }
+    }
+    if (it.je == 0) it.jb = 0;
+    return it;
+}
+
+// ---- scores ---------------------------------------------------------------------------
+
+// Keys outside [lo, hi) (relative to the block) become -inf.
+__device__ __forceinline__ void mask_row(uint32_t (&r)[128], int lo, int hi) {
+#pragma unroll
+    for (int i = 0; i < 128; ++i)
+        if (i < lo || i >= hi) r[i] = 0xff800000u;
+}
+
+// 2^(s c + a) of the row's 128 scores; writes them, rounded to 16 bits, over the first 64
+// columns of S, and returns their sum.
+template <bool kBf16>
+__device__ __forceinline__ float exp_store(uint32_t s_addr, const uint32_t (&r)[128], float c, float a) {
+    float2 acc[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[t] = make_float2(0.0f, 0.0f);
+    const float2 c2 = make_float2(c, c), a2 = make_float2(a, a);
+#pragma unroll
+    for (int chunk = 0; chunk < 4; ++chunk) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int idx = 32 * chunk + 2 * i;
+            const float2 x = fma2(make_float2(__uint_as_float(r[idx]), __uint_as_float(r[idx + 1])), c2, a2);
+            const float2 e = make_float2(ex2(x.x), ex2(x.y));
+            acc[i & 3] = attn::add2(acc[i & 3], e);
+            pk[i] = pack2<kBf16>(e.x, e.y);
+        }
+        tmem_st_32x32b_x16(s_addr + 16 * chunk, pk);
+    }
+    const float2 t = attn::add2(attn::add2(acc[0], acc[1]), attn::add2(acc[2], acc[3]));
+    return t.x + t.y;
+}
+
+// softcap * tanh(s scale / softcap) in log2 units, in place:
+// tanh(x) = 1 - 2 / (1 + e^2x), which is 1 and -1 where the exponential is infinite or 0.
+__device__ __forceinline__ void cap_row(uint32_t (&r)[128], float over, float cap) {
+    const float in = over * 2.0f * kLog2e, out = cap * kLog2e;
+#pragma unroll
+    for (int i = 0; i < 128; ++i) {
+        const float e = ex2(__uint_as_float(r[i]) * in);
+        r[i] = __float_as_uint(fmaf(-2.0f * out, rcp_approx(1.0f + e), out));
+    }
+}
+
+// s c - slope |pos - j|, in place; `from` = pos - first key of the block.
+__device__ __forceinline__ void bias_row(uint32_t (&r)[128], float c, float slope, int from) {
+    const float f = static_cast<float>(from);
+#pragma unroll
+    for (int i = 0; i < 128; ++i)
+        r[i] = __float_as_uint(fmaf(fabsf(f - static_cast<float>(i)), -slope, __uint_as_float(r[i]) * c));
+}
+
+// ---- kernel ---------------------------------------------------------------------------
+
+template <int kDPad, bool kBf16, bool kChange>
+__global__ void __launch_bounds__(kThreads, 1)
+    masked_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const Params p) {
+    using C = Cfg<kDPad, kBf16>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_base = smem_u32(smem_raw);
+    const uint32_t base = (raw_base + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (base - raw_base);
+    const uint32_t bars = base + C::kBarOffset;
+    auto kv_full = [&](int s) { return bars + 8u * s; };
+    auto kv_empty = [&](int s) { return bars + 8u * (kKvSlots + s); };
+    constexpr int kB = 2 * kKvSlots;
+    const uint32_t q_full = bars + 8u * kB;
+    const uint32_t q_empty = bars + 8u * (kB + 1);
+    auto s_full = [&](int g) { return bars + 8u * (kB + 2 + g); };
+    auto p_ready = [&](int g) { return bars + 8u * (kB + 4 + g); };
+    auto o_final = [&](int g) { return bars + 8u * (kB + 6 + g); };
+    auto o_empty = [&](int g) { return bars + 8u * (kB + 8 + g); };
+    auto item_full = [&](int s) { return bars + 8u * (kB + 10 + s); };
+    auto item_empty = [&](int s) { return bars + 8u * (kB + 12 + s); };
+    auto v_clean = [&](int s) { return bars + 8u * (kB + 14 + s); };  // documents: V slot s has no padding rows left
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBarOffset + 8 * (kB + 14 + kKvSlots));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* item_info = reinterpret_cast<volatile int*>(tmem_slot + 2);  // two entries
+    static_assert(8 * (kB + 14 + kKvSlots) + 16 <= 256, "barrier block");
+
+    const uint32_t warp = warp_id();
+    const uint32_t lane = lane_id();
+    const bool documents = p.rows != nullptr;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kKvSlots; ++s) {
+            mbar_init(kv_full(s), 1);
+            mbar_init(kv_empty(s), 1);
+            mbar_init(v_clean(s), 1);
+        }
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        for (int g = 0; g < 2; ++g) {
+            mbar_init(s_full(g), 1);
+            mbar_init(p_ready(g), 4);
+            mbar_init(o_final(g), 1);
+            mbar_init(o_empty(g), 4);
+            mbar_init(item_full(g), 1);
+            mbar_init(item_empty(g), documents ? 10 : 9);  // the MMA thread, eight softmax warps, warp 10
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 9) {
+        tmem_alloc<1>(smem_u32(tmem_slot), kTmemCols);
+        tmem_relinquish<1>();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp >= 8) {
+        setmaxnreg_dec<kRegsControl>();
+        if (warp == 8) {
+            // ---------------- TMA producer and scheduler (one thread) ----------------
+            if (lane == 0) {
+                tma_prefetch_desc(&map_q);
+                tma_prefetch_desc(&map_k);
+                tma_prefetch_desc(&map_v);
+                int slot = 0;
+                uint32_t phase = 0;
+                int issued = 0;
+                int items = 0;    // published
+                int loaded = 0;   // of them with keys, so with Q loaded
+                bool ok = true;
+                int w = static_cast<int>(blockIdx.x);
+                for (int it_slot = 0;; it_slot ^= 1) {
+                    if (items > 0) {
+                        w = p.next_item != nullptr ? static_cast<int>(gridDim.x) + atomicAdd(p.next_item, 1)
+                                                   : w + static_cast<int>(gridDim.x);
+                    }
+                    const int wi = w < p.num_items ? w : -1;
+                    // Entry it_slot was last used two items ago.
+                    if (items >= 2 &&
+                        !mbar_wait(item_empty(it_slot), static_cast<uint32_t>((items - 2) >> 1) & 1u,
+                                   kFaultProducerWait, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    item_info[it_slot] = wi;
+                    mbar_arrive(item_full(it_slot));
+                    if (wi < 0) break;
+                    ++items;
+                    const Item it = make_item(wi, p);
+                    if (it.jb >= it.je) continue;
+                    // Q of the previous item is free once all its S MMAs have completed.
+                    if (loaded > 0 &&
+                        !mbar_wait(q_empty, static_cast<uint32_t>(loaded - 1) & 1u, kFaultProducerWait, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const int ntiles = it.q0 + kBlockQ < p.seq_q ? 2 : 1;
+                    mbar_arrive_expect_tx(q_full, ntiles * C::kTileBytes);
+                    for (int g = 0; g < ntiles; ++g)
+                        for (int x = 0; x < C::kBoxes; ++x)
+                            tma_load_4d(base + C::kQOffset + g * C::kTileBytes + x * 16384, &map_q, q_full, x * 64,
+                                        it.q0 + g * kBlockQ, it.head, it.batch);
+                    ++loaded;
+                    for (int j = it.jb; j < it.je && ok; ++j) {
+                        for (int which = 0; which < 2; ++which) {  // K then V
+                            if (!mbar_wait(kv_empty(slot), phase ^ 1u, kFaultProducerWait, abort_flag)) {
+                                ok = false;
+                                break;
+                            }
+                            const uint32_t dst = base + C::kKvOffset + slot * C::kTileBytes;
+                            mbar_arrive_expect_tx(kv_full(slot), C::kTileBytes);
+                            for (int x = 0; x < C::kBoxes; ++x)
+                                tma_load_4d(dst + x * 16384, which == 0 ? &map_k : &map_v, kv_full(slot), x * 64,
+                                            j * kBlockKV, it.head_kv, it.batch);
+                            ++issued;
+                            if (++slot == kKvSlots) {
+                                slot = 0;
+                                phase ^= 1u;
+                            }
+                        }
+                    }
+                    if (!ok) break;
+                }
+                if (!ok) {
+                    // Let every issued load land before the CTA may exit: the last Q load
+                    // and the last (up to kKvSlots) K/V loads.
+                    if (loaded > 0) mbar_wait(q_full, static_cast<uint32_t>(loaded - 1) & 1u, kFaultDrainWait, nullptr);
+                    int s = slot;
+                    uint32_t ph = phase;
+                    for (int i = 0; i < min(issued, kKvSlots); ++i) {
+                        if (--s < 0) {
+                            s = kKvSlots - 1;
+                            ph ^= 1u;
+                        }
+                        mbar_wait(kv_full(s), ph, kFaultDrainWait, nullptr);
+                    }
+                }
+            }
+            __syncwarp();
+        } else if (warp == 9) {
+            // ---------------- MMA issuer (one thread) ----------------
+            if (lane == 0) {
+                const uint32_t q_addr[2] = {base + C::kQOffset, base + C::kQOffset + C::kTileBytes};
+                auto kv_addr = [&](int slot) { return base + C::kKvOffset + slot * C::kTileBytes; };
+                const uint64_t dq[2] = {sw128_desc(q_addr[0], 16, 1024), sw128_desc(q_addr[1], 16, 1024)};
+                auto issue_s = [&](int g, uint32_t k_addr) {
+                    const uint64_t dk = sw128_desc(k_addr, 16, 1024);
+#pragma unroll
+                    for (int kk = 0; kk < kDPad / 16; ++kk) {
+                        const uint64_t off = static_cast<uint64_t>(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
+                        mma_f16_ss<1>(tmem + 256u * g, dq[g] + off, dk + off, C::kIdescS, kk > 0 ? 1u : 0u);
+                    }
+                    mma_commit(s_full(g));
+                };
+                auto issue_pv = [&](int g, uint32_t v_addr, bool first) {
+                    const uint64_t dv = sw128_desc(v_addr, 16384, 1024);
+#pragma unroll
+                    for (int kk = 0; kk < kBlockKV / 16; ++kk)
+                        mma_f16_ts(tmem + 256u * g + 128u, tmem + 256u * g + kk * 8,
+                                   dv + static_cast<uint64_t>((kk * 2048) >> 4), C::kIdescO, (!first || kk > 0) ? 1u : 0u);
+                };
+                uint32_t pr_phase[2] = {0, 0};
+                int done[2] = {0, 0};  // items in which tile g has produced an output
+                int kv_base = 0;       // K/V loads of the previous items
+                int loaded = 0;
+                bool ok = true;
+                auto o_free = [&](int g) {
+                    return done[g] == 0 ||
+                           mbar_wait(o_empty(g), static_cast<uint32_t>(done[g] - 1) & 1u, kFaultAttnWait, abort_flag);
+                };
+                for (int items = 0, it_slot = 0; ok; it_slot ^= 1, ++items) {
+                    if (!mbar_wait(item_full(it_slot), static_cast<uint32_t>(items >> 1) & 1u, kFaultAttnWait, abort_flag))
+                        break;
+                    const int wi = item_info[it_slot];
+                    mbar_arrive(item_empty(it_slot));
+                    if (wi < 0) break;
+                    const Item it = make_item(wi, p);
+                    if (it.jb >= it.je) continue;
+                    auto slot_of = [&](int load) { return (kv_base + load) % kKvSlots; };
+                    auto phase_of = [&](int load) { return static_cast<uint32_t>((kv_base + load) / kKvSlots) & 1u; };
+                    auto act = [&](int g, int j) { return j >= it.b0[g] && j < it.b1[g]; };
+                    auto wait_k = [&](int j) {
+                        return mbar_wait(kv_full(slot_of(2 * (j - it.jb))), phase_of(2 * (j - it.jb)), kFaultAttnWait, abort_flag);
+                    };
+                    auto wait_v = [&](int j) {
+                        const int load = 2 * (j - it.jb) + 1;
+                        return mbar_wait(documents ? v_clean(slot_of(load)) : kv_full(slot_of(load)), phase_of(load),
+                                         kFaultAttnWait, abort_flag);
+                    };
+                    // PV of tile g, block j, once its probabilities are there.
+                    auto pv = [&](int g, int j) {
+                        if (!mbar_wait(p_ready(g), pr_phase[g], kFaultAttnWait, abort_flag)) return false;
+                        pr_phase[g] ^= 1u;
+                        const bool first = j == it.b0[g];
+                        if (first && !o_free(g)) return false;
+                        tc_fence_after();
+                        issue_pv(g, kv_addr(slot_of(2 * (j - it.jb) + 1)), first);
+                        if (j == it.b1[g] - 1) mma_commit(o_final(g));
+                        return true;
+                    };
+                    ok = mbar_wait(q_full, static_cast<uint32_t>(loaded) & 1u, kFaultAttnWait, abort_flag);
+                    ++loaded;
+                    if (ok && act(0, it.jb)) {
+                        ok = wait_k(it.jb);
+                        tc_fence_after();
+                        if (ok) issue_s(0, kv_addr(slot_of(0)));
+                    }
+                    for (int j = it.jb; j < it.je && ok; ++j) {
+                        ok = false;
+                        const int load = 2 * (j - it.jb);
+                        // PV1 of the block before, then its V is free.
+                        if (j > it.jb) {
+                            if (act(1, j - 1) && !pv(1, j - 1)) break;
+                            mma_commit(kv_empty(slot_of(load - 1)));
+                        }
+                        // S1, then K is free. K was waited for before S0, where tile 0 works on it.
+                        if (!act(0, j) && !wait_k(j)) break;
+                        if (act(1, j)) {
+                            tc_fence_after();
+                            issue_s(1, kv_addr(slot_of(load)));
+                        }
+                        mma_commit(kv_empty(slot_of(load)));
+                        if (j == it.je - 1) mma_commit(q_empty);
+                        // PV0 and the next block's S0, back to back.
+                        if (!wait_v(j)) break;
+                        const bool next = act(0, j + 1);
+                        if (next && !wait_k(j + 1)) break;
+                        if (act(0, j) && !pv(0, j)) break;
+                        if (next) {
+                            tc_fence_after();
+                            issue_s(0, kv_addr(slot_of(load + 2)));
+                        }
+                        if (j == it.je - 1) {
+                            if (act(1, j) && !pv(1, j)) break;
+                            mma_commit(kv_empty(slot_of(load + 1)));
+                        }
+                        ok = true;
+                    }
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+                        if (it.b0[g] < it.b1[g]) ++done[g];
+                    kv_base += 2 * (it.je - it.jb);
+                }
+            }
+            __syncwarp();
+        } else if (warp == 10 && documents) {
+            // ---------------- padding rows of V become 0 ----------------
+            int kv_base = 0;
+            bool ok = true;
+            for (int items = 0, it_slot = 0; ok; it_slot ^= 1, ++items) {
+                if (!mbar_wait_warp(item_full(it_slot), static_cast<uint32_t>(items >> 1) & 1u, kFaultAttnWait, abort_flag))
+                    break;
+                const int wi = item_info[it_slot];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(item_empty(it_slot));
+                if (wi < 0) break;
+                const Item it = make_item(wi, p);
+                for (int j = it.jb; j < it.je; ++j) {
+                    const int load = kv_base + 2 * (j - it.jb) + 1;
+                    const int slot = load % kKvSlots;
+                    if (!mbar_wait_warp(kv_full(slot), static_cast<uint32_t>(load / kKvSlots) & 1u, kFaultAttnWait, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    // Documents have seq_kv = seq_q: key block j holds the rows of tile j.
+                    if (__ldg(p.tiles + (static_cast<long long>(it.batch) * 2 * p.pairs + j)).z != 0) {
+                        const uint32_t tile = base + C::kKvOffset + slot * C::kTileBytes;
+#pragma unroll
+                        for (int i = 0; i < kBlockKV / 32; ++i) {
+                            const int row = i * 32 + static_cast<int>(lane);
+                            const int key = j * kBlockKV + row;
+                            if (key >= p.seq_kv) continue;  // zero already
+                            const int2 r = __ldg(p.rows + (static_cast<long long>(it.batch) * p.seq_kv + key));
+                            if (r.x < r.y) continue;
+                            for (int x = 0; x < C::kBoxes; ++x)
+#pragma unroll
+                                for (int c = 0; c < 8; ++c) st_shared_v4(tile + x * 16384 + row * 128 + c * 16, 0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(v_clean(slot));
+                }
+                kv_base += 2 * (it.je - it.jb);
+            }
+        }
+    } else {
+        setmaxnreg_inc<kRegsSoftmax>();
+        // ---------------- softmax warpgroups (warps 0-3: tile 0, 4-7: tile 1) ----------------
+        const int g = static_cast<int>(warp >> 2);
+        const uint32_t quarter = warp & 3u;
+        const int row_in_tile = static_cast<int>(quarter * 32 + lane);
+        const uint32_t lane_bits = (quarter * 32u) << 16;
+        const uint32_t s_addr = tmem + lane_bits + 256u * g;
+        const uint32_t o_addr = s_addr + 128u;
+        uint32_t sf_phase = 0;  // s_full(g) completions seen
+        uint32_t of_phase = 0;  // o_final(g) completions seen
+        bool ok = true;
+        for (int it_slot = 0, items = 0; ok; it_slot ^= 1, ++items) {
+            if (!mbar_wait_warp(item_full(it_slot), static_cast<uint32_t>(items >> 1) & 1u, kFaultAttnWait, abort_flag))
+                break;
+            const int wi = item_info[it_slot];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(item_empty(it_slot));
+            if (wi < 0) break;
+            const Item it = make_item(wi, p);
+            const int q_row = it.q0 + g * kBlockQ + row_in_tile;
+            if (it.q0 + g * kBlockQ >= p.seq_q) continue;
+            const int pos = q_row + p.seq_kv - p.seq_q;
+            // The row's keys [lo, hi). Rows past the end take every key, so that they never
+            // make their warp compute a mask; they are not stored.
+            int lo = 0, hi = INT_MAX;
+            if (q_row < p.seq_q) {
+                lo = 0;
+                hi = p.seq_kv;
+                if (documents) {
+                    const int2 r = __ldg(p.rows + (static_cast<long long>(it.batch) * p.seq_q + q_row));
+                    lo = r.x;
+                    hi = p.causal ? min(r.y, pos + 1) : r.y;
+                } else if (p.causal) {
+                    hi = pos + 1;
+                    if (p.prefix != nullptr) hi = min(max(hi, __ldg(p.prefix + it.batch)), p.seq_kv);
+                }
+            }
+            float slope = 0.0f;
+            if (kChange && p.slopes != nullptr) slope = __ldg(p.slopes + it.head) * kLog2e;
+            float m_run = -INFINITY;  // reference point, log2 units
+            float l_run = 0.0f;       // running sum of 2^(x - m_run + kLift)
+            const int b0 = it.b0[g], b1 = it.b1[g];
+            for (int j = b0; j < b1; ++j) {
+                if (!mbar_wait_warp(s_full(g), sf_phase, kFaultAttnWait, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                sf_phase ^= 1u;
+                tc_fence_after();
+                const int kv0 = j * kBlockKV;
+                const bool need_mask = __any_sync(0xffffffffu, lo > kv0 || hi < kv0 + kBlockKV);
+                uint32_t r[128];
+                attn::load_row128(s_addr, r);
+                // Scores in log2 units are r * c; with a change of scores r already is.
+                float c = p.scale_log2;
+                if constexpr (kChange) {
+                    if (p.softcap > 0.0f) {
+                        cap_row(r, p.scale / p.softcap, p.softcap);
+                        c = 1.0f;
+                    }
+                    // A non-positive scale (the max of r * c is not that of r) is applied here too.
+                    if (p.slopes != nullptr || p.softcap == 0.0f) bias_row(r, c, slope, pos - kv0);
+                    c = 1.0f;
+                }
+                if (need_mask) mask_row(r, lo - kv0, hi - kv0);
+                const float m_blk = attn::row_max128(r) * c;
+                // The point moves only when the max grows by more than 8, so P <= 2^(8 + kLift).
+                const float m_new = fmaxf(m_run, m_blk);
+                const float m_use = m_new > m_run + 8.0f ? m_new : m_run;
+                const float alpha = m_use == m_run ? 1.0f : ex2(m_run - m_use);
+                const float e_sum = exp_store<kBf16>(s_addr, r, c, kLift - (m_use == -INFINITY ? 0.0f : m_use));
+                // tcgen05.ld/st are warp-collective: the rescale runs for the whole warp
+                // when any of its rows needs it.
+                if (j > b0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                    // PV_{j-1} has completed (in-order tcgen05).
+#pragma unroll
+                    for (int x = 0; x < kDPad / 16; ++x) {
+                        uint32_t o[16];
+                        tmem_ld_32x32b_x16(o_addr + 16 * x, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tmem_st_32x32b_x16(o_addr + 16 * x, o);
+                    }
+                }
+                l_run = l_run * alpha + e_sum;
+                m_run = m_use;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready(g));
+            }
+            if (!ok) break;
+            const bool row_ok = q_row < p.seq_q;
+            uint16_t* orow = p.out + it.batch * p.out_b + it.head * p.out_h + static_cast<long long>(q_row) * p.out_s;
+            if (b0 >= b1) {
+                // No row of the tile sees a key: nothing was multiplied.
+                if (row_ok) {
+                    for (int col = 0; col < p.head_dim; ++col) orow[col] = 0;
+                }
+                continue;
+            }
+            if (!mbar_wait_warp(o_final(g), of_phase, kFaultAttnWait, abort_flag)) {
+                ok = false;
+                break;
+            }
+            of_phase ^= 1u;
+            tc_fence_after();
+            const float inv_l = l_run > 0.0f ? __frcp_rn(l_run) : 0.0f;  // a row without a key is 0
+#pragma unroll
+            for (int x = 0; x < kDPad / 32; ++x) {
+                uint32_t r[32];
+                tmem_ld_32x32b_x32(o_addr + 32 * x, r);
+                tmem_wait_ld();
+                if (x == kDPad / 32 - 1) {
+                    // O_g is in registers: the next item's first PV may overwrite it.
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(o_empty(g));
+                }
+                if (row_ok) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int col = 32 * x + 8 * q;
+                        if (col < p.head_dim) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                w[i] = pack2<kBf16>(__uint_as_float(r[8 * q + 2 * i]) * inv_l,
+                                                    __uint_as_float(r[8 * q + 2 * i + 1]) * inv_l);
+                            if (p.out_vec) {
+                                *reinterpret_cast<uint4*>(orow + col) = make_uint4(w[0], w[1], w[2], w[3]);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    orow[col + 2 * i] = static_cast<uint16_t>(w[i]);
+                                    orow[col + 2 * i + 1] = static_cast<uint16_t>(w[i] >> 16);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc<1>(tmem, kTmemCols);
+    }
+}
+
+// ---- host -------------------------------------------------------------------------------
+
+// A [batch, heads, rows, dim] operand and its strides in elements (dim: 1).
+struct View {
+    const void* p;
+    long long b, h, s;
+};
+
+// Rows TMA cannot address, as a contiguous [batch, heads, rows, dim] copy.
+__global__ void gather_rows_kernel(const uint16_t* src, long long sb, long long sh, long long ss, uint16_t* dst, int heads,
+                                   int rows, int dim, long long count) {
+    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < count;
+         i += static_cast<long long>(gridDim.x) * blockDim.x) {
+        const int d = static_cast<int>(i % dim);
+        const long long row = i / dim;
+        const int s = static_cast<int>(row % rows);
+        const long long bh = row / rows;
+        dst[i] = src[(bh / heads) * sb + (bh % heads) * sh + s * ss + d];
+    }
+}
+
+template <int kDPad, bool kBf16, bool kChange>
+cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int device, int grid,
+                   cudaStream_t stream) {
+    using C = Cfg<kDPad, kBf16>;
+    static std::atomic<bool> configured[host::kMaxDevices];
+    auto kernel = masked_kernel<kDPad, kBf16, kChange>;
+    if (!configured[device].load(std::memory_order_acquire)) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+        if (e != cudaSuccess) return e;
+        configured[device].store(true, std::memory_order_release);
+    }
+    kernel<<<static_cast<unsigned>(grid), kThreads, C::kSmemBytes, stream>>>(mq, mk, mv, p);
+    return cudaGetLastError();
+}
+
+// Strides of a dimension of size 1 are never used; the others have to be positive.
+inline bool strides_ok(const View& v, int batch, int heads, int rows) {
+    return (batch == 1 || v.b > 0) && (heads == 1 || v.h > 0) && (rows == 1 || v.s > 0);
+}
+
+// Elements from the first to behind the last one (saturating far above any allocation).
+inline bool extent_of(const View& v, int batch, int heads, int rows, int dim, size_t* elems) {
+    const __int128 e = static_cast<__int128>(batch - 1) * (batch > 1 ? v.b : 0) +
+                       static_cast<__int128>(heads - 1) * (heads > 1 ? v.h : 0) +
+                       static_cast<__int128>(rows - 1) * (rows > 1 ? v.s : 0) + dim;
+    if (e > (static_cast<__int128>(1) << 60)) return false;
+    *elems = static_cast<size_t>(e);
+    return true;
+}
+
+// No two (batch, head, row) of an output share an element: taken from the smallest
+// stride up, each dimension steps over all that the smaller ones reach.
+inline bool rows_apart(const View& v, int batch, int heads, int rows, int dim) {
+    long long st[3] = {v.b, v.h, v.s};
+    int n[3] = {batch, heads, rows};
+    for (int i = 0; i < 2; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (st[j] < st[i]) {
+                const long long a = st[i];
+                st[i] = st[j];
+                st[j] = a;
+                const int c = n[i];
+                n[i] = n[j];
+                n[j] = c;
+            }
+    __int128 reach = dim;
+    for (int i = 0; i < 3; ++i) {
+        if (n[i] == 1) continue;
+        if (st[i] < reach) return false;
+        reach += static_cast<__int128>(n[i] - 1) * st[i];
+    }
+    return true;
+}
+
+inline bool make_map(CUtensorMap* map, const View& v, int batch, int heads, int rows, int dim) {
+    const uint64_t dims[4] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(rows), static_cast<uint64_t>(heads),
+                              static_cast<uint64_t>(batch)};
+    // A dimension of size 1 gets any stride that the encoding takes.
+    const uint64_t strides[3] = {rows > 1 ? static_cast<uint64_t>(v.s) * 2 : 256, heads > 1 ? static_cast<uint64_t>(v.h) * 2 : 256,
+                                 batch > 1 ? static_cast<uint64_t>(v.b) * 2 : 256};
+    const uint32_t box[4] = {64, 128, 1, 1};
+    return host::make_map_f16(map, v.p, 4, dims, strides, box);
+}
+
+inline cudaError_t masked_entry(bool bf16, const void* q, const void* k, const void* v, void* out, const int64_t* strides,
+                                int batch, int heads, int heads_kv, int seq_q, int seq_kv, int dim, float scale, float softcap,
+                                const float* slopes, const int* doc_ids, const int* prefix, int causal, cudaStream_t stream) {
+    if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || batch <= 0 || heads <= 0 || heads_kv <= 0 ||
+        heads % heads_kv != 0 || seq_q <= 0 || seq_kv <= 0 || (dim != 16 && dim != 32 && dim != 64 && dim != 128) ||
+        (causal != 0 && causal != 1) || !(scale - scale == 0.0f) || !(softcap >= 0.0f) || !(softcap - softcap == 0.0f) ||
+        (doc_ids != nullptr && (prefix != nullptr || seq_q != seq_kv)) || (prefix != nullptr && causal == 0)) {
+        return cudaErrorInvalidValue;
+    }
+    const long long bh = static_cast<long long>(batch) * heads;
+    const int pairs = static_cast<int>((seq_q + 255LL) / 256);
+    // Positions and the last tile's ends stay below 2^31.
+    if (bh * pairs > INT_MAX / 2 || seq_q > INT_MAX - 512 || seq_kv > INT_MAX - 512) return cudaErrorInvalidValue;
+    const long long dq = static_cast<long long>(seq_q) * dim, dk = static_cast<long long>(seq_kv) * dim;
+    View vq{q, heads * dq, dq, dim}, vk{k, heads_kv * dk, dk, dim}, vv{v, heads_kv * dk, dk, dim}, vo{out, heads * dq, dq, dim};
+    if (strides != nullptr) {
+        View* views[4] = {&vq, &vk, &vv, &vo};
+        for (int i = 0; i < 4; ++i) {
+            views[i]->b = strides[3 * i];
+            views[i]->h = strides[3 * i + 1];
+            views[i]->s = strides[3 * i + 2];
+        }
+    }
+    size_t eq, ek, ev, eo;
+    if (!strides_ok(vq, batch, heads, seq_q) || !strides_ok(vk, batch, heads_kv, seq_kv) || !strides_ok(vv, batch, heads_kv, seq_kv) ||
+        !strides_ok(vo, batch, heads, seq_q) || !extent_of(vq, batch, heads, seq_q, dim, &eq) ||
+        !extent_of(vk, batch, heads_kv, seq_kv, dim, &ek) || !extent_of(vv, batch, heads_kv, seq_kv, dim, &ev) ||
+        !extent_of(vo, batch, heads, seq_q, dim, &eo) || !rows_apart(vo, batch, heads, seq_q, dim)) {
+        return cudaErrorInvalidValue;
+    }
+    if (host::ranges_overlap(out, eo * 2, q, eq * 2) || host::ranges_overlap(out, eo * 2, k, ek * 2) ||
+        host::ranges_overlap(out, eo * 2, v, ev * 2) ||
+        (doc_ids != nullptr && host::ranges_overlap(out, eo * 2, doc_ids, static_cast<size_t>(batch) * seq_q * 4)) ||
+        (prefix != nullptr && host::ranges_overlap(out, eo * 2, prefix, static_cast<size_t>(batch) * 4)) ||
+        (slopes != nullptr && host::ranges_overlap(out, eo * 2, slopes, static_cast<size_t>(heads) * 4))) {
+        return cudaErrorInvalidValue;
+    }
+    int device = 0, sm_count = 0;
+    cudaError_t err = host::current_device(&device, &sm_count);
+    if (err != cudaSuccess) return err;
+    static_cast<void>(cudaGetLastError());
+
+    Params p{};
+    p.seq_q = seq_q;
+    p.seq_kv = seq_kv;
+    p.head_dim = dim;
+    p.pairs = pairs;
+    p.heads_q = heads;
+    p.heads_kv = heads_kv;
+    p.group = heads / heads_kv;
+    p.num_items = static_cast<int>(bh * pairs);
+    p.causal = causal;
+    p.prefix = prefix;
+    p.scale = scale;
+    p.scale_log2 = scale * kLog2e;
+    p.softcap = softcap;
+    p.slopes = slopes;
+    p.out = static_cast<uint16_t*>(out);
+    p.out_b = vo.b;
+    p.out_h = vo.h;
+    p.out_s = vo.s;
+    p.out_vec = (reinterpret_cast<uintptr_t>(out) & 15u) == 0 && (batch == 1 || vo.b % 8 == 0) && (heads == 1 || vo.h % 8 == 0) &&
+                (seq_q == 1 || vo.s % 8 == 0);
+    const int grid = p.num_items < sm_count ? p.num_items : sm_count;
+
+    // One scratch buffer: the item counter, the documents' tiles and rows, copies of
+    // operands whose rows TMA cannot address.
+    const bool counted = p.num_items > grid;
+    const size_t n_tiles = static_cast<size_t>(batch) * 2 * pairs;
+    View* in[3] = {&vq, &vk, &vv};
+    const int in_heads[3] = {heads, heads_kv, heads_kv}, in_rows[3] = {seq_q, seq_kv, seq_kv};
+    size_t bytes = counted ? 256 : 0, tiles_at = 0, rows_at = 0, copy_at[3] = {0, 0, 0};
+    auto take = [&](size_t n) {
+        const size_t at = bytes;
+        bytes += (n + 255) / 256 * 256;
+        return at;
+    };
+    if (doc_ids != nullptr) {
+        tiles_at = take(n_tiles * sizeof(int4));
+        rows_at = take(static_cast<size_t>(batch) * seq_q * sizeof(int2));
+    }
+    bool copied[3];
+    for (int i = 0; i < 3; ++i) {
+        copied[i] = (reinterpret_cast<uintptr_t>(in[i]->p) & 15u) != 0 || (batch > 1 && in[i]->b % 8 != 0) ||
+                    (in_heads[i] > 1 && in[i]->h % 8 != 0) || (in_rows[i] > 1 && in[i]->s % 8 != 0);
+        if (copied[i]) copy_at[i] = take(static_cast<size_t>(batch) * in_heads[i] * in_rows[i] * dim * 2);
+    }
+    uint8_t* scratch = nullptr;
+    if (bytes > 0) {
+        err = host::scratch_alloc(reinterpret_cast<void**>(&scratch), bytes, device, stream);
+        if (err != cudaSuccess) return err;
+    }
+    for (int i = 0; i < 3; ++i) {
+        if (!copied[i]) continue;
+        const long long rows = in_rows[i], h = in_heads[i];
+        uint16_t* dst = reinterpret_cast<uint16_t*>(scratch + copy_at[i]);
+        gather_rows_kernel<<<1024, 256, 0, stream>>>(static_cast<const uint16_t*>(in[i]->p), in[i]->b, in[i]->h, in[i]->s, dst,
+                                                     in_heads[i], in_rows[i], dim, batch * h * rows * dim);
+        *in[i] = View{dst, h * rows * dim, rows * dim, dim};
+    }
+    if (counted) p.next_item = reinterpret_cast<int*>(scratch);
+    if (doc_ids != nullptr) {
+        p.tiles = reinterpret_cast<const int4*>(scratch + tiles_at);
+        p.rows = reinterpret_cast<const int2*>(scratch + rows_at);
+        runs_kernel<<<static_cast<unsigned>(batch), kRunThreads, 0, stream>>>(
+            doc_ids, seq_q, 2 * pairs, causal, reinterpret_cast<int2*>(scratch + rows_at),
+            reinterpret_cast<int4*>(scratch + tiles_at), p.next_item);
+    } else if (counted) {
+        err = cudaMemsetAsync(scratch, 0, sizeof(int), stream);
+    }
+    CUtensorMap mq, mk, mv;
+    if (err == cudaSuccess && !(make_map(&mq, vq, batch, heads, seq_q, dim) && make_map(&mk, vk, batch, heads_kv, seq_kv, dim) &&
+                                make_map(&mv, vv, batch, heads_kv, seq_kv, dim))) {
+        err = cudaErrorInvalidValue;
+    }
+    if (err == cudaSuccess) {
+        const bool change = softcap > 0.0f || slopes != nullptr || !(scale > 0.0f);
+        switch ((dim == 128 ? 4 : 0) + (bf16 ? 2 : 0) + (change ? 1 : 0)) {
+            case 0: err = launch<64, false, false>(mq, mk, mv, p, device, grid, stream); break;
+            case 1: err = launch<64, false, true>(mq, mk, mv, p, device, grid, stream); break;
+            case 2: err = launch<64, true, false>(mq, mk, mv, p, device, grid, stream); break;
+            case 3: err = launch<64, true, true>(mq, mk, mv, p, device, grid, stream); break;
+            case 4: err = launch<128, false, false>(mq, mk, mv, p, device, grid, stream); break;
+            case 5: err = launch<128, false, true>(mq, mk, mv, p, device, grid, stream); break;
+            case 6: err = launch<128, true, false>(mq, mk, mv, p, device, grid, stream); break;
+            default: err = launch<128, true, true>(mq, mk, mv, p, device, grid, stream); break;
+        }
+    }
+    if (scratch != nullptr) cudaFreeAsync(scratch, stream);
+    if (err != cudaSuccess) return err;
+    return cudaGetLastError();
+}
+
+}  // namespace masked
+}  // namespace tk

@@ -1,0 +1,500 @@
+// kvcache.cuh — a paged key/value cache held in 8 bits: the plan that gives new
+// tokens their places (block tables, slot maps) and the append that quantises
+// them into it.
+//
+// A cache has n_pages pages of `page_size` token places. Page p holds, for each
+// key/value head h, a [page_size, head_dim] tile of e4m3 bytes, contiguous, and one
+// FP32 scale: a place stands for scale[p, h] * e4m3. Slot s is place s % page_size
+// of page s / page_size (64 bits: a cache may hold more than 2^31 places x heads).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <climits>
+#include <cstdint>
+
+#include "tk_host.cuh"
+#include "tk_ptx.cuh"
+
+namespace tk {
+namespace kv {
+
+// ---------------------------------------------------------------------------
+// e4m3
+// ---------------------------------------------------------------------------
+
+// Two FP32 values to two e4m3 bytes (lo in the low byte), nearest even, saturating
+// at 448; NaN stays NaN.
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Two e4m3 bytes to binary16, exact (subnormals and NaN included).
+__device__ __forceinline__ uint32_t from_e4m3x2(uint32_t two) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(two)));
+    return r;
+}
+
+__device__ __forceinline__ float2 half2_bits_to_float2(uint32_t bits) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&bits));
+}
+
+__device__ __forceinline__ float2 bf162_bits_to_float2(uint32_t bits) {
+    return make_float2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xffff0000u));
+}
+
+template <bool kBf16>
+__device__ __forceinline__ float2 pair_to_float2(uint32_t bits) {
+    return kBf16 ? bf162_bits_to_float2(bits) : half2_bits_to_float2(bits);
+}
+
+// ---------------------------------------------------------------------------
+// Plan
+// ---------------------------------------------------------------------------
+
+constexpr int kPlanThreads = 1024;
+
+struct PlanParams {
+    const int* cached;   // tokens each request holds in the cache
+    const int* fresh;    // tokens it adds now
+    int n_requests;
+    int page;
+    int* table;          // [n_requests, width]
+    int width;
+    const int* free_pages;
+    int free_capacity;
+    const int* n_free;
+    int* lens_out;       // may be `cached`
+    int* seq_lens;
+    int* starts;         // [n_requests + 1]
+    int64_t* slots;    // [max_tokens]
+    int max_tokens;
+    int* n_free_out;     // may be `n_free`
+};
+
+// Inclusive sum over the CTA's threads (1024), in thread order; `total` gets the sum
+// of all. `warp_sums`: 32 values of shared memory.
+__device__ __forceinline__ long long block_scan(long long v, long long* warp_sums, long long& total) {
+    const int lane = static_cast<int>(lane_id());
+    const int warp = static_cast<int>(threadIdx.x >> 5);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += up;
+    }
+    if (lane == 31) warp_sums[warp] = v;
+    __syncthreads();
+    long long w = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += up;
+    }
+    total = __shfl_sync(0xffffffffu, w, 31);
+    const long long before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+    __syncthreads();
+    return warp > 0 ? v + before : v;
+}
+
+// First index in ends[0, n) (ascending) with ends[i] > x; n if none.
+__device__ __forceinline__ int upper_bound(const int* ends, int n, int x) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (ends[mid] > x) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
+
+// One cluster of CTAs. Requests are taken 1024 at a time: every CTA computes the two
+// prefix sums (new tokens, pages needed) of the same 1024 requests for itself, and
+// the CTAs share out the slots and table entries. Only CTA 0 writes the lengths; the
+// cluster barrier before that lets lens_out be the array the others have read.
+//
+//   need_r  = ceil((c_r + n_r) / page) - ceil(c_r / page)
+//   taken_r = n_r > 0, the row and the slots are wide enough, and need_r = 0 or
+//             need_0 + .. + need_r <= n_free
+//   page k of the call = free_pages[n_free - 1 - k]
+//
+// What bounds it: one launch and the chain lengths -> sums -> entries; the bytes are
+// a few MB at most (8 per slot).
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
+    __shared__ long long warp_sums[32];
+    __shared__ int s_ends[kPlanThreads];   // running new tokens, clamped to INT_MAX
+    __shared__ int s_upto[kPlanThreads];   // running pages needed, clamped
+    __shared__ int s_cached[kPlanThreads];
+    __shared__ int s_taken[kPlanThreads];
+    __shared__ int s_used;
+    const int tid = static_cast<int>(threadIdx.x);
+    const int rank = static_cast<int>(blockIdx.x);
+    const int ctas = static_cast<int>(gridDim.x);
+    int n_free = *p.n_free;
+    n_free = n_free < 0 ? 0 : (n_free > p.free_capacity ? p.free_capacity : n_free);
+    if (tid == 0) s_used = 0;
+    long long tokens = 0, pages = 0;  // sums over the earlier requests
+    for (int r0 = 0; r0 < p.n_requests; r0 += kPlanThreads) {
+        const int r = r0 + tid;
+        int c = 0, n = 0;
+        if (r < p.n_requests) {
+            c = max(p.cached[r], 0);
+            n = max(p.fresh[r], 0);
+        }
+        long long sum;
+        const long long end = tokens + block_scan(n, warp_sums, sum);
+        const long long whole = static_cast<long long>(c) + n;
+        const int have = static_cast<int>((static_cast<long long>(c) + p.page - 1) / p.page);
+        const bool fits = n > 0 && whole <= static_cast<long long>(p.width) * p.page && end <= p.max_tokens;
+        const int need = fits ? static_cast<int>((whole + p.page - 1) / p.page) - have : 0;
+        long long page_sum;
+        const long long upto = pages + block_scan(need, warp_sums, page_sum);
+        const bool taken = fits && (need == 0 || upto <= n_free);
+        s_ends[tid] = static_cast<int>(min(end, static_cast<long long>(INT_MAX)));
+        s_upto[tid] = static_cast<int>(min(upto, static_cast<long long>(INT_MAX)));
+        s_cached[tid] = c;
+        s_taken[tid] = taken ? 1 : 0;
+        if (taken && need > 0) atomicMax(&s_used, static_cast<int>(upto));
+        if (ctas > 1) cluster_sync(); else __syncthreads();
+        if (rank == 0 && r < p.n_requests) {
+            p.lens_out[r] = taken ? static_cast<int>(whole) : c;
+            p.seq_lens[r] = taken ? static_cast<int>(whole) : 0;
+            p.starts[r] = static_cast<int>(min(end - n, static_cast<long long>(INT_MAX)));
+        }
+        const int here = min(kPlanThreads, p.n_requests - r0);
+        // Table entries: page number k of the call goes to the request whose range holds it.
+        const int last_page = static_cast<int>(min(pages + page_sum, static_cast<long long>(n_free)));
+        for (long long k = pages + rank * kPlanThreads + tid; k < last_page; k += ctas * kPlanThreads) {
+            const int i = upper_bound(s_upto, here, static_cast<int>(k));
+            if (i >= here || !s_taken[i]) continue;
+            const int first = i > 0 ? s_upto[i - 1] : static_cast<int>(pages);
+            const int have_i = static_cast<int>((static_cast<long long>(s_cached[i]) + p.page - 1) / p.page);
+            p.table[static_cast<long long>(r0 + i) * p.width + have_i + (k - first)] = p.free_pages[n_free - 1 - k];
+        }
+        // Slots.
+        const int last_token = static_cast<int>(min(tokens + sum, static_cast<long long>(p.max_tokens)));
+        for (long long t = tokens + rank * kPlanThreads + tid; t < last_token; t += ctas * kPlanThreads) {
+            const int i = upper_bound(s_ends, here, static_cast<int>(t));
+            long long slot = -1;
+            if (i < here && s_taken[i]) {
+                const int first_token = i > 0 ? s_ends[i - 1] : static_cast<int>(tokens);
+                const int pos = s_cached[i] + static_cast<int>(t - first_token);
+                const int col = pos / p.page;
+                const int have_i = static_cast<int>((static_cast<long long>(s_cached[i]) + p.page - 1) / p.page);
+                const int first_page = i > 0 ? s_upto[i - 1] : static_cast<int>(pages);
+                const int page = col < have_i ? p.table[static_cast<long long>(r0 + i) * p.width + col]
+                                              : p.free_pages[n_free - 1 - (first_page + col - have_i)];
+                if (page >= 0) slot = static_cast<long long>(page) * p.page + pos % p.page;
+            }
+            p.slots[t] = slot;
+        }
+        tokens += sum;
+        pages += page_sum;
+        __syncthreads();  // the shared arrays are rewritten by the next 1024 requests
+    }
+    // Slots behind the last token stand for nothing.
+    for (long long t = tokens + rank * kPlanThreads + tid; t < p.max_tokens; t += ctas * kPlanThreads) p.slots[t] = -1;
+    // Every CTA has read *n_free before its first barrier; with no request there was none.
+    if (p.n_requests == 0) {
+        if (ctas > 1) cluster_sync(); else __syncthreads();
+    }
+    if (rank == 0 && tid == 0) {
+        p.starts[p.n_requests] = static_cast<int>(min(tokens, static_cast<long long>(INT_MAX)));
+        *p.n_free_out = n_free - s_used;
+    }
+}
+
+// One CTA up to this many slots and requests, above them the largest portable cluster.
+constexpr int kPlanOneCta = 4096;
+constexpr int kPlanCluster = 8;
+
+inline cudaError_t plan_entry(const int* cached, const int* fresh, int n_requests, int page, int* table, int width,
+                              const int* free_pages, int free_capacity, const int* n_free, int* lens_out, int* seq_lens,
+                              int* starts, int64_t* slots, int max_tokens, int* n_free_out, cudaStream_t stream) {
+    if (cached == nullptr || fresh == nullptr || n_free == nullptr || lens_out == nullptr || seq_lens == nullptr ||
+        starts == nullptr || n_free_out == nullptr || table == nullptr || n_requests < 0 || width <= 0 || page <= 0 ||
+        free_capacity < 0 || max_tokens < 0 || (free_pages == nullptr && free_capacity > 0) ||
+        (slots == nullptr && max_tokens > 0)) {
+        return cudaErrorInvalidValue;
+    }
+    const size_t bytes = static_cast<size_t>(n_requests) * 4;
+    const size_t table_bytes = bytes * static_cast<size_t>(width);
+    struct Range { const void* p; size_t n; };
+    const Range in[] = {{cached, bytes}, {fresh, bytes}, {free_pages, static_cast<size_t>(free_capacity) * 4}, {n_free, 4}};
+    const Range out[] = {{table, table_bytes}, {lens_out, bytes}, {seq_lens, bytes}, {starts, bytes + 4},
+                         {slots, static_cast<size_t>(max_tokens) * 8}, {n_free_out, 4}};
+    for (int i = 0; i < 6; ++i) {
+        for (int j = 0; j < 4; ++j) {
+            const bool in_place = (i == 1 && j == 0 && out[i].p == in[j].p) || (i == 5 && j == 3 && out[i].p == in[j].p);
+            if (!in_place && host::ranges_overlap(out[i].p, out[i].n, in[j].p, in[j].n)) return cudaErrorInvalidValue;
+        }
+        for (int j = i + 1; j < 6; ++j)
+            if (host::ranges_overlap(out[i].p, out[i].n, out[j].p, out[j].n)) return cudaErrorInvalidValue;
+    }
+    cudaError_t err = host::current_device(nullptr, nullptr);
+    if (err != cudaSuccess) return err;
+    static_cast<void>(cudaGetLastError());
+    PlanParams p{cached, fresh, n_requests, page, table, width, free_pages, free_capacity, n_free,
+                 lens_out, seq_lens, starts, slots, max_tokens, n_free_out};
+    const unsigned ctas = max_tokens <= kPlanOneCta && n_requests <= kPlanOneCta ? 1 : kPlanCluster;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kPlanThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    err = cudaLaunchKernelEx(&cfg, plan_kernel, p);
+    if (err != cudaSuccess) return err;
+    return cudaGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Append
+// ---------------------------------------------------------------------------
+
+constexpr int kAppendThreads = 128;
+constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kLeastExponent = -100;  // of a scale: what is smaller than 2^-109 becomes 0
+
+struct AppendParams {
+    const uint16_t* x[2];       // keys, values: [n_tokens, heads, dim], 16-bit
+    long long stride[2];        // elements from one token to the next
+    const int64_t* slots;
+    int n_tokens, heads;
+    uint8_t* cache[2];
+    float* scale[2];
+    long long n_pages;
+    int page, page_shift;       // a power of two, and which
+    int chunk;                  // tokens per CTA
+};
+
+// The smallest power of two s >= 2^kLeastExponent with amax <= 448 s (amax >= 0, finite).
+// 448 = 1.75 * 2^8. A power of two costs a floating format no precision, and moving a
+// page to a larger scale is then exact but for what falls below e4m3's last step.
+__device__ __forceinline__ float scale_for(float amax) {
+    const uint32_t bits = __float_as_uint(amax);
+    int e = static_cast<int>(bits >> 23) - 127;  // subnormals: -127, below the least anyway
+    e = e - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    e = max(e, kLeastExponent);
+    return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+// |x| of finite values; infinities and NaN do not set a scale (they are stored as 448
+// and NaN).
+__device__ __forceinline__ float finite_abs(float x) {
+    const float a = fabsf(x);
+    return a <= 3.402823466e38f ? a : 0.0f;
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// x / s; by the reciprocal where s is a power of two (then both are the same value).
+struct Divider {
+    float s, inv;
+    bool exact;
+    __device__ __forceinline__ explicit Divider(float scale) : s(scale) {
+        exact = (__float_as_uint(scale) & 0x7fffffu) == 0 && scale >= 7.9e-31f && scale < 1.7e38f;
+        inv = exact ? 1.0f / scale : 0.0f;
+    }
+    __device__ __forceinline__ float operator()(float x) const { return exact ? x * inv : __fdiv_rn(x, s); }
+};
+
+// A run is a stretch of consecutive tokens whose slots are consecutive places of one
+// page. One warp takes one run of one head: the largest |x| of the run sets the scale
+// (never below the page's own, if the page already held tokens before the run's first
+// place), the tokens already there move to it if it grew, and the run is stored.
+// Grid: (token chunks, heads, keys / values). A run belongs to the CTA that holds its
+// first token; it may end behind that CTA's chunk.
+//
+// What bounds it: 2 bytes read and 1 written per element; at a few tokens, the chain
+// slot -> run -> values -> scale -> bytes.
+template <int kDim, bool kBf16>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+    constexpr int kLanes = kDim / 8;           // lanes that read one token, 16 bytes each
+    constexpr int kRows = 32 / kLanes;         // tokens per warp step
+    constexpr int kHeld = 8;                   // steps held in registers
+    const int which = static_cast<int>(blockIdx.z);
+    const int head = static_cast<int>(blockIdx.y);
+    const int lane = static_cast<int>(lane_id());
+    const int warp = static_cast<int>(threadIdx.x >> 5);
+    const long long t0 = static_cast<long long>(blockIdx.x) * p.chunk;
+    const int end = static_cast<int>(min(t0 + p.chunk, static_cast<long long>(p.n_tokens)));
+    const uint16_t* x = p.x[which] + head * kDim;
+    const long long stride = p.stride[which];
+    const long long n_slots = p.n_pages * p.page;
+    const int sub = lane / kLanes, col = (lane % kLanes) * 8;
+
+    // Each warp finds the first tokens of runs 32 tokens at a time and takes every fourth.
+    int seen = 0;
+    for (int base = static_cast<int>(t0); base < end; base += 32) {
+        const int t = base + lane;
+        bool first = false;
+        if (t < end) {
+            const long long s = p.slots[t];
+            if (s >= 0 && s < n_slots) {
+                const long long before = t > 0 ? p.slots[t - 1] : -1;
+                first = before < 0 || before + 1 != s || (s & (p.page - 1)) == 0;
+            }
+        }
+        uint32_t firsts = __ballot_sync(0xffffffffu, first);
+        while (firsts != 0) {
+            const int i = __ffs(firsts) - 1;
+            firsts &= firsts - 1;
+            if ((seen++ & (kAppendWarps - 1)) != warp) continue;
+            const int begin = base + i;
+            const long long slot = p.slots[begin];
+            const long long page = slot >> p.page_shift;
+            const int place = static_cast<int>(slot & (p.page - 1));
+            // Length of the run: at most to the page's end.
+            const int most = min(p.page - place, p.n_tokens - begin);
+            int n = 1;
+            while (n < most) {
+                const int j = n + lane;
+                const bool on = j < most && p.slots[begin + j] == slot + j;
+                const uint32_t mask = __ballot_sync(0xffffffffu, on);
+                const int more = mask == 0xffffffffu ? 32 : __ffs(~mask) - 1;
+                n += more;
+                if (more < 32) break;
+            }
+            const long long tile = page * p.heads + head;
+            uint8_t* bytes = p.cache[which] + tile * p.page * kDim;
+            float* scale_at = p.scale[which] + tile;
+            const float old = place > 0 ? *scale_at : 0.0f;
+            const uint16_t* rows = x + begin * stride + col;
+            uint4 held[kHeld];
+            float amax = 0.0f;
+            for (int j0 = 0; j0 < n; j0 += kRows * kHeld) {
+#pragma unroll
+                for (int u = 0; u < kHeld; ++u) {
+                    const int j = j0 + u * kRows + sub;
+                    held[u] = j < n ? __ldg(reinterpret_cast<const uint4*>(rows + j * stride)) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int u = 0; u < kHeld; ++u) {
+                    const uint32_t w[4] = {held[u].x, held[u].y, held[u].z, held[u].w};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float2 f = pair_to_float2<kBf16>(w[c]);
+                        amax = fmaxf(amax, fmaxf(finite_abs(f.x), finite_abs(f.y)));
+                    }
+                }
+            }
+            amax = warp_max(amax);
+            const float now = fmaxf(old, scale_for(amax));
+            if (place > 0 && now != old) {
+                // The tokens already in the page, to the new scale.
+                const float factor = __fdiv_rn(old, now);
+                for (int b = lane * 16; b < place * kDim; b += 512) {
+                    uint4 v = *reinterpret_cast<const uint4*>(bytes + b);
+                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float2 lo = half2_bits_to_float2(from_e4m3x2(w[c] & 0xffffu));
+                        const float2 hi = half2_bits_to_float2(from_e4m3x2(w[c] >> 16));
+                        w[c] = to_e4m3x2(lo.x * factor, lo.y * factor) | to_e4m3x2(hi.x * factor, hi.y * factor) << 16;
+                    }
+                    *reinterpret_cast<uint4*>(bytes + b) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            const Divider over(now);
+            const bool still = n <= kRows * kHeld;  // the registers still hold the whole run
+            for (int j0 = 0; j0 < n; j0 += kRows * kHeld) {
+                if (!still) {
+#pragma unroll
+                    for (int u = 0; u < kHeld; ++u) {
+                        const int j = j0 + u * kRows + sub;
+                        if (j < n) held[u] = __ldg(reinterpret_cast<const uint4*>(rows + j * stride));
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < kHeld; ++u) {
+                    const int j = j0 + u * kRows + sub;
+                    if (j < n) {
+                        const uint32_t w[4] = {held[u].x, held[u].y, held[u].z, held[u].w};
+                        uint32_t b[4];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const float2 f = pair_to_float2<kBf16>(w[c]);
+                            b[c] = to_e4m3x2(over(f.x), over(f.y));
+                        }
+                        *reinterpret_cast<uint2*>(bytes + static_cast<long long>(place + j) * kDim + col) =
+                            make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+                    }
+                }
+            }
+            if (lane == 0) *scale_at = now;
+        }
+    }
+}
+
+inline cudaError_t append_entry(bool bf16, const void* k, const void* v, long long k_stride, long long v_stride,
+                                const int64_t* slots, int n_tokens, int heads, int dim, void* k_cache, void* v_cache,
+                                float* k_scale, float* v_scale, long long n_pages, int page, cudaStream_t stream) {
+    if (k == nullptr || v == nullptr || slots == nullptr || k_cache == nullptr || v_cache == nullptr ||
+        k_scale == nullptr || v_scale == nullptr || n_tokens < 0 || heads <= 0 || heads > 65535 ||
+        (dim != 64 && dim != 128) || n_pages <= 0 || (page != 16 && page != 32 && page != 64 && page != 128)) {
+        return cudaErrorInvalidValue;
+    }
+    const long long row = static_cast<long long>(heads) * dim;
+    auto off = [](const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; };
+    if (k_stride < row || v_stride < row || k_stride % 8 != 0 || v_stride % 8 != 0 || off(k, 16) || off(v, 16) ||
+        off(k_cache, 16) || off(v_cache, 16) || off(k_scale, 4) || off(v_scale, 4) || off(slots, 8) ||
+        n_pages > LLONG_MAX / page / row || (n_tokens > 0 && (k_stride > LLONG_MAX / 2 / n_tokens || v_stride > LLONG_MAX / 2 / n_tokens))) {
+        return cudaErrorInvalidValue;
+    }
+    const size_t cache_bytes = static_cast<size_t>(n_pages) * page * row, scale_bytes = static_cast<size_t>(n_pages) * heads * 4;
+    const size_t x_bytes[2] = {n_tokens > 0 ? (static_cast<size_t>(n_tokens - 1) * k_stride + row) * 2 : 0,
+                               n_tokens > 0 ? (static_cast<size_t>(n_tokens - 1) * v_stride + row) * 2 : 0};
+    const void* outs[4] = {k_cache, v_cache, k_scale, v_scale};
+    const size_t out_bytes[4] = {cache_bytes, cache_bytes, scale_bytes, scale_bytes};
+    for (int i = 0; i < 4; ++i) {
+        if (host::ranges_overlap(outs[i], out_bytes[i], k, x_bytes[0]) || host::ranges_overlap(outs[i], out_bytes[i], v, x_bytes[1]) ||
+            host::ranges_overlap(outs[i], out_bytes[i], slots, static_cast<size_t>(n_tokens) * 8))
+            return cudaErrorInvalidValue;
+        for (int j = i + 1; j < 4; ++j)
+            if (host::ranges_overlap(outs[i], out_bytes[i], outs[j], out_bytes[j])) return cudaErrorInvalidValue;
+    }
+    cudaError_t err = host::current_device(nullptr, nullptr);
+    if (err != cudaSuccess) return err;
+    static_cast<void>(cudaGetLastError());
+    if (n_tokens == 0) return cudaSuccess;
+    AppendParams p{};
+    p.x[0] = static_cast<const uint16_t*>(k);
+    p.x[1] = static_cast<const uint16_t*>(v);
+    p.stride[0] = k_stride;
+    p.stride[1] = v_stride;
+    p.slots = slots;
+    p.n_tokens = n_tokens;
+    p.heads = heads;
+    p.cache[0] = static_cast<uint8_t*>(k_cache);
+    p.cache[1] = static_cast<uint8_t*>(v_cache);
+    p.scale[0] = k_scale;
+    p.scale[1] = v_scale;
+    p.n_pages = n_pages;
+    p.page = page;
+    p.page_shift = page == 16 ? 4 : (page == 32 ? 5 : (page == 64 ? 6 : 7));
+    p.chunk = n_tokens <= 1024 ? 4 : (n_tokens <= 8192 ? 16 : 64);
+    const dim3 grid(static_cast<unsigned>((n_tokens + p.chunk - 1) / p.chunk), static_cast<unsigned>(heads), 2);
+    if (dim == 128) {
+        if (bf16) append_kernel<128, true><<<grid, kAppendThreads, 0, stream>>>(p);
+        else append_kernel<128, false><<<grid, kAppendThreads, 0, stream>>>(p);
+    } else {
+        if (bf16) append_kernel<64, true><<<grid, kAppendThreads, 0, stream>>>(p);
+        else append_kernel<64, false><<<grid, kAppendThreads, 0, stream>>>(p);
+    }
+    return cudaGetLastError();
+}
+
+}  // namespace kv
+}  // namespace tk

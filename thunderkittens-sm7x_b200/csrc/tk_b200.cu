@@ -14,8 +14,11 @@
 #include <mutex>
 
 #include "attention.cuh"
+#include "attention_masked.cuh"
+#include "attention_paged.cuh"
 #include "attention_pair.cuh"
 #include "gemm.cuh"
+#include "kvcache.cuh"
 #include "rowops.cuh"
 #include "tk_host.cuh"
 
@@ -878,6 +881,66 @@ cudaError_t tk_attention_forward_gqa_f16(const void* q, const void* k, const voi
                                          float scale, int causal, cudaStream_t stream) {
     return tk::attn::attention_entry(q, k, v, out, batch, heads_q, heads_kv, seq, head_dim, scale, causal,
                                      false, stream);
+}
+
+cudaError_t tk_attention_masked_f16(const void* q, const void* k, const void* v, void* out, const int64_t* strides, int batch,
+                                    int heads_q, int heads_kv, int seq_q, int seq_kv, int head_dim, float scale, float softcap,
+                                    const float* alibi_slopes, const int32_t* doc_ids, const int32_t* prefix_lens, int causal,
+                                    cudaStream_t stream) {
+    return tk::masked::masked_entry(false, q, k, v, out, strides, batch, heads_q, heads_kv, seq_q, seq_kv, head_dim, scale,
+                                    softcap, alibi_slopes, doc_ids, prefix_lens, causal, stream);
+}
+
+cudaError_t tk_attention_masked_bf16(const void* q, const void* k, const void* v, void* out, const int64_t* strides, int batch,
+                                     int heads_q, int heads_kv, int seq_q, int seq_kv, int head_dim, float scale, float softcap,
+                                     const float* alibi_slopes, const int32_t* doc_ids, const int32_t* prefix_lens, int causal,
+                                     cudaStream_t stream) {
+    return tk::masked::masked_entry(true, q, k, v, out, strides, batch, heads_q, heads_kv, seq_q, seq_kv, head_dim, scale,
+                                    softcap, alibi_slopes, doc_ids, prefix_lens, causal, stream);
+}
+
+cudaError_t tk_kv_plan(const int32_t* cached_lens, const int32_t* new_lens, int n_requests, int page_size, int32_t* block_table,
+                       int max_pages, const int32_t* free_pages, int n_free_capacity, const int32_t* n_free, int32_t* lens_out,
+                       int32_t* seq_lens, int32_t* starts, int64_t* slots, int max_tokens, int32_t* n_free_out,
+                       cudaStream_t stream) {
+    return tk::kv::plan_entry(cached_lens, new_lens, n_requests, page_size, block_table, max_pages, free_pages, n_free_capacity,
+                              n_free, lens_out, seq_lens, starts, slots, max_tokens, n_free_out, stream);
+}
+
+cudaError_t tk_kv_append_e4m3_f16(const void* k, const void* v, int64_t k_stride, int64_t v_stride, const int64_t* slots,
+                                  int n_tokens, int heads_kv, int head_dim, void* k_cache, void* v_cache, float* k_scale,
+                                  float* v_scale, int n_pages, int page_size, cudaStream_t stream) {
+    return tk::kv::append_entry(false, k, v, k_stride, v_stride, slots, n_tokens, heads_kv, head_dim, k_cache, v_cache, k_scale,
+                                v_scale, n_pages, page_size, stream);
+}
+
+cudaError_t tk_kv_append_e4m3_bf16(const void* k, const void* v, int64_t k_stride, int64_t v_stride, const int64_t* slots,
+                                   int n_tokens, int heads_kv, int head_dim, void* k_cache, void* v_cache, float* k_scale,
+                                   float* v_scale, int n_pages, int page_size, cudaStream_t stream) {
+    return tk::kv::append_entry(true, k, v, k_stride, v_stride, slots, n_tokens, heads_kv, head_dim, k_cache, v_cache, k_scale,
+                                v_scale, n_pages, page_size, stream);
+}
+
+cudaError_t tk_attention_paged_e4m3_f16(const void* q, int64_t q_stride, void* out, int64_t out_stride, int n_tokens,
+                                        const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                                        int n_pages, int page_size, const int32_t* block_table, int max_pages,
+                                        const int32_t* seq_lens, const int32_t* starts, int n_requests, int heads_q, int heads_kv,
+                                        int head_dim, int max_query_len, int max_seq_len, float scale, float softcap,
+                                        const float* alibi_slopes, cudaStream_t stream) {
+    return tk::paged::paged_entry(false, q, q_stride, out, out_stride, n_tokens, k_cache, v_cache, k_scale, v_scale, n_pages,
+                                  page_size, block_table, max_pages, seq_lens, starts, n_requests, heads_q, heads_kv, head_dim,
+                                  max_query_len, max_seq_len, scale, softcap, alibi_slopes, stream);
+}
+
+cudaError_t tk_attention_paged_e4m3_bf16(const void* q, int64_t q_stride, void* out, int64_t out_stride, int n_tokens,
+                                         const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                                         int n_pages, int page_size, const int32_t* block_table, int max_pages,
+                                         const int32_t* seq_lens, const int32_t* starts, int n_requests, int heads_q,
+                                         int heads_kv, int head_dim, int max_query_len, int max_seq_len, float scale,
+                                         float softcap, const float* alibi_slopes, cudaStream_t stream) {
+    return tk::paged::paged_entry(true, q, q_stride, out, out_stride, n_tokens, k_cache, v_cache, k_scale, v_scale, n_pages,
+                                  page_size, block_table, max_pages, seq_lens, starts, n_requests, heads_q, heads_kv, head_dim,
+                                  max_query_len, max_seq_len, scale, softcap, alibi_slopes, stream);
 }
 
 cudaError_t tk_device_status(uint32_t* status, int clear) {

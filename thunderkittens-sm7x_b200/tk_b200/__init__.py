@@ -27,7 +27,10 @@ CUDA_ERROR_INVALID_DEVICE_FUNCTION = 98
 CUDA_ERROR_NOT_SUPPORTED = 801
 
 # Every symbol include/tk_b200.h declares, with its ctypes signature.
-_VP, _I, _SZ, _F = C.c_void_p, C.c_int, C.c_size_t, C.c_float
+_VP, _I, _SZ, _F, _L = C.c_void_p, C.c_int, C.c_size_t, C.c_float, C.c_int64
+_MASKED = [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _F, _VP, _VP, _VP, _I, _VP]
+_APPEND = [_VP, _VP, _L, _L, _VP, _I, _I, _I, _VP, _VP, _VP, _VP, _I, _I, _VP]
+_PAGED = [_VP, _L, _VP, _L, _I, _VP, _VP, _VP, _VP, _I, _I, _VP, _I, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _F, _VP, _VP]
 SIGNATURES = {
     "tk_gemm_f16_f16_f32_nn": (_I, [_I, _I, _I, _VP, _I, _VP, _I, _VP, _I, _VP]),
     "tk_gemm_f16_f16_f32_nn_rowstats": (_I, [_I, _I, _I, _VP, _I, _VP, _I, _VP, _I, _VP, _VP, _VP]),
@@ -50,6 +53,13 @@ SIGNATURES = {
     "tk_attention_forward_16x16_causal": (_I, [_VP, _VP, _VP, _VP, _VP]),
     "tk_attention_forward_f16": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _F, _I, _VP]),
     "tk_attention_forward_gqa_f16": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _F, _I, _VP]),
+    "tk_attention_masked_f16": (_I, _MASKED),
+    "tk_attention_masked_bf16": (_I, _MASKED),
+    "tk_kv_plan": (_I, [_VP, _VP, _I, _I, _VP, _I, _VP, _I, _VP, _VP, _VP, _VP, _VP, _I, _VP, _VP]),
+    "tk_kv_append_e4m3_f16": (_I, _APPEND),
+    "tk_kv_append_e4m3_bf16": (_I, _APPEND),
+    "tk_attention_paged_e4m3_f16": (_I, _PAGED),
+    "tk_attention_paged_e4m3_bf16": (_I, _PAGED),
     "tk_attention_set_cta_group": (_I, [_I]),
     "tk_gemm_set_group_rows": (_I, [_I]),
     "tk_gemm_set_small_m": (_I, [_I]),
@@ -272,4 +282,204 @@ def attention(q, k, v, *, scale, causal=False, out=None, stream=None):
     if out is None:
         out = torch.empty((b, h, s, d), dtype=torch.float32, device=q.device)
     _check("tk_attention_forward_f16", attention_raw(q, k, v, out, b, h, s, d, scale, causal, stream))
+    return out
+
+
+# ---- attention of language models, and the paged 8-bit cache ---------------------------
+
+def _require(ok, message):
+    if not ok:
+        raise ValueError(message)
+
+
+def _half_type(t, name):
+    import torch
+    _require(t.dtype in (torch.float16, torch.bfloat16), f"{name} must be float16 or bfloat16, got {t.dtype}")
+    return t.dtype
+
+
+def _same_device(device, **tensors):
+    for name, t in tensors.items():
+        _require(t is None or t.device == device, f"{name} is on {getattr(t, 'device', None)}, expected {device}")
+
+
+def _vector(t, name, dtype, shape):
+    """None, or a contiguous tensor of this type and shape."""
+    if t is None:
+        return
+    _require(t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous(),
+             f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+class _Launch:
+    """The stream of a call on `device`, current there while the call allocates its outputs,
+    so that they belong to that stream."""
+
+    def __init__(self, device, stream):
+        import torch
+        _require(device.type == "cuda", f"tensors must be on a CUDA device, got {device}")
+        self.device = torch.cuda.device(device)
+        if stream is None:
+            self.scope, self.handle = None, torch.cuda.current_stream(device).cuda_stream
+        else:
+            if isinstance(stream, int):
+                stream = torch.cuda.ExternalStream(stream, device=device)
+            _require(stream.device == device, f"stream is on {stream.device}, tensors on {device}")
+            self.scope, self.handle = torch.cuda.stream(stream), stream.cuda_stream
+
+    def __enter__(self):
+        self.device.__enter__()
+        if self.scope is not None:
+            self.scope.__enter__()
+        return self.handle
+
+    def __exit__(self, *exc):
+        if self.scope is not None:
+            self.scope.__exit__(*exc)
+        self.device.__exit__(*exc)
+
+
+def attention_masked(q, k, v, *, scale, causal=False, softcap=0.0, alibi_slopes=None, doc_ids=None, prefix_lens=None,
+                     out=None, stream=None):
+    """Attention under masks and score changes (tk_attention_masked_*).
+
+    q: [B, Hq, Sq, D], k, v: [B, Hkv, Skv, D], float16 or bfloat16, any strides with the last
+    one 1 (a [B, S, H, D] tensor goes in as its transpose(1, 2)). Returns [B, Hq, Sq, D] of the
+    same type, with q's order of strides if `out` is not given. alibi_slopes: float32 [Hq];
+    doc_ids: int32 [B, Sq] (each run of equal ids a document, negative: padding);
+    prefix_lens: int32 [B] (with causal). A row that may see no key is 0."""
+    import torch
+    kind = _half_type(q, "q")
+    _require(q.dim() == 4 and k.dim() == 4 and v.shape == k.shape, "q, k, v must be [B, H, S, D], k and v alike")
+    b, h, sq, d = q.shape
+    hkv, skv = k.shape[1], k.shape[2]
+    _require(k.shape[0] == b and k.shape[3] == d, f"k has shape {tuple(k.shape)}, q {tuple(q.shape)}")
+    _require(k.dtype == kind and v.dtype == kind, "q, k, v must have one type")
+    _require(all(t.stride(3) == 1 or d == 1 for t in (q, k, v)), "the last stride must be 1")
+    _vector(alibi_slopes, "alibi_slopes", torch.float32, (h,))
+    _vector(doc_ids, "doc_ids", torch.int32, (b, sq))
+    _vector(prefix_lens, "prefix_lens", torch.int32, (b,))
+    _same_device(q.device, k=k, v=v, out=out, alibi_slopes=alibi_slopes, doc_ids=doc_ids, prefix_lens=prefix_lens)
+    with _Launch(q.device, stream) as handle:
+        if out is None:
+            first = h > 1 and sq > 1 and q.stride(1) < q.stride(2)
+            out = torch.empty((b, sq, h, d) if first else (b, h, sq, d), dtype=kind, device=q.device)
+            out = out.transpose(1, 2) if first else out
+        _require(out.dtype == kind and out.shape == q.shape and out.stride(3) == 1, "out must have q's type and shape, last stride 1")
+        strides = (C.c_int64 * 12)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3])
+        name = "tk_attention_masked_f16" if kind == torch.float16 else "tk_attention_masked_bf16"
+        _check(name, getattr(lib(), name)(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), C.cast(strides, C.c_void_p),
+                                          b, h, hkv, sq, skv, d, float(scale), float(softcap), _ptr(alibi_slopes), _ptr(doc_ids),
+                                          _ptr(prefix_lens), 1 if causal else 0, handle))
+    return out
+
+
+def kv_plan(cached_lens, new_lens, block_table, free_pages, n_free, *, page_size, max_tokens, lens_out=None, seq_lens=None,
+            starts=None, slots=None, n_free_out=None, stream=None):
+    """Places for the new tokens of a step (tk_kv_plan): fills block_table in place and returns
+    (lens, seq_lens, starts, slots, n_free). cached_lens, new_lens: int32 [R]; block_table: int32
+    [R, max_pages]; free_pages: int32; n_free: int32 [1]. lens_out may be cached_lens and
+    n_free_out n_free, for a state that moves on in place."""
+    import torch
+    r = cached_lens.shape[0]
+    i32, dev = torch.int32, cached_lens.device
+    _vector(cached_lens, "cached_lens", i32, (r,))
+    _vector(new_lens, "new_lens", i32, (r,))
+    _require(block_table.dim() == 2, "block_table must be [R, max_pages]")
+    _vector(block_table, "block_table", i32, (r, block_table.shape[1]))
+    _vector(free_pages, "free_pages", i32, (free_pages.numel(),))
+    _vector(n_free, "n_free", i32, (1,))
+    with _Launch(dev, stream) as handle:
+        lens_out = torch.empty(r, dtype=i32, device=dev) if lens_out is None else lens_out
+        seq_lens = torch.empty(r, dtype=i32, device=dev) if seq_lens is None else seq_lens
+        starts = torch.empty(r + 1, dtype=i32, device=dev) if starts is None else starts
+        slots = torch.empty(max_tokens, dtype=torch.int64, device=dev) if slots is None else slots
+        n_free_out = torch.empty(1, dtype=i32, device=dev) if n_free_out is None else n_free_out
+        _vector(lens_out, "lens_out", i32, (r,))
+        _vector(seq_lens, "seq_lens", i32, (r,))
+        _vector(starts, "starts", i32, (r + 1,))
+        _vector(slots, "slots", torch.int64, (max_tokens,))
+        _vector(n_free_out, "n_free_out", i32, (1,))
+        _same_device(dev, new_lens=new_lens, block_table=block_table, free_pages=free_pages, n_free=n_free, lens_out=lens_out,
+                     seq_lens=seq_lens, starts=starts, slots=slots, n_free_out=n_free_out)
+        _check("tk_kv_plan", lib().tk_kv_plan(cached_lens.data_ptr(), new_lens.data_ptr(), r, page_size, block_table.data_ptr(),
+                                              block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(),
+                                              lens_out.data_ptr(), seq_lens.data_ptr(), starts.data_ptr(), slots.data_ptr(),
+                                              max_tokens, n_free_out.data_ptr(), handle))
+    return lens_out, seq_lens, starts, slots, n_free_out
+
+
+def _cache_shape(k_cache, v_cache, k_scale, v_scale):
+    import torch
+    _require(k_cache.dim() == 4, "k_cache must be [pages, Hkv, page_size, D]")
+    shape = k_cache.shape
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _require(t.dtype in (torch.uint8, torch.float8_e4m3fn), f"{name} must hold bytes (uint8 or float8_e4m3fn)")
+        _vector(t, name, t.dtype, shape)
+    _vector(k_scale, "k_scale", torch.float32, shape[:2])
+    _vector(v_scale, "v_scale", torch.float32, shape[:2])
+    return shape
+
+
+def _tokens(t, name, heads, dim):
+    """Elements between the tokens of a packed [T, heads, dim] tensor."""
+    _require(t.dim() == 3 and t.shape[1] == heads and t.shape[2] == dim, f"{name} must be [T, {heads}, {dim}], got {tuple(t.shape)}")
+    _require(t.stride(2) == 1 and (heads == 1 or t.stride(1) == dim), f"the heads of a token of {name} must be adjacent")
+    return t.stride(0) if t.shape[0] > 1 else heads * dim
+
+
+def kv_append(k, v, slots, k_cache, v_cache, k_scale, v_scale, *, stream=None):
+    """Quantises packed tokens k, v [T, Hkv, D] (float16 or bfloat16) into the cache at slots
+    (int64 [T], -1: skipped), in place (tk_kv_append_e4m3_*)."""
+    import torch
+    kind = _half_type(k, "k")
+    pages, heads, page, dim = _cache_shape(k_cache, v_cache, k_scale, v_scale)
+    n = k.shape[0]
+    ks, vs = _tokens(k, "k", heads, dim), _tokens(v, "v", heads, dim)
+    _require(v.dtype == kind and v.shape[0] == n, "k and v must have one type and length")
+    _vector(slots, "slots", torch.int64, (n,))
+    _same_device(k.device, v=v, slots=slots, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
+    if n == 0:
+        return
+    with _Launch(k.device, stream) as handle:
+        name = "tk_kv_append_e4m3_f16" if kind == torch.float16 else "tk_kv_append_e4m3_bf16"
+        _check(name, getattr(lib(), name)(k.data_ptr(), v.data_ptr(), ks, vs, slots.data_ptr(), n, heads, dim, k_cache.data_ptr(),
+                                          v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, page, handle))
+
+
+def attention_paged(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, starts, *, scale, softcap=0.0,
+                    alibi_slopes=None, max_query_len=1, max_seq_len=None, out=None, stream=None):
+    """Attention of packed newest tokens q [T, Hq, D] over the paged cache
+    (tk_attention_paged_e4m3_*); returns [T, Hq, D] of q's type. max_query_len: at least the most
+    query tokens of a request; max_seq_len: about the longest context (default: what the block
+    table can hold). Rows behind the last request are left as they were in `out`."""
+    import torch
+    kind = _half_type(q, "q")
+    pages, hkv, page, dim = _cache_shape(k_cache, v_cache, k_scale, v_scale)
+    _require(q.dim() == 3, "q must be [T, Hq, D]")
+    n, h = q.shape[0], q.shape[1]
+    _require(block_table.dim() == 2, "block_table must be [R, max_pages]")
+    r = block_table.shape[0]
+    _vector(block_table, "block_table", torch.int32, block_table.shape)
+    _vector(seq_lens, "seq_lens", torch.int32, (r,))
+    _vector(starts, "starts", torch.int32, (r + 1,))
+    _vector(alibi_slopes, "alibi_slopes", torch.float32, (h,))
+    q_stride = _tokens(q, "q", h, dim)
+    _same_device(q.device, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, block_table=block_table,
+                 seq_lens=seq_lens, starts=starts, alibi_slopes=alibi_slopes, out=out)
+    if max_seq_len is None:
+        max_seq_len = block_table.shape[1] * page
+    with _Launch(q.device, stream) as handle:
+        if out is None:
+            out = torch.empty((n, h, dim), dtype=kind, device=q.device)
+        _require(out.dtype == kind and out.shape == q.shape, "out must have q's type and shape")
+        out_stride = _tokens(out, "out", h, dim)
+        if n == 0 or r == 0:
+            return out
+        name = "tk_attention_paged_e4m3_f16" if kind == torch.float16 else "tk_attention_paged_e4m3_bf16"
+        _check(name, getattr(lib(), name)(q.data_ptr(), q_stride, out.data_ptr(), out_stride, n, k_cache.data_ptr(),
+                                          v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, page,
+                                          block_table.data_ptr(), block_table.shape[1], seq_lens.data_ptr(), starts.data_ptr(), r,
+                                          h, hkv, dim, max_query_len, max_seq_len, float(scale), float(softcap),
+                                          _ptr(alibi_slopes), handle))
     return out
