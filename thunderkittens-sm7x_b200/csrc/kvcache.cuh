@@ -121,20 +121,28 @@ __device__ __forceinline__ int upper_bound(const int* ends, int n, int x) {
 //   page k of the call = free_pages[n_free - 1 - k]
 //
 // What bounds it: one launch and the chain lengths -> sums -> entries; the bytes are
-// a few MB at most (8 per slot).
+// a few MB at most (8 per slot). Each warp writes one stretch of consecutive slots, so
+// it searches for its request once and again only where a request ends; four slots a
+// lane are in flight, since each waits for a page number from L2.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
     __shared__ long long warp_sums[32];
     __shared__ int s_ends[kPlanThreads];   // running new tokens, clamped to INT_MAX
     __shared__ int s_upto[kPlanThreads];   // running pages needed, clamped
-    __shared__ int s_cached[kPlanThreads];
+    __shared__ int s_shift[kPlanThreads];  // position of token t of the call: t + shift
+    __shared__ int s_have[kPlanThreads];   // pages held before
+    __shared__ int s_base[kPlanThreads];   // number in the call of the page of column c: c + base
     __shared__ int s_taken[kPlanThreads];
     __shared__ int s_used;
     const int tid = static_cast<int>(threadIdx.x);
+    const int lane = static_cast<int>(lane_id());
     const int rank = static_cast<int>(blockIdx.x);
     const int ctas = static_cast<int>(gridDim.x);
     int n_free = *p.n_free;
     n_free = n_free < 0 ? 0 : (n_free > p.free_capacity ? p.free_capacity : n_free);
     if (tid == 0) s_used = 0;
+    const bool pow2 = (p.page & (p.page - 1)) == 0;
+    const int shift = 31 - __clz(p.page);
+    auto column_of = [&](int pos) { return pow2 ? pos >> shift : pos / p.page; };
     long long tokens = 0, pages = 0;  // sums over the earlier requests
     for (int r0 = 0; r0 < p.n_requests; r0 += kPlanThreads) {
         const int r = r0 + tid;
@@ -154,7 +162,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
         const bool taken = fits && (need == 0 || upto <= n_free);
         s_ends[tid] = static_cast<int>(min(end, static_cast<long long>(INT_MAX)));
         s_upto[tid] = static_cast<int>(min(upto, static_cast<long long>(INT_MAX)));
-        s_cached[tid] = c;
+        // Only read where taken: then end <= max_tokens and, if pages are needed, upto <= n_free.
+        s_shift[tid] = c - static_cast<int>(end - n);
+        s_have[tid] = have;
+        s_base[tid] = static_cast<int>(upto - need) - have;
         s_taken[tid] = taken ? 1 : 0;
         if (taken && need > 0) atomicMax(&s_used, static_cast<int>(upto));
         if (ctas > 1) cluster_sync(); else __syncthreads();
@@ -168,27 +179,40 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
         const int last_page = static_cast<int>(min(pages + page_sum, static_cast<long long>(n_free)));
         for (long long k = pages + rank * kPlanThreads + tid; k < last_page; k += ctas * kPlanThreads) {
             const int i = upper_bound(s_upto, here, static_cast<int>(k));
-            if (i >= here || !s_taken[i]) continue;
-            const int first = i > 0 ? s_upto[i - 1] : static_cast<int>(pages);
-            const int have_i = static_cast<int>((static_cast<long long>(s_cached[i]) + p.page - 1) / p.page);
-            p.table[static_cast<long long>(r0 + i) * p.width + have_i + (k - first)] = p.free_pages[n_free - 1 - k];
+            if (i < here && s_taken[i])
+                p.table[static_cast<long long>(r0 + i) * p.width + (k - s_base[i])] = p.free_pages[n_free - 1 - k];
         }
-        // Slots.
-        const int last_token = static_cast<int>(min(tokens + sum, static_cast<long long>(p.max_tokens)));
-        for (long long t = tokens + rank * kPlanThreads + tid; t < last_token; t += ctas * kPlanThreads) {
-            const int i = upper_bound(s_ends, here, static_cast<int>(t));
-            long long slot = -1;
-            if (i < here && s_taken[i]) {
-                const int first_token = i > 0 ? s_ends[i - 1] : static_cast<int>(tokens);
-                const int pos = s_cached[i] + static_cast<int>(t - first_token);
-                const int col = pos / p.page;
-                const int have_i = static_cast<int>((static_cast<long long>(s_cached[i]) + p.page - 1) / p.page);
-                const int first_page = i > 0 ? s_upto[i - 1] : static_cast<int>(pages);
-                const int page = col < have_i ? p.table[static_cast<long long>(r0 + i) * p.width + col]
-                                              : p.free_pages[n_free - 1 - (first_page + col - have_i)];
-                if (page >= 0) slot = static_cast<long long>(page) * p.page + pos % p.page;
+        // Slots, a stretch of whole 128s for each warp of the cluster.
+        const long long last_token = min(tokens + sum, static_cast<long long>(p.max_tokens));
+        const int warps = ctas * (kPlanThreads / 32);
+        const long long each = last_token > tokens ? ((last_token - tokens + warps - 1) / warps + 127) / 128 * 128 : 0;
+        const long long from = tokens + each * (rank * (kPlanThreads / 32) + (tid >> 5));
+        const long long to = min(from + each, last_token);
+        int i = from < to ? upper_bound(s_ends, here, static_cast<int>(from)) : 0;
+        for (long long t0 = from; t0 < to; t0 += 128) {
+            const int first = static_cast<int>(t0), last = static_cast<int>(min(t0 + 128, to)) - 1;
+            while (i < here && s_ends[i] <= first) ++i;
+            const bool one = i < here && s_ends[i] > last;  // all of them belong to request i
+            int owner[4], place[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int t = first + 32 * u + lane;
+                owner[u] = -1;
+                place[u] = 0;
+                if (t > last) continue;
+                const int q = one ? i : upper_bound(s_ends, here, t);
+                if (q >= here || !s_taken[q]) continue;
+                const int pos = t + s_shift[q];
+                const int col = column_of(pos);
+                place[u] = pos - col * p.page;
+                owner[u] = col < s_have[q] ? p.table[static_cast<long long>(r0 + q) * p.width + col]
+                                           : __ldg(p.free_pages + (n_free - 1 - (col + s_base[q])));
             }
-            p.slots[t] = slot;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int t = first + 32 * u + lane;
+                if (t <= last) p.slots[t] = owner[u] >= 0 ? static_cast<long long>(owner[u]) * p.page + place[u] : -1;
+            }
         }
         tokens += sum;
         pages += page_sum;
@@ -261,6 +285,8 @@ inline cudaError_t plan_entry(const int* cached, const int* fresh, int n_request
 
 constexpr int kAppendThreads = 128;
 constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kMostPage = 128;
+constexpr int kMostChunk = 64;
 constexpr int kLeastExponent = -100;  // of a scale: what is smaller than 2^-109 becomes 0
 
 struct AppendParams {
@@ -293,6 +319,13 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a <= 3.402823466e38f ? a : 0.0f;
 }
 
+// The same for a pair of 16-bit values, as bits (whose order is that of the magnitudes).
+template <bool kBf16>
+__device__ __forceinline__ uint32_t finite_magnitudes(uint32_t pair) {
+    const uint32_t a = pair & 0x7fff7fffu;
+    return a & __vcmpltu2(a, kBf16 ? 0x7f807f80u : 0x7c007c00u);
+}
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -311,69 +344,79 @@ struct Divider {
 };
 
 // A run is a stretch of consecutive tokens whose slots are consecutive places of one
-// page. One warp takes one run of one head: the largest |x| of the run sets the scale
-// (never below the page's own, if the page already held tokens before the run's first
-// place), the tokens already there move to it if it grew, and the run is stored.
-// Grid: (token chunks, heads, keys / values). A run belongs to the CTA that holds its
-// first token; it may end behind that CTA's chunk.
+// page. One warp (or, kCta, the four warps of a CTA together) takes one run of one
+// head: the largest |x| of the run sets the scale (never below the page's own, if the
+// page already held tokens before the run's first place), the tokens already there move
+// to it if it grew, and the run is stored. Grid: (token chunks, heads, keys / values). A
+// run belongs to the CTA that holds its first token; it may end behind that CTA's chunk,
+// so the CTA looks at one slot before its chunk and a page's worth behind it.
 //
 // What bounds it: 2 bytes read and 1 written per element; at a few tokens, the chain
-// slot -> run -> values -> scale -> bytes.
-template <int kDim, bool kBf16>
+// slots -> values -> scale -> bytes.
+template <int kDim, bool kBf16, bool kCta>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
-    constexpr int kLanes = kDim / 8;           // lanes that read one token, 16 bytes each
-    constexpr int kRows = 32 / kLanes;         // tokens per warp step
-    constexpr int kHeld = 8;                   // steps held in registers
-    const int which = static_cast<int>(blockIdx.z);
+    constexpr int kLanes = kDim / 8;                      // threads that read one token, 16 bytes each
+    constexpr int kGroup = kCta ? kAppendThreads : 32;    // threads that work on one run
+    constexpr int kRows = kGroup / kLanes;                // tokens per step
+    constexpr int kHeld = 8;                              // steps held in registers
+    __shared__ long long s_slots[1 + kMostChunk + kMostPage];
+    __shared__ float s_max[kAppendWarps];
+    const bool values = blockIdx.z != 0;
     const int head = static_cast<int>(blockIdx.y);
+    const int tid = static_cast<int>(threadIdx.x);
     const int lane = static_cast<int>(lane_id());
-    const int warp = static_cast<int>(threadIdx.x >> 5);
-    const long long t0 = static_cast<long long>(blockIdx.x) * p.chunk;
-    const int end = static_cast<int>(min(t0 + p.chunk, static_cast<long long>(p.n_tokens)));
-    const uint16_t* x = p.x[which] + head * kDim;
-    const long long stride = p.stride[which];
+    const int warp = tid >> 5;
+    const int in_group = kCta ? tid : lane;
+    const int t0 = static_cast<int>(blockIdx.x) * p.chunk;
+    const int count = min(p.chunk, p.n_tokens - t0);
+    const uint16_t* x = (values ? p.x[1] : p.x[0]) + head * kDim;
+    const long long stride = values ? p.stride[1] : p.stride[0];
+    uint8_t* cache = values ? p.cache[1] : p.cache[0];
+    float* scales = values ? p.scale[1] : p.scale[0];
     const long long n_slots = p.n_pages * p.page;
-    const int sub = lane / kLanes, col = (lane % kLanes) * 8;
+    const int sub = in_group / kLanes, col = (in_group % kLanes) * 8;
 
-    // Each warp finds the first tokens of runs 32 tokens at a time and takes every fourth.
+    // s_slots[1 + i]: slot of token t0 + i, -1 where there is no such token or place.
+    for (int i = tid; i < 1 + count + p.page; i += kAppendThreads) {
+        const long long t = static_cast<long long>(t0) + i - 1;
+        long long s = t >= 0 && t < p.n_tokens ? __ldg(p.slots + t) : -1;
+        if (s < 0 || s >= n_slots) s = -1;
+        s_slots[i] = s;
+    }
+    __syncthreads();
+
+    // Every warp finds the first tokens of runs; without kCta it takes every fourth.
     int seen = 0;
-    for (int base = static_cast<int>(t0); base < end; base += 32) {
-        const int t = base + lane;
+    for (int base = 0; base < count; base += 32) {
+        const int i = base + lane;
         bool first = false;
-        if (t < end) {
-            const long long s = p.slots[t];
-            if (s >= 0 && s < n_slots) {
-                const long long before = t > 0 ? p.slots[t - 1] : -1;
-                first = before < 0 || before + 1 != s || (s & (p.page - 1)) == 0;
-            }
+        if (i < count) {
+            const long long s = s_slots[1 + i], before = s_slots[i];
+            first = s >= 0 && (before < 0 || before + 1 != s || (s & (p.page - 1)) == 0);
         }
         uint32_t firsts = __ballot_sync(0xffffffffu, first);
         while (firsts != 0) {
-            const int i = __ffs(firsts) - 1;
+            const int begin = base + __ffs(firsts) - 1;
             firsts &= firsts - 1;
-            if ((seen++ & (kAppendWarps - 1)) != warp) continue;
-            const int begin = base + i;
-            const long long slot = p.slots[begin];
-            const long long page = slot >> p.page_shift;
+            if (!kCta && (seen++ & (kAppendWarps - 1)) != warp) continue;
+            const long long slot = s_slots[1 + begin];
             const int place = static_cast<int>(slot & (p.page - 1));
             // Length of the run: at most to the page's end.
-            const int most = min(p.page - place, p.n_tokens - begin);
+            const int most = p.page - place;
             int n = 1;
             while (n < most) {
                 const int j = n + lane;
-                const bool on = j < most && p.slots[begin + j] == slot + j;
-                const uint32_t mask = __ballot_sync(0xffffffffu, on);
+                const uint32_t mask = __ballot_sync(0xffffffffu, j < most && s_slots[1 + begin + j] == slot + j);
                 const int more = mask == 0xffffffffu ? 32 : __ffs(~mask) - 1;
                 n += more;
                 if (more < 32) break;
             }
-            const long long tile = page * p.heads + head;
-            uint8_t* bytes = p.cache[which] + tile * p.page * kDim;
-            float* scale_at = p.scale[which] + tile;
-            const float old = place > 0 ? *scale_at : 0.0f;
-            const uint16_t* rows = x + begin * stride + col;
+            const long long tile = (slot >> p.page_shift) * p.heads + head;
+            uint8_t* bytes = cache + tile * p.page * kDim;
+            const float old = place > 0 ? scales[tile] : 0.0f;
+            const uint16_t* rows = x + static_cast<long long>(t0 + begin) * stride + col;
             uint4 held[kHeld];
-            float amax = 0.0f;
+            uint32_t top = 0;  // two 16-bit maxima
             for (int j0 = 0; j0 < n; j0 += kRows * kHeld) {
 #pragma unroll
                 for (int u = 0; u < kHeld; ++u) {
@@ -384,19 +427,23 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
                 for (int u = 0; u < kHeld; ++u) {
                     const uint32_t w[4] = {held[u].x, held[u].y, held[u].z, held[u].w};
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const float2 f = pair_to_float2<kBf16>(w[c]);
-                        amax = fmaxf(amax, fmaxf(finite_abs(f.x), finite_abs(f.y)));
-                    }
+                    for (int c = 0; c < 4; ++c) top = __vmaxu2(top, finite_magnitudes<kBf16>(w[c]));
                 }
             }
-            amax = warp_max(amax);
+            const float2 tops = pair_to_float2<kBf16>(top);
+            float amax = warp_max(fmaxf(tops.x, tops.y));
+            if constexpr (kCta) {
+                __syncthreads();  // the last run's maxima have been read, and its scale
+                if (lane == 0) s_max[warp] = amax;
+                __syncthreads();
+                amax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+            }
             const float now = fmaxf(old, scale_for(amax));
             if (place > 0 && now != old) {
                 // The tokens already in the page, to the new scale.
                 const float factor = __fdiv_rn(old, now);
-                for (int b = lane * 16; b < place * kDim; b += 512) {
-                    uint4 v = *reinterpret_cast<const uint4*>(bytes + b);
+                for (int b = in_group * 16; b < place * kDim; b += kGroup * 16) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(bytes + b);
                     uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
@@ -408,9 +455,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
                 }
             }
             const Divider over(now);
-            const bool still = n <= kRows * kHeld;  // the registers still hold the whole run
             for (int j0 = 0; j0 < n; j0 += kRows * kHeld) {
-                if (!still) {
+                if (n > kRows * kHeld) {  // else the registers still hold the run
 #pragma unroll
                     for (int u = 0; u < kHeld; ++u) {
                         const int j = j0 + u * kRows + sub;
@@ -428,12 +474,11 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
                             const float2 f = pair_to_float2<kBf16>(w[c]);
                             b[c] = to_e4m3x2(over(f.x), over(f.y));
                         }
-                        *reinterpret_cast<uint2*>(bytes + static_cast<long long>(place + j) * kDim + col) =
-                            make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+                        *reinterpret_cast<uint2*>(bytes + (place + j) * kDim + col) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
                     }
                 }
             }
-            if (lane == 0) *scale_at = now;
+            if (in_group == 0) scales[tile] = now;
         }
     }
 }
@@ -484,14 +529,20 @@ inline cudaError_t append_entry(bool bf16, const void* k, const void* v, long lo
     p.n_pages = n_pages;
     p.page = page;
     p.page_shift = page == 16 ? 4 : (page == 32 ? 5 : (page == 64 ? 6 : 7));
-    p.chunk = n_tokens <= 1024 ? 4 : (n_tokens <= 8192 ? 16 : 64);
+    // Few tokens: each is likely a run of its own (a decode step), one to a warp. Many: runs
+    // of up to a page, one at a time by the whole CTA.
+    const bool cta = n_tokens > 1024;
+    p.chunk = cta ? (n_tokens <= 8192 ? 16 : kMostChunk) : kAppendWarps;
     const dim3 grid(static_cast<unsigned>((n_tokens + p.chunk - 1) / p.chunk), static_cast<unsigned>(heads), 2);
-    if (dim == 128) {
-        if (bf16) append_kernel<128, true><<<grid, kAppendThreads, 0, stream>>>(p);
-        else append_kernel<128, false><<<grid, kAppendThreads, 0, stream>>>(p);
-    } else {
-        if (bf16) append_kernel<64, true><<<grid, kAppendThreads, 0, stream>>>(p);
-        else append_kernel<64, false><<<grid, kAppendThreads, 0, stream>>>(p);
+    switch ((dim == 128 ? 4 : 0) + (bf16 ? 2 : 0) + (cta ? 1 : 0)) {
+        case 0: append_kernel<64, false, false><<<grid, kAppendThreads, 0, stream>>>(p); break;
+        case 1: append_kernel<64, false, true><<<grid, kAppendThreads, 0, stream>>>(p); break;
+        case 2: append_kernel<64, true, false><<<grid, kAppendThreads, 0, stream>>>(p); break;
+        case 3: append_kernel<64, true, true><<<grid, kAppendThreads, 0, stream>>>(p); break;
+        case 4: append_kernel<128, false, false><<<grid, kAppendThreads, 0, stream>>>(p); break;
+        case 5: append_kernel<128, false, true><<<grid, kAppendThreads, 0, stream>>>(p); break;
+        case 6: append_kernel<128, true, false><<<grid, kAppendThreads, 0, stream>>>(p); break;
+        default: append_kernel<128, true, true><<<grid, kAppendThreads, 0, stream>>>(p); break;
     }
     return cudaGetLastError();
 }
