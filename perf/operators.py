@@ -258,13 +258,16 @@ def prepare(case, seed):
 
 # ---- one pass --------------------------------------------------------------------------
 
+def _framework():
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "thunderkittens-sm7x_b200"))
+    import tk_b200
+    return tk_b200
+
+
 def run(s):
     op = s["case"]["op"]
     if own:
-        here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "thunderkittens-sm7x_b200")
-        if here not in sys.path:
-            sys.path.insert(0, here)
-        import tk_b200
+        tk_b200 = sys.modules.get("tk_b200") or _framework()
         if op == "masked":
             return tk_b200.attention_masked(s["q"], s["k"], s["v"], scale=s["scale"], causal=s["case"]["causal"], softcap=s["case"]["cap"],
                                             alibi_slopes=s["slopes"], doc_ids=s["documents"], prefix_lens=s["prefix"])
