@@ -25,7 +25,10 @@
 //  - V: lane holds dims [D/8 g, D/8 (g + 1)) of tokens 2t, 2t + 1, 2t + 8, 2t + 9; byte
 //    pairs of two tokens are one register of V^T. Output dims are permuted alike.
 //  - P^T as B operand is the transpose of the S^T accumulator: one movmatrix per 8 x 8.
-// The next 16 tokens' loads are in flight while one is computed.
+// Bytes go through shared memory, a ring of kStages x 16 tokens for each warp alone
+// (cp.async and __syncwarp, no CTA barrier): what HBM needs in flight, some 100 KB an SM,
+// does not fit the registers. The ring's 16-byte pieces are swizzled so that both the
+// K reads (rows g, pieces 2t) and the V reads (rows 2t, pieces g) hit distinct banks.
 //
 // Long contexts are cut into `splits` chunks, each a CTA of its own, whose (max, sum, O)
 // a second kernel joins in chunk order: results do not depend on timing.
@@ -44,6 +47,7 @@ using attn::ex2;
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kStep = 16;       // tokens per warp step
+constexpr int kCtasPerSm = 24;
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are held in binary16 as 2^(x - m + kLift), with the reference point m
 // at most 8 below the row's max: at most 2^15, so that binary16 keeps 11 bits down to
@@ -103,19 +107,22 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     return y;
 }
 
-// kWords 32-bit words from a 4 * kWords byte aligned address, not kept in L1.
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// kWords 32-bit words of shared memory, aligned to their size.
 template <int kWords>
-__device__ __forceinline__ void load_words(uint32_t (&w)[kWords], const uint8_t* at) {
-    if constexpr (kWords == 8) {
-        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                     : "l"(at));
-    } else if constexpr (kWords == 4) {
-        asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                     : "l"(at));
+__device__ __forceinline__ void load_shared(uint32_t (&w)[kWords], uint32_t at) {
+    if constexpr (kWords == 4) {
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
     } else {
-        asm volatile("ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(at));
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
     }
 }
 
@@ -125,31 +132,39 @@ __device__ __forceinline__ float tanh_of(float x) {
     return fmaf(-2.0f, rcp_approx(1.0f + ex2(x * (2.0f * kLog2e))), 1.0f);
 }
 
-// 16 tokens of one key head as loaded.
-template <int D>
+// 16 tokens of one key head in a warp's ring: K, then V, 16 D bytes each, in lines of 128
+// bytes (a token, or two of head_dim 64). Piece c of token r stands at piece_at.
+template <int D, bool kV>
+__device__ __forceinline__ uint32_t piece_at(int r, int c) {
+    if constexpr (D == 128) return r * 128 + ((c ^ (kV ? r & 6 : r & 1)) << 4);
+    return (r >> 1) * 128 + ((((r & 1) * 4 + c) ^ (kV ? r & 6 : 0)) << 4);
+}
+
+// What comes with 16 tokens in registers.
 struct Step {
-    uint32_t k[2][D / 16];
-    uint32_t v[4][D / 32];
     float ks, vs;
-    bool on;
+    bool on;  // the page is there
 };
 
 template <int D>
-__device__ __forceinline__ void load_step(Step<D>& st, const Params& p, int head, int page, int token, int g, int t) {
+__device__ __forceinline__ void load_step(Step& st, uint32_t stage, const Params& p, int head, int page, int token, int lane) {
     st.on = page >= 0 && page < p.n_pages;
-    if (!st.on) return;
-    const long long tile = static_cast<long long>(page) * p.heads_kv + head;
-    const long long at = (tile * p.page + (token & (p.page - 1))) * D;
-    const uint8_t* k = p.k_cache + at + t * (D / 4);
-    load_words(st.k[0], k + g * D);
-    load_words(st.k[1], k + (g + 8) * D);
-    const uint8_t* v = p.v_cache + at + 2 * t * D + g * (D / 8);
-    load_words(st.v[0], v);
-    load_words(st.v[1], v + D);
-    load_words(st.v[2], v + 8 * D);
-    load_words(st.v[3], v + 9 * D);
-    st.ks = __ldg(p.k_scale + tile);
-    st.vs = __ldg(p.v_scale + tile);
+    if (st.on) {
+        const long long tile = static_cast<long long>(page) * p.heads_kv + head;
+        const long long at = (tile * p.page + (token & (p.page - 1))) * D + lane * 16;
+        constexpr int kPieces = D / 16;             // of a token
+        constexpr int kRows = 32 / kPieces;         // tokens per instruction
+        const int r = lane / kPieces, c = lane % kPieces;
+#pragma unroll
+        for (int i = 0; i < kStep / kRows; ++i)
+            cp_async_16(stage + piece_at<D, false>(r + i * kRows, c), p.k_cache + at + i * 512);
+#pragma unroll
+        for (int i = 0; i < kStep / kRows; ++i)
+            cp_async_16(stage + kStep * D + piece_at<D, true>(r + i * kRows, c), p.v_cache + at + i * 512);
+        st.ks = __ldg(p.k_scale + tile);
+        st.vs = __ldg(p.v_scale + tile);
+    }
+    cp_async_commit();
 }
 
 // What one lane knows of its 2 NT score columns (rows 8 nt + 2 t + {0, 1}).
@@ -178,13 +193,21 @@ __device__ __forceinline__ uint16_t out_bits(float x) {
     }
 }
 
+template <int D>
+constexpr int kStages = D == 128 ? 3 : 4;
+template <int D, int NT>
+constexpr int kSmemBytes = kWarps * kStages<D> * kStep * 2 * D > kWarps * 8 * NT * ((D + 4) * 4 + 8)
+                               ? kWarps * kStages<D> * kStep * 2 * D : kWarps * 8 * NT * ((D + 4) * 4 + 8);
+
 template <int D, int NT, bool kBf16, bool kChange>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const Params p) {
     constexpr int kRows = 8 * NT;
     constexpr int kM = D / 16;          // MMA tiles of output dims; k-steps of S^T
     constexpr int kPitch = D + 4;       // floats: rows 2t of a store fall on other banks
-    __shared__ float s_o[kWarps][kRows][kPitch];
-    __shared__ float2 s_ml[kWarps][kRows];
+    extern __shared__ __align__(128) uint8_t smem[];
+    // After the loop the rings' memory holds each warp's O, and the (point, sum) of its rows.
+    float (*s_o)[kRows][kPitch] = reinterpret_cast<float (*)[kRows][kPitch]>(smem);
+    float2 (*s_ml)[kRows] = reinterpret_cast<float2 (*)[kRows]>(smem + kWarps * kRows * kPitch * 4);
 
     const int lane = static_cast<int>(lane_id());
     const int warp = static_cast<int>(threadIdx.x >> 5);
@@ -278,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
     const int* table = p.table + static_cast<long long>(r) * p.width;
     auto page_at = [&](int token) { return token < end ? __ldg(table + (token >> p.page_shift)) : -1; };
 
-    auto compute = [&](Step<D>& st, int token) {
+    auto compute = [&](const Step& st, uint32_t stage, int token) {
         if (!st.on) return;  // no such page: as if its tokens were not there
         float s[NT][4];
 #pragma unroll
@@ -286,11 +309,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
 #pragma unroll
             for (int c = 0; c < 4; ++c) s[nt][c] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kM; ++w) {
-            const uint32_t a0 = kv::from_e4m3x2(st.k[0][w] & 0xffffu), a2 = kv::from_e4m3x2(st.k[0][w] >> 16);
-            const uint32_t a1 = kv::from_e4m3x2(st.k[1][w] & 0xffffu), a3 = kv::from_e4m3x2(st.k[1][w] >> 16);
+        for (int c = 0; c < D / 64; ++c) {
+            uint32_t near[4], far[4];  // tokens g and g + 8
+            load_shared(near, stage + piece_at<D, false>(g, t * (D / 64) + c));
+            load_shared(far, stage + piece_at<D, false>(g + 8, t * (D / 64) + c));
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt], a0, a1, a2, a3, q[nt][2 * w], q[nt][2 * w + 1]);
+            for (int i = 0; i < 4; ++i) {
+                const int w = 4 * c + i;
+                const uint32_t a0 = kv::from_e4m3x2(near[i] & 0xffffu), a2 = kv::from_e4m3x2(near[i] >> 16);
+                const uint32_t a1 = kv::from_e4m3x2(far[i] & 0xffffu), a3 = kv::from_e4m3x2(far[i] >> 16);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt], a0, a1, a2, a3, q[nt][2 * w], q[nt][2 * w + 1]);
+            }
         }
         const bool partial = token + kStep > end || token + kStep - 1 > first_pos;
         bool grow = false;
@@ -359,13 +389,20 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
             b[nt][0] = transpose_8x8(attn::pack_half2(e[0] * vr, e[1] * vr));
             b[nt][1] = transpose_8x8(attn::pack_half2(e[2] * vr, e[3] * vr));
         }
+        uint32_t v[4][D / 32];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int r = 2 * t + (u & 1) + (u >> 1) * 8;
+            if constexpr (D == 128) load_shared(v[u], stage + kStep * D + piece_at<D, true>(r, g));
+            else load_shared(v[u], stage + kStep * D + piece_at<D, true>(r, g >> 1) + (g & 1) * 8);
+        }
         if (token + kStep > end) {
             // Places behind the last token hold anything, NaN included: they become 0.
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (token + 2 * t + (u & 1) + (u >> 1) * 8 >= end)
 #pragma unroll
-                    for (int i = 0; i < D / 32; ++i) st.v[u][i] = 0;
+                    for (int i = 0; i < D / 32; ++i) v[u][i] = 0;
         }
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
@@ -373,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const uint32_t pick = half == 0 ? 0x5140u : 0x7362u;
-                const uint32_t near = __byte_perm(st.v[0][i], st.v[1][i], pick), far = __byte_perm(st.v[2][i], st.v[3][i], pick);
+                const uint32_t near = __byte_perm(v[0][i], v[1][i], pick), far = __byte_perm(v[2][i], v[3][i], pick);
                 const uint32_t a0 = kv::from_e4m3x2(near & 0xffffu), a1 = kv::from_e4m3x2(near >> 16);
                 const uint32_t a2 = kv::from_e4m3x2(far & 0xffffu), a3 = kv::from_e4m3x2(far >> 16);
 #pragma unroll
@@ -382,23 +419,38 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
         }
     };
 
-    // Warp w takes steps w, w + 4, ... of the chunk; two steps in registers.
+    // Warp w takes steps w, w + 4, ... of the chunk; kStages - 1 of them are in flight.
     constexpr int kStride = kWarps * kStep;
-    Step<D> one, two;
+    constexpr int kRing = kStages<D>;
+    const uint32_t ring = smem_u32(smem) + warp * (kRing * kStep * 2 * D);
+    Step steps[kRing];
     int token = begin + warp * kStep;
-    load_step<D>(one, p, head, page_at(token), token, g, t);
-    int next_page = page_at(token + kStride);
+    int load_token = token;
+    int next_page = page_at(load_token);
+    auto load_next = [&](Step& st, int stage) {
+        const int page = next_page;
+        const int at = load_token;
+        load_token += kStride;
+        next_page = page_at(load_token);
+        load_step<D>(st, ring + stage * (kStep * 2 * D), p, head, page, at, lane);
+    };
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) load_next(steps[i], i);
     while (token < end) {
-        load_step<D>(two, p, head, next_page, token + kStride, g, t);
-        next_page = page_at(token + 2 * kStride);
-        compute(one, token);
-        token += kStride;
-        if (token >= end) break;
-        load_step<D>(one, p, head, next_page, token + kStride, g, t);
-        next_page = page_at(token + 2 * kStride);
-        compute(two, token);
-        token += kStride;
+#pragma unroll
+        for (int i = 0; i < kRing; ++i) {
+            if (token < end) {
+                cp_async_wait<kRing - 2>();
+                __syncwarp();  // every lane's copies of this step have landed, and the step before is read
+                load_next(steps[(i + kRing - 1) % kRing], (i + kRing - 1) % kRing);
+                compute(steps[i], ring + i * (kStep * 2 * D), token);
+                token += kStride;
+            }
+        }
     }
+    cp_async_wait<0>();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __syncthreads();
 
     // Join the four warps, in warp order.
 #pragma unroll
@@ -469,6 +521,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
     const Request rq = request_of(p, r);
     const int n_rows = min(kRows, rq.n * p.group - tile * kRows);
     if (n_rows <= 0) return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int kv_end = max(rq.len - rq.n + (tile * kRows + n_rows - 1) / p.group + 1, 0);
     const int used = max(min((kv_end + p.chunk - 1) / p.chunk, p.splits), 1);
     const long long item = item_of(p, r, head, tile, 0);
@@ -499,11 +552,35 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
     }
 }
 
+template <int D, int NT, bool kBf16, bool kChange>
+cudaError_t launch_one(const Params& p, unsigned items, int device, cudaStream_t stream) {
+    static std::atomic<bool> configured[host::kMaxDevices];
+    auto kernel = paged_kernel<D, NT, kBf16, kChange>;
+    if (!configured[device].load(std::memory_order_acquire)) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<D, NT>);
+        if (e != cudaSuccess) return e;
+        configured[device].store(true, std::memory_order_release);
+    }
+    kernel<<<items * p.splits, kThreads, kSmemBytes<D, NT>, stream>>>(p);
+    return cudaGetLastError();
+}
+
 template <int D, int NT, bool kBf16>
-void launch(const Params& p, bool change, unsigned items, cudaStream_t stream) {
-    if (change) paged_kernel<D, NT, kBf16, true><<<items * p.splits, kThreads, 0, stream>>>(p);
-    else paged_kernel<D, NT, kBf16, false><<<items * p.splits, kThreads, 0, stream>>>(p);
-    if (p.splits > 1) join_kernel<D, NT, kBf16><<<items, 256, 0, stream>>>(p);
+cudaError_t launch(const Params& p, bool change, unsigned items, int device, cudaStream_t stream) {
+    cudaError_t err = change ? launch_one<D, NT, kBf16, true>(p, items, device, stream)
+                             : launch_one<D, NT, kBf16, false>(p, items, device, stream);
+    if (err != cudaSuccess || p.splits == 1) return err;
+    // Programmatic dependent launch: the join's launch overlaps the last chunks.
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(items);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, join_kernel<D, NT, kBf16>, p);
 }
 
 inline cudaError_t paged_entry(bool bf16, const void* q, long long q_stride, void* out, long long out_stride, int n_tokens,
@@ -575,7 +652,7 @@ inline cudaError_t paged_entry(bool bf16, const void* q, long long q_stride, voi
     p.softcap = softcap;
     p.slopes = slopes;
     // Chunks: enough CTAs for several rounds of the GPU, at least 128 tokens each.
-    const long long want = (12LL * sm_count + items - 1) / items;
+    const long long want = (kCtasPerSm * static_cast<long long>(sm_count) + items - 1) / items;
     const long long most = (max_seq_len + 127LL) / 128;
     long long splits = want < most ? want : most;
     if (splits < 1) splits = 1;
@@ -597,18 +674,18 @@ inline cudaError_t paged_entry(bool bf16, const void* q, long long q_stride, voi
     const unsigned count = static_cast<unsigned>(items);
     const int kind = (dim == 128 ? 4 : 0) + (nt == 2 ? 2 : 0) + (bf16 ? 1 : 0);
     switch (kind) {
-        case 0: launch<64, 1, false>(p, change, count, stream); break;
-        case 1: launch<64, 1, true>(p, change, count, stream); break;
-        case 2: launch<64, 2, false>(p, change, count, stream); break;
-        case 3: launch<64, 2, true>(p, change, count, stream); break;
-        case 4: launch<128, 1, false>(p, change, count, stream); break;
-        case 5: launch<128, 1, true>(p, change, count, stream); break;
-        case 6: launch<128, 2, false>(p, change, count, stream); break;
-        default: launch<128, 2, true>(p, change, count, stream); break;
+        case 0: err = launch<64, 1, false>(p, change, count, device, stream); break;
+        case 1: err = launch<64, 1, true>(p, change, count, device, stream); break;
+        case 2: err = launch<64, 2, false>(p, change, count, device, stream); break;
+        case 3: err = launch<64, 2, true>(p, change, count, device, stream); break;
+        case 4: err = launch<128, 1, false>(p, change, count, device, stream); break;
+        case 5: err = launch<128, 1, true>(p, change, count, device, stream); break;
+        case 6: err = launch<128, 2, false>(p, change, count, device, stream); break;
+        default: err = launch<128, 2, true>(p, change, count, device, stream); break;
     }
-    err = cudaGetLastError();
     if (scratch != nullptr) cudaFreeAsync(scratch, stream);
-    return err;
+    if (err != cudaSuccess) return err;
+    return cudaGetLastError();
 }
 
 }  // namespace paged

@@ -110,39 +110,98 @@ __device__ __forceinline__ int upper_bound(const int* ends, int n, int x) {
     return lo;
 }
 
-// One cluster of CTAs. Requests are taken 1024 at a time: every CTA computes the two
-// prefix sums (new tokens, pages needed) of the same 1024 requests for itself, and
-// the CTAs share out the slots and table entries. Only CTA 0 writes the lengths; the
-// cluster barrier before that lets lens_out be the array the others have read.
+// 1024 requests and what their tokens and pages get, in shared memory.
+struct PlanPart {
+    int ends[kPlanThreads];   // running new tokens, clamped to INT_MAX
+    int upto[kPlanThreads];   // running pages needed, clamped
+    int shift[kPlanThreads];  // position of token t of the call: t + shift
+    int have[kPlanThreads];   // pages held before
+    int base[kPlanThreads];   // number in the call of the page of column c: c + base
+    int taken[kPlanThreads];
+    long long warp_sums[32];
+    int used;                 // pages taken so far
+};
+
+__device__ __forceinline__ int clamp_int(long long x) { return static_cast<int>(min(x, static_cast<long long>(INT_MAX))); }
+
+// Table entries and slots of requests r0 .. r0 + here, whose tokens are [tokens, tokens +
+// sum) and whose pages [pages, pages + page_sum) of the call, shared out over `ctas` CTAs.
+// A warp writes one stretch of consecutive slots, so it searches for its request once, and
+// again only where a request ends; four slots a lane are in flight, since each waits for a
+// page number from L2.
+__device__ __forceinline__ void plan_fill(const PlanParams& p, const PlanPart& part, int r0, int here, long long tokens,
+                                          long long sum, long long pages, long long page_sum, int n_free, int rank, int ctas) {
+    const int tid = static_cast<int>(threadIdx.x);
+    const int lane = static_cast<int>(lane_id());
+    const bool pow2 = (p.page & (p.page - 1)) == 0;
+    const int shift = 31 - __clz(p.page);
+    // Page number k of the call goes to the request whose range holds it.
+    const int last_page = static_cast<int>(min(pages + page_sum, static_cast<long long>(n_free)));
+    for (long long k = pages + rank * kPlanThreads + tid; k < last_page; k += ctas * kPlanThreads) {
+        const int i = upper_bound(part.upto, here, static_cast<int>(k));
+        if (i < here && part.taken[i])
+            p.table[static_cast<long long>(r0 + i) * p.width + (k - part.base[i])] = __ldg(p.free_pages + (n_free - 1 - k));
+    }
+    const long long last_token = min(tokens + sum, static_cast<long long>(p.max_tokens));
+    const int warps = ctas * (kPlanThreads / 32);
+    const long long each = last_token > tokens ? ((last_token - tokens + warps - 1) / warps + 127) / 128 * 128 : 0;
+    const long long from = tokens + each * (rank * (kPlanThreads / 32) + (tid >> 5));
+    const long long to = min(from + each, last_token);
+    int i = from < to ? upper_bound(part.ends, here, static_cast<int>(from)) : 0;
+    for (long long t0 = from; t0 < to; t0 += 128) {
+        const int first = static_cast<int>(t0), last = static_cast<int>(min(t0 + 128, to)) - 1;
+        while (i < here && part.ends[i] <= first) ++i;
+        const bool one = i < here && part.ends[i] > last;  // all of them belong to request i
+        int owner[4], place[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int t = first + 32 * u + lane;
+            owner[u] = -1;
+            place[u] = 0;
+            if (t > last) continue;
+            const int q = one ? i : upper_bound(part.ends, here, t);
+            if (q >= here || !part.taken[q]) continue;
+            const int pos = t + part.shift[q];
+            const int col = pow2 ? pos >> shift : pos / p.page;
+            place[u] = pos - col * p.page;
+            owner[u] = col < part.have[q] ? p.table[static_cast<long long>(r0 + q) * p.width + col]
+                                          : __ldg(p.free_pages + (n_free - 1 - (col + part.base[q])));
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int t = first + 32 * u + lane;
+            if (t <= last) p.slots[t] = owner[u] >= 0 ? static_cast<long long>(owner[u]) * p.page + place[u] : -1;
+        }
+    }
+}
+
+// Slots behind the last token stand for nothing.
+__device__ __forceinline__ void plan_rest(const PlanParams& p, long long tokens, int rank, int ctas) {
+    for (long long t = tokens + rank * kPlanThreads + threadIdx.x; t < p.max_tokens; t += ctas * kPlanThreads) p.slots[t] = -1;
+}
+
+// One CTA, requests 1024 at a time:
 //
 //   need_r  = ceil((c_r + n_r) / page) - ceil(c_r / page)
 //   taken_r = n_r > 0, the row and the slots are wide enough, and need_r = 0 or
 //             need_0 + .. + need_r <= n_free
 //   page k of the call = free_pages[n_free - 1 - k]
 //
-// What bounds it: one launch and the chain lengths -> sums -> entries; the bytes are
-// a few MB at most (8 per slot). Each warp writes one stretch of consecutive slots, so
-// it searches for its request once and again only where a request ends; four slots a
-// lane are in flight, since each waits for a page number from L2.
+// Two prefix sums (new tokens, pages needed), the lengths, and with kFill the entries and
+// slots too. Without it plan_fill_kernel follows with as many CTAs as the slots need. It
+// works from this kernel's outputs alone, so no scratch is passed between the two.
+// What bounds both: the launches and the chain lengths -> sums -> entries; the bytes are a
+// few MB at most (8 a slot). 1024 requests with 385,000 tokens: 39 us when one cluster of
+// 8 CTAs did all of it (8 SMs wait for their page numbers), 12.5 us in two kernels.
+template <bool kFill>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
-    __shared__ long long warp_sums[32];
-    __shared__ int s_ends[kPlanThreads];   // running new tokens, clamped to INT_MAX
-    __shared__ int s_upto[kPlanThreads];   // running pages needed, clamped
-    __shared__ int s_shift[kPlanThreads];  // position of token t of the call: t + shift
-    __shared__ int s_have[kPlanThreads];   // pages held before
-    __shared__ int s_base[kPlanThreads];   // number in the call of the page of column c: c + base
-    __shared__ int s_taken[kPlanThreads];
-    __shared__ int s_used;
+    __shared__ PlanPart part;
     const int tid = static_cast<int>(threadIdx.x);
-    const int lane = static_cast<int>(lane_id());
-    const int rank = static_cast<int>(blockIdx.x);
-    const int ctas = static_cast<int>(gridDim.x);
+    if constexpr (!kFill) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int n_free = *p.n_free;
     n_free = n_free < 0 ? 0 : (n_free > p.free_capacity ? p.free_capacity : n_free);
-    if (tid == 0) s_used = 0;
-    const bool pow2 = (p.page & (p.page - 1)) == 0;
-    const int shift = 31 - __clz(p.page);
-    auto column_of = [&](int pos) { return pow2 ? pos >> shift : pos / p.page; };
+    if (tid == 0) part.used = 0;
+    __syncthreads();
     long long tokens = 0, pages = 0;  // sums over the earlier requests
     for (int r0 = 0; r0 < p.n_requests; r0 += kPlanThreads) {
         const int r = r0 + tid;
@@ -151,88 +210,101 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
             c = max(p.cached[r], 0);
             n = max(p.fresh[r], 0);
         }
-        long long sum;
-        const long long end = tokens + block_scan(n, warp_sums, sum);
+        long long sum, page_sum;
+        const long long end = tokens + block_scan(n, part.warp_sums, sum);
         const long long whole = static_cast<long long>(c) + n;
         const int have = static_cast<int>((static_cast<long long>(c) + p.page - 1) / p.page);
         const bool fits = n > 0 && whole <= static_cast<long long>(p.width) * p.page && end <= p.max_tokens;
         const int need = fits ? static_cast<int>((whole + p.page - 1) / p.page) - have : 0;
-        long long page_sum;
-        const long long upto = pages + block_scan(need, warp_sums, page_sum);
+        const long long upto = pages + block_scan(need, part.warp_sums, page_sum);
         const bool taken = fits && (need == 0 || upto <= n_free);
-        s_ends[tid] = static_cast<int>(min(end, static_cast<long long>(INT_MAX)));
-        s_upto[tid] = static_cast<int>(min(upto, static_cast<long long>(INT_MAX)));
-        // Only read where taken: then end <= max_tokens and, if pages are needed, upto <= n_free.
-        s_shift[tid] = c - static_cast<int>(end - n);
-        s_have[tid] = have;
-        s_base[tid] = static_cast<int>(upto - need) - have;
-        s_taken[tid] = taken ? 1 : 0;
-        if (taken && need > 0) atomicMax(&s_used, static_cast<int>(upto));
-        if (ctas > 1) cluster_sync(); else __syncthreads();
-        if (rank == 0 && r < p.n_requests) {
+        if (taken && need > 0) atomicMax(&part.used, static_cast<int>(upto));
+        if (r < p.n_requests) {
+            // Each thread has read its own request: lens_out may be `cached`.
             p.lens_out[r] = taken ? static_cast<int>(whole) : c;
             p.seq_lens[r] = taken ? static_cast<int>(whole) : 0;
-            p.starts[r] = static_cast<int>(min(end - n, static_cast<long long>(INT_MAX)));
+            p.starts[r] = clamp_int(end - n);
         }
-        const int here = min(kPlanThreads, p.n_requests - r0);
-        // Table entries: page number k of the call goes to the request whose range holds it.
-        const int last_page = static_cast<int>(min(pages + page_sum, static_cast<long long>(n_free)));
-        for (long long k = pages + rank * kPlanThreads + tid; k < last_page; k += ctas * kPlanThreads) {
-            const int i = upper_bound(s_upto, here, static_cast<int>(k));
-            if (i < here && s_taken[i])
-                p.table[static_cast<long long>(r0 + i) * p.width + (k - s_base[i])] = p.free_pages[n_free - 1 - k];
-        }
-        // Slots, a stretch of whole 128s for each warp of the cluster.
-        const long long last_token = min(tokens + sum, static_cast<long long>(p.max_tokens));
-        const int warps = ctas * (kPlanThreads / 32);
-        const long long each = last_token > tokens ? ((last_token - tokens + warps - 1) / warps + 127) / 128 * 128 : 0;
-        const long long from = tokens + each * (rank * (kPlanThreads / 32) + (tid >> 5));
-        const long long to = min(from + each, last_token);
-        int i = from < to ? upper_bound(s_ends, here, static_cast<int>(from)) : 0;
-        for (long long t0 = from; t0 < to; t0 += 128) {
-            const int first = static_cast<int>(t0), last = static_cast<int>(min(t0 + 128, to)) - 1;
-            while (i < here && s_ends[i] <= first) ++i;
-            const bool one = i < here && s_ends[i] > last;  // all of them belong to request i
-            int owner[4], place[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int t = first + 32 * u + lane;
-                owner[u] = -1;
-                place[u] = 0;
-                if (t > last) continue;
-                const int q = one ? i : upper_bound(s_ends, here, t);
-                if (q >= here || !s_taken[q]) continue;
-                const int pos = t + s_shift[q];
-                const int col = column_of(pos);
-                place[u] = pos - col * p.page;
-                owner[u] = col < s_have[q] ? p.table[static_cast<long long>(r0 + q) * p.width + col]
-                                           : __ldg(p.free_pages + (n_free - 1 - (col + s_base[q])));
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int t = first + 32 * u + lane;
-                if (t <= last) p.slots[t] = owner[u] >= 0 ? static_cast<long long>(owner[u]) * p.page + place[u] : -1;
-            }
+        if constexpr (kFill) {
+            part.ends[tid] = clamp_int(end);
+            part.upto[tid] = clamp_int(upto);
+            // Only read where taken: then end <= max_tokens and, if pages are needed, upto <= n_free.
+            part.shift[tid] = c - static_cast<int>(end - n);
+            part.have[tid] = have;
+            part.base[tid] = static_cast<int>(upto - need) - have;
+            part.taken[tid] = taken ? 1 : 0;
+            __syncthreads();
+            plan_fill(p, part, r0, min(kPlanThreads, p.n_requests - r0), tokens, sum, pages, page_sum, n_free, 0, 1);
+            __syncthreads();  // the shared arrays are rewritten by the next 1024 requests
         }
         tokens += sum;
         pages += page_sum;
-        __syncthreads();  // the shared arrays are rewritten by the next 1024 requests
     }
-    // Slots behind the last token stand for nothing.
-    for (long long t = tokens + rank * kPlanThreads + tid; t < p.max_tokens; t += ctas * kPlanThreads) p.slots[t] = -1;
-    // Every CTA has read *n_free before its first barrier; with no request there was none.
-    if (p.n_requests == 0) {
-        if (ctas > 1) cluster_sync(); else __syncthreads();
-    }
-    if (rank == 0 && tid == 0) {
-        p.starts[p.n_requests] = static_cast<int>(min(tokens, static_cast<long long>(INT_MAX)));
-        *p.n_free_out = n_free - s_used;
+    __syncthreads();
+    if constexpr (kFill) plan_rest(p, tokens, 0, 1);
+    if (tid == 0) {
+        p.starts[p.n_requests] = clamp_int(tokens);
+        *p.n_free_out = n_free - part.used;  // read by this CTA alone, at its start
     }
 }
 
-// One CTA up to this many slots and requests, above them the largest portable cluster.
+// The table entries and slots that follow from plan_kernel's outputs: a request is taken if
+// its seq_lens is not 0; then it held lens_out - new tokens. The taken requests that need
+// pages are the first ones that do, so the sum of their needs is what n_free went down by.
+__global__ void __launch_bounds__(kPlanThreads) plan_fill_kernel(const PlanParams p) {
+    __shared__ PlanPart part;
+    const int tid = static_cast<int>(threadIdx.x);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // The pages taken in all: free_pages counts from the n_free before the call.
+    long long used = 0;
+    for (int r0 = 0; r0 < p.n_requests; r0 += kPlanThreads) {
+        const int r = r0 + tid;
+        int need = 0;
+        if (r < p.n_requests && p.seq_lens[r] > 0) {
+            const int whole = p.lens_out[r], c = whole - p.fresh[r];
+            need = static_cast<int>((static_cast<long long>(whole) + p.page - 1) / p.page - (static_cast<long long>(c) + p.page - 1) / p.page);
+        }
+        long long page_sum;
+        block_scan(need, part.warp_sums, page_sum);
+        used += page_sum;
+    }
+    const int n_free = *p.n_free_out + static_cast<int>(used);
+    long long tokens = 0, pages = 0;
+    for (int r0 = 0; r0 < p.n_requests; r0 += kPlanThreads) {
+        const int r = r0 + tid;
+        int c = 0, n = 0, whole = 0;
+        bool taken = false;
+        long long end = INT_MAX;
+        if (r < p.n_requests) {
+            n = max(p.fresh[r], 0);
+            taken = p.seq_lens[r] > 0;
+            whole = p.lens_out[r];
+            c = taken ? whole - n : whole;
+            end = static_cast<long long>(p.starts[r]) + n;
+        }
+        const int have = static_cast<int>((static_cast<long long>(c) + p.page - 1) / p.page);
+        const int need = taken ? static_cast<int>((static_cast<long long>(whole) + p.page - 1) / p.page) - have : 0;
+        long long page_sum;
+        const long long upto = pages + block_scan(need, part.warp_sums, page_sum);
+        part.ends[tid] = clamp_int(end);
+        part.upto[tid] = clamp_int(upto);
+        part.shift[tid] = c - static_cast<int>(end - n);
+        part.have[tid] = have;
+        part.base[tid] = static_cast<int>(upto - need) - have;
+        part.taken[tid] = taken ? 1 : 0;
+        __syncthreads();
+        const int here = min(kPlanThreads, p.n_requests - r0);
+        const long long sum = part.ends[here - 1] - tokens;
+        plan_fill(p, part, r0, here, tokens, sum, pages, page_sum, n_free, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+        __syncthreads();
+        tokens += sum;
+        pages += page_sum;
+    }
+    plan_rest(p, tokens, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+}
+
+// Up to this many slots and requests in one kernel of one CTA.
 constexpr int kPlanOneCta = 4096;
-constexpr int kPlanCluster = 8;
 
 inline cudaError_t plan_entry(const int* cached, const int* fresh, int n_requests, int page, int* table, int width,
                               const int* free_pages, int free_capacity, const int* n_free, int* lens_out, int* seq_lens,
@@ -257,24 +329,30 @@ inline cudaError_t plan_entry(const int* cached, const int* fresh, int n_request
         for (int j = i + 1; j < 6; ++j)
             if (host::ranges_overlap(out[i].p, out[i].n, out[j].p, out[j].n)) return cudaErrorInvalidValue;
     }
-    cudaError_t err = host::current_device(nullptr, nullptr);
+    int sm_count = 0;
+    cudaError_t err = host::current_device(nullptr, &sm_count);
     if (err != cudaSuccess) return err;
     static_cast<void>(cudaGetLastError());
     PlanParams p{cached, fresh, n_requests, page, table, width, free_pages, free_capacity, n_free,
                  lens_out, seq_lens, starts, slots, max_tokens, n_free_out};
-    const unsigned ctas = max_tokens <= kPlanOneCta && n_requests <= kPlanOneCta ? 1 : kPlanCluster;
+    if (max_tokens <= kPlanOneCta && n_requests <= kPlanOneCta) {
+        plan_kernel<true><<<1, kPlanThreads, 0, stream>>>(p);
+        return cudaGetLastError();
+    }
+    plan_kernel<false><<<1, kPlanThreads, 0, stream>>>(p);
+    // A warp writes 128 slots at a time; programmatic dependent launch: this launch overlaps
+    // the first kernel.
+    const int want = (max_tokens + 4095) / 4096;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas);
+    cfg.gridDim = dim3(static_cast<unsigned>(want < 1 ? 1 : (want < sm_count ? want : sm_count)));
     cfg.blockDim = dim3(kPlanThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ctas;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    err = cudaLaunchKernelEx(&cfg, plan_kernel, p);
+    err = cudaLaunchKernelEx(&cfg, plan_fill_kernel, p);
     if (err != cudaSuccess) return err;
     return cudaGetLastError();
 }
@@ -332,16 +410,10 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
-// x / s; by the reciprocal where s is a power of two (then both are the same value).
-struct Divider {
-    float s, inv;
-    bool exact;
-    __device__ __forceinline__ explicit Divider(float scale) : s(scale) {
-        exact = (__float_as_uint(scale) & 0x7fffffu) == 0 && scale >= 7.9e-31f && scale < 1.7e38f;
-        inv = exact ? 1.0f / scale : 0.0f;
-    }
-    __device__ __forceinline__ float operator()(float x) const { return exact ? x * inv : __fdiv_rn(x, s); }
-};
+// Whether x * (1 / s) is x / s: s a power of two with a normal reciprocal.
+__device__ __forceinline__ bool exact_reciprocal(float s) {
+    return (__float_as_uint(s) & 0x7fffffu) == 0 && s >= 7.9e-31f && s < 1.7e38f;
+}
 
 // A run is a stretch of consecutive tokens whose slots are consecutive places of one
 // page. One warp (or, kCta, the four warps of a CTA together) takes one run of one
@@ -454,19 +526,18 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
                     *reinterpret_cast<uint4*>(bytes + b) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
-            const Divider over(now);
-            for (int j0 = 0; j0 < n; j0 += kRows * kHeld) {
-                if (n > kRows * kHeld) {  // else the registers still hold the run
+            auto store = [&](auto over) {
+                for (int j0 = 0; j0 < n; j0 += kRows * kHeld) {
+                    if (n > kRows * kHeld) {  // else the registers still hold the run
+#pragma unroll
+                        for (int u = 0; u < kHeld; ++u) {
+                            const int j = j0 + u * kRows + sub;
+                            if (j < n) held[u] = __ldg(reinterpret_cast<const uint4*>(rows + j * stride));
+                        }
+                    }
+                    uint8_t* at = bytes + (place + j0 + sub) * kDim + col;
 #pragma unroll
                     for (int u = 0; u < kHeld; ++u) {
-                        const int j = j0 + u * kRows + sub;
-                        if (j < n) held[u] = __ldg(reinterpret_cast<const uint4*>(rows + j * stride));
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < kHeld; ++u) {
-                    const int j = j0 + u * kRows + sub;
-                    if (j < n) {
                         const uint32_t w[4] = {held[u].x, held[u].y, held[u].z, held[u].w};
                         uint32_t b[4];
 #pragma unroll
@@ -474,9 +545,17 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
                             const float2 f = pair_to_float2<kBf16>(w[c]);
                             b[c] = to_e4m3x2(over(f.x), over(f.y));
                         }
-                        *reinterpret_cast<uint2*>(bytes + (place + j) * kDim + col) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+                        if (j0 + u * kRows + sub < n)
+                            *reinterpret_cast<uint2*>(at + u * kRows * kDim) =
+                                make_uint2(__byte_perm(b[0], b[1], 0x5410), __byte_perm(b[2], b[3], 0x5410));
                     }
                 }
+            };
+            if (exact_reciprocal(now)) {
+                const float inv = 1.0f / now;
+                store([inv](float f) { return f * inv; });
+            } else {  // a page's older scale that this library did not choose
+                store([now](float f) { return __fdiv_rn(f, now); });
             }
             if (in_group == 0) scales[tile] = now;
         }
