@@ -30,8 +30,10 @@
 // does not fit the registers. The ring's 16-byte pieces are swizzled so that both the
 // K reads (rows g, pieces 2t) and the V reads (rows 2t, pieces g) hit distinct banks.
 //
-// Long contexts are cut into `splits` chunks, each a CTA of its own, whose (max, sum, O)
-// a second kernel joins in chunk order: results do not depend on timing.
+// Long contexts are cut into `splits` chunks, each a CTA of its own. Up to 8 chunks of one
+// (request, key head, row tile) form a cluster that joins their (point, sum, O) through
+// distributed shared memory; more of them leave theirs in scratch, and a second kernel
+// joins those. Either way in chunk order: results do not depend on timing.
 #pragma once
 
 #include <atomic>
@@ -46,8 +48,21 @@ using attn::ex2;
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kStep = 16;       // tokens per warp step
-constexpr int kCtasPerSm = 24;
+// A warp step is kSub blocks of 16 tokens: 4 KB of cache, either way.
+template <int D>
+constexpr int kSub = 128 / D;
+template <int D>
+constexpr int kStep = 16 * kSub<D>;
+template <int D>
+constexpr int kStageBytes = kStep<D> * 2 * D;
+constexpr int kStages = 3;
+constexpr int kMaxCluster = 8;
+#ifndef TK_PAGED_ROUNDS
+#define TK_PAGED_ROUNDS 6
+#endif
+#ifndef TK_PAGED_CLUSTER_BYTES
+#define TK_PAGED_CLUSTER_BYTES 131072
+#endif
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are held in binary16 as 2^(x - m + kLift), with the reference point m
 // at most 8 below the row's max: at most 2^15, so that binary16 keeps 11 bits down to
@@ -74,8 +89,10 @@ struct Params {
     int splits, chunk;  // chunks per (request, key head, tile), and tokens in each (the last takes the rest)
     float scale, softcap;
     const float* slopes;
-    float* part_o;      // [item][rows][D], unnormalised, splits > 1
+    bool cluster;       // the chunks of an item are one cluster
+    float* part_o;      // [item][rows][D], unnormalised; or null
     float2* part_ml;    // [item][rows]: reference point (log2 units), sum
+    int join_runs, join_ctas;
 };
 
 struct Request {
@@ -140,31 +157,30 @@ __device__ __forceinline__ uint32_t piece_at(int r, int c) {
     return (r >> 1) * 128 + ((((r & 1) * 4 + c) ^ (kV ? r & 6 : 0)) << 4);
 }
 
-// What comes with 16 tokens in registers.
-struct Step {
+// What comes with a block of 16 tokens in registers.
+struct Block {
     float ks, vs;
     bool on;  // the page is there
 };
 
 template <int D>
-__device__ __forceinline__ void load_step(Step& st, uint32_t stage, const Params& p, int head, int page, int token, int lane) {
-    st.on = page >= 0 && page < p.n_pages;
-    if (st.on) {
+__device__ __forceinline__ void load_block(Block& bl, uint32_t stage, const Params& p, int head, int page, int token, int lane) {
+    bl.on = page >= 0 && page < p.n_pages;
+    if (bl.on) {
         const long long tile = static_cast<long long>(page) * p.heads_kv + head;
-        const long long at = (tile * p.page + (token & (p.page - 1))) * D + lane * 16;
+        const long long at = ((tile << p.page_shift) + (token & (p.page - 1))) * D + lane * 16;
         constexpr int kPieces = D / 16;             // of a token
         constexpr int kRows = 32 / kPieces;         // tokens per instruction
         const int r = lane / kPieces, c = lane % kPieces;
+        const uint8_t* k = p.k_cache + at;
+        const uint8_t* v = p.v_cache + at;
 #pragma unroll
-        for (int i = 0; i < kStep / kRows; ++i)
-            cp_async_16(stage + piece_at<D, false>(r + i * kRows, c), p.k_cache + at + i * 512);
+        for (int i = 0; i < 16 / kRows; ++i) cp_async_16(stage + piece_at<D, false>(r + i * kRows, c), k + i * 512);
 #pragma unroll
-        for (int i = 0; i < kStep / kRows; ++i)
-            cp_async_16(stage + kStep * D + piece_at<D, true>(r + i * kRows, c), p.v_cache + at + i * 512);
-        st.ks = __ldg(p.k_scale + tile);
-        st.vs = __ldg(p.v_scale + tile);
+        for (int i = 0; i < 16 / kRows; ++i) cp_async_16(stage + 16 * D + piece_at<D, true>(r + i * kRows, c), v + i * 512);
+        bl.ks = __ldg(p.k_scale + tile);
+        bl.vs = __ldg(p.v_scale + tile);
     }
-    cp_async_commit();
 }
 
 // What one lane knows of its 2 NT score columns (rows 8 nt + 2 t + {0, 1}).
@@ -193,21 +209,55 @@ __device__ __forceinline__ uint16_t out_bits(float x) {
     }
 }
 
-template <int D>
-constexpr int kStages = D == 128 ? 3 : 4;
+// (point, sum, O) of a row, merged one by one in a fixed order.
+struct Merged {
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    __device__ __forceinline__ void add(float2 ml, float4 v) {
+        if (ml.x == -INFINITY) return;
+        const float now = fmaxf(m, ml.x);
+        const float a = ex2(m - now), b = ex2(ml.x - now);  // 0 for the first: m is -inf
+        m = now;
+        l = l * a + ml.y * b;
+        o.x = o.x * a + v.x * b;
+        o.y = o.y * a + v.y * b;
+        o.z = o.z * a + v.z * b;
+        o.w = o.w * a + v.w * b;
+    }
+};
+
+template <int D, bool kBf16>
+__device__ __forceinline__ void write_out(const Params& p, const Request& rq, int head, int row, int col, const Merged& x) {
+    const float inv = x.l > 0.0f ? __frcp_rn(x.l) : 0.0f;  // a row without a key is 0
+    uint16_t* dst = p.out + (rq.first + row / p.group) * p.out_stride + (head * p.group + row % p.group) * D + col;
+    uint2 w;
+    w.x = out_bits<kBf16>(x.o.x * inv) | static_cast<uint32_t>(out_bits<kBf16>(x.o.y * inv)) << 16;
+    w.y = out_bits<kBf16>(x.o.z * inv) | static_cast<uint32_t>(out_bits<kBf16>(x.o.w * inv)) << 16;
+    *reinterpret_cast<uint2*>(dst) = w;
+}
+
+// Shared memory: the warps' rings; after the loop, in their place, each warp's O rows (D + 4
+// floats apart: rows 2t of a store fall on other banks), its (point, sum), and the CTA's.
 template <int D, int NT>
-constexpr int kSmemBytes = kWarps * kStages<D> * kStep * 2 * D > kWarps * 8 * NT * ((D + 4) * 4 + 8)
-                               ? kWarps * kStages<D> * kStep * 2 * D : kWarps * 8 * NT * ((D + 4) * 4 + 8);
+struct Smem {
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kPitch = D + 4;
+    static constexpr int kMl = kWarps * kRows * kPitch * 4;
+    static constexpr int kCtaO = kMl + kWarps * kRows * 8;
+    static constexpr int kCtaMl = kCtaO + kRows * D * 4;
+    static constexpr int kAfter = kCtaMl + kRows * 8;
+    static constexpr int kRings = kWarps * kStages * kStageBytes<D>;
+    static constexpr int kBytes = kRings > kAfter ? kRings : kAfter;
+};
 
 template <int D, int NT, bool kBf16, bool kChange>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const Params p) {
     constexpr int kRows = 8 * NT;
     constexpr int kM = D / 16;          // MMA tiles of output dims; k-steps of S^T
-    constexpr int kPitch = D + 4;       // floats: rows 2t of a store fall on other banks
+    using S = Smem<D, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
-    // After the loop the rings' memory holds each warp's O, and the (point, sum) of its rows.
-    float (*s_o)[kRows][kPitch] = reinterpret_cast<float (*)[kRows][kPitch]>(smem);
-    float2 (*s_ml)[kRows] = reinterpret_cast<float2 (*)[kRows]>(smem + kWarps * kRows * kPitch * 4);
+    float (*s_o)[kRows][S::kPitch] = reinterpret_cast<float (*)[kRows][S::kPitch]>(smem);
+    float2 (*s_ml)[kRows] = reinterpret_cast<float2 (*)[kRows]>(smem + S::kMl);
 
     const int lane = static_cast<int>(lane_id());
     const int warp = static_cast<int>(threadIdx.x >> 5);
@@ -219,15 +269,50 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
     rest /= p.tiles;
     const int head = rest % p.heads_kv;
     const int r = rest / p.heads_kv;
+    // The chain to the first bytes of cache is lengths -> pages -> cache. Which table entries a
+    // warp starts with does not depend on the lengths: they are fetched together.
+    constexpr int kB = kSub<D>;
+    constexpr int kStride = kWarps * kStep<D>;
+    const int begin = split * p.chunk;
+    const int* table = p.table + static_cast<long long>(r) * p.width;
+    int page_of[kStages][kB];
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
+#pragma unroll
+        for (int u = 0; u < kB; ++u) {
+            const int col = (begin + (i * kWarps + warp) * kStep<D> + 16 * u) >> p.page_shift;
+            page_of[i][u] = col < p.width ? __ldg(table + col) : -1;
+        }
+    }
     const Request rq = request_of(p, r);
     const int n_rows = min(kRows, rq.n * p.group - tile * kRows);  // of this tile
     if (n_rows <= 0) return;
     // Keys up to the last row's position.
     const int last_pos = rq.len - rq.n + (tile * kRows + n_rows - 1) / p.group;
     const int kv_end = max(last_pos + 1, 0);
-    const int begin = split * p.chunk;
     const int end = split == p.splits - 1 ? kv_end : min(kv_end, begin + p.chunk);
-    if (begin >= end && split > 0) return;
+    if (begin >= end && split > 0 && !p.cluster) return;
+
+    // Warp w takes steps w, w + 4, ... of the chunk; kStages - 1 of them are in flight.
+    const uint32_t ring = smem_u32(smem) + warp * (kStages * kStageBytes<D>);
+    Block blocks[kStages][kB];
+    int token = begin + warp * kStep<D>;
+    int load_token = token;
+    int next_page[kB];
+    auto page_at = [&](int at) { return at < end ? __ldg(table + (at >> p.page_shift)) : -1; };
+    auto load_pages = [&](Block (&bl)[kB], const int (&pages)[kB], int stage) {
+#pragma unroll
+        for (int u = 0; u < kB; ++u) {
+            const int at = load_token + 16 * u;
+            load_block<D>(bl[u], ring + stage * kStageBytes<D> + u * 32 * D, p, head, at < end ? pages[u] : -1, at, lane);
+        }
+        cp_async_commit();
+        load_token += kStride;
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) load_pages(blocks[i], page_of[i], i);
+#pragma unroll
+    for (int u = 0; u < kB; ++u) next_page[u] = page_of[kStages - 1][u];
 
     // Q as B operand: row g of each 8, dims [D/4 t, D/4 (t + 1)).
     uint32_t q[NT][2 * kM];
@@ -298,46 +383,55 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
     // so that probabilities times page scale / unit stay in binary16's range.
     float v_unit = 0.0f, v_over = 0.0f;
 
-    const int* table = p.table + static_cast<long long>(r) * p.width;
-    auto page_at = [&](int token) { return token < end ? __ldg(table + (token >> p.page_shift)) : -1; };
-
-    auto compute = [&](const Step& st, uint32_t stage, int token) {
-        if (!st.on) return;  // no such page: as if its tokens were not there
-        float s[NT][4];
+    auto compute = [&](const Block (&bl)[kB], uint32_t stage, int token) {
+        float s[kB][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int u = 0; u < kB; ++u) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) s[nt][c] = 0.0f;
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-            uint32_t near[4], far[4];  // tokens g and g + 8
-            load_shared(near, stage + piece_at<D, false>(g, t * (D / 64) + c));
-            load_shared(far, stage + piece_at<D, false>(g + 8, t * (D / 64) + c));
+                for (int c = 0; c < 4; ++c) s[u][nt][c] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int w = 4 * c + i;
-                const uint32_t a0 = kv::from_e4m3x2(near[i] & 0xffffu), a2 = kv::from_e4m3x2(near[i] >> 16);
-                const uint32_t a1 = kv::from_e4m3x2(far[i] & 0xffffu), a3 = kv::from_e4m3x2(far[i] >> 16);
+            for (int c = 0; c < D / 64; ++c) {
+                uint32_t near[4], far[4];  // tokens g and g + 8
+                const uint32_t k = stage + u * 32 * D;
+                load_shared(near, k + piece_at<D, false>(g, t * (D / 64) + c));
+                load_shared(far, k + piece_at<D, false>(g + 8, t * (D / 64) + c));
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt], a0, a1, a2, a3, q[nt][2 * w], q[nt][2 * w + 1]);
+                for (int i = 0; i < 4; ++i) {
+                    const int w = 4 * c + i;
+                    const uint32_t a0 = kv::from_e4m3x2(near[i] & 0xffffu), a2 = kv::from_e4m3x2(near[i] >> 16);
+                    const uint32_t a1 = kv::from_e4m3x2(far[i] & 0xffffu), a3 = kv::from_e4m3x2(far[i] >> 16);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_16816(s[u][nt], a0, a1, a2, a3, q[nt][2 * w], q[nt][2 * w + 1]);
+                }
             }
         }
-        const bool partial = token + kStep > end || token + kStep - 1 > first_pos;
+        bool partial = token + kStep<D> > end || token + kStep<D> - 1 > first_pos;
+#pragma unroll
+        for (int u = 0; u < kB; ++u) partial = partial || !bl[u].on;
         bool grow = false;
+        float unit = v_unit;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float x = s[nt][c] * (st.ks * rows.factor[nt][c & 1]);
-                const int j = token + g + (c >> 1) * 8;
-                if constexpr (kChange) {
-                    if (cap > 0.0f) x = cap * tanh_of(x * over_cap);
-                    x = fmaf(static_cast<float>(j - rows.pos[nt][c & 1]), rows.slope[nt][c & 1], x * kLog2e);
+            for (int u = 0; u < kB; ++u) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float x = s[u][nt][c] * (bl[u].ks * rows.factor[nt][c & 1]);
+                    const int j = token + 16 * u + g + (c >> 1) * 8;
+                    if constexpr (kChange) {
+                        if (cap > 0.0f) x = cap * tanh_of(x * over_cap);
+                        x = fmaf(static_cast<float>(j - rows.pos[nt][c & 1]), rows.slope[nt][c & 1], x * kLog2e);
+                    }
+                    // Without a page a block's tokens are not there, whatever the ring holds.
+                    if (partial && (!bl[u].on || j >= end || j > rows.pos[nt][c & 1])) x = -INFINITY;
+                    s[u][nt][c] = x;
+                    top[c & 1] = fmaxf(top[c & 1], x);
                 }
-                if (partial && (j >= end || j > rows.pos[nt][c & 1])) x = -INFINITY;
-                s[nt][c] = x;
             }
-            grow = grow || fmaxf(s[nt][0], s[nt][2]) > rows.m[nt][0] + 8.0f || fmaxf(s[nt][1], s[nt][3]) > rows.m[nt][1] + 8.0f;
+            grow = grow || top[0] > rows.m[nt][0] + 8.0f || top[1] > rows.m[nt][1] + 8.0f;
         }
         if (__any_sync(0xffffffffu, grow)) {
             // Move the reference points to the max so far.
@@ -345,7 +439,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float mx = fmaxf(s[nt][c], s[nt][c + 2]);
+                    float mx = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
+#pragma unroll
+                    for (int u = 1; u < kB; ++u) mx = fmaxf(mx, fmaxf(s[u][nt][c], s[u][nt][c + 2]));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -361,9 +457,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
                 }
             }
         }
-        if (st.vs > v_unit) {
-            const uint32_t bits = __float_as_uint(st.vs);
-            const float unit = __uint_as_float(((bits + 0x7fffffu) & 0xff800000u));  // the next power of two
+#pragma unroll
+        for (int u = 0; u < kB; ++u)
+            if (bl[u].on && bl[u].vs > unit)  // the next power of two
+                unit = __uint_as_float((__float_as_uint(bl[u].vs) + 0x7fffffu) & 0xff800000u);
+        if (unit > v_unit) {
             const float alpha = v_unit > 0.0f ? __fdiv_rn(v_unit, unit) : 1.0f;
             v_unit = unit;
             v_over = __fdiv_rn(1.0f, unit);
@@ -374,82 +472,77 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
 #pragma unroll
                     for (int c = 0; c < 4; ++c) o[nt][i][c] *= alpha;
         }
-        const float vr = st.vs * v_over;
-        uint32_t b[NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            float e[4];
+        for (int u = 0; u < kB; ++u) {
+            if (!bl[u].on) continue;
+            const float vr = bl[u].vs * v_over;
+            uint32_t b[NT][2];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float m = rows.m[nt][c & 1];
-                e[c] = ex2(s[nt][c] - (m == -INFINITY ? 0.0f : m) + kLift);
+            for (int nt = 0; nt < NT; ++nt) {
+                float e[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float m = rows.m[nt][c & 1];
+                    e[c] = ex2(s[u][nt][c] + (m == -INFINITY ? 0.0f : kLift - m));
+                }
+                rows.l[nt][0] += e[0] + e[2];
+                rows.l[nt][1] += e[1] + e[3];
+                b[nt][0] = transpose_8x8(attn::pack_half2(e[0] * vr, e[1] * vr));
+                b[nt][1] = transpose_8x8(attn::pack_half2(e[2] * vr, e[3] * vr));
             }
-            rows.l[nt][0] += e[0] + e[2];
-            rows.l[nt][1] += e[1] + e[3];
-            b[nt][0] = transpose_8x8(attn::pack_half2(e[0] * vr, e[1] * vr));
-            b[nt][1] = transpose_8x8(attn::pack_half2(e[2] * vr, e[3] * vr));
-        }
-        uint32_t v[4][D / 32];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
+            uint32_t v[4][D / 32];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
+            const uint32_t at = stage + u * 32 * D + 16 * D;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int r = 2 * t + (u & 1) + (u >> 1) * 8;
-            if constexpr (D == 128) load_shared(v[u], stage + kStep * D + piece_at<D, true>(r, g));
-            else load_shared(v[u], stage + kStep * D + piece_at<D, true>(r, g >> 1) + (g & 1) * 8);
-        }
-        if (token + kStep > end) {
-            // Places behind the last token hold anything, NaN included: they become 0.
+            for (int i = 0; i < 4; ++i) {
+                const int r = 2 * t + (i & 1) + (i >> 1) * 8;
+                if constexpr (D == 128) load_shared(v[i], at + piece_at<D, true>(r, g));
+                else load_shared(v[i], at + piece_at<D, true>(r, g >> 1) + (g & 1) * 8);
+            }
+            if (token + 16 * u + 16 > end) {
+                // Places behind the last token hold anything, NaN included: they become 0.
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (token + 2 * t + (u & 1) + (u >> 1) * 8 >= end)
+                for (int i = 0; i < 4; ++i)
+                    if (token + 16 * u + 2 * t + (i & 1) + (i >> 1) * 8 >= end)
 #pragma unroll
-                    for (int i = 0; i < D / 32; ++i) v[u][i] = 0;
-        }
+                        for (int w = 0; w < D / 32; ++w) v[i][w] = 0;
+            }
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            // Bytes 0..3 of a word: dims 4 i .. 4 i + 3 of the lane's D / 8.
+            for (int i = 0; i < D / 32; ++i) {
+                // Bytes 0..3 of a word: dims 4 i .. 4 i + 3 of the lane's D / 8.
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t pick = half == 0 ? 0x5140u : 0x7362u;
-                const uint32_t near = __byte_perm(v[0][i], v[1][i], pick), far = __byte_perm(v[2][i], v[3][i], pick);
-                const uint32_t a0 = kv::from_e4m3x2(near & 0xffffu), a1 = kv::from_e4m3x2(near >> 16);
-                const uint32_t a2 = kv::from_e4m3x2(far & 0xffffu), a3 = kv::from_e4m3x2(far >> 16);
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t pick = half == 0 ? 0x5140u : 0x7362u;
+                    const uint32_t near = __byte_perm(v[0][i], v[1][i], pick), far = __byte_perm(v[2][i], v[3][i], pick);
+                    const uint32_t a0 = kv::from_e4m3x2(near & 0xffffu), a1 = kv::from_e4m3x2(near >> 16);
+                    const uint32_t a2 = kv::from_e4m3x2(far & 0xffffu), a3 = kv::from_e4m3x2(far >> 16);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][2 * i + half], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][2 * i + half], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+                }
             }
         }
     };
 
-    // Warp w takes steps w, w + 4, ... of the chunk; kStages - 1 of them are in flight.
-    constexpr int kStride = kWarps * kStep;
-    constexpr int kRing = kStages<D>;
-    const uint32_t ring = smem_u32(smem) + warp * (kRing * kStep * 2 * D);
-    Step steps[kRing];
-    int token = begin + warp * kStep;
-    int load_token = token;
-    int next_page = page_at(load_token);
-    auto load_next = [&](Step& st, int stage) {
-        const int page = next_page;
-        const int at = load_token;
-        load_token += kStride;
-        next_page = page_at(load_token);
-        load_step<D>(st, ring + stage * (kStep * 2 * D), p, head, page, at, lane);
-    };
-#pragma unroll
-    for (int i = 0; i < kRing - 1; ++i) load_next(steps[i], i);
     while (token < end) {
 #pragma unroll
-        for (int i = 0; i < kRing; ++i) {
+        for (int i = 0; i < kStages; ++i) {
             if (token < end) {
-                cp_async_wait<kRing - 2>();
+                cp_async_wait<kStages - 2>();
                 __syncwarp();  // every lane's copies of this step have landed, and the step before is read
-                load_next(steps[(i + kRing - 1) % kRing], (i + kRing - 1) % kRing);
-                compute(steps[i], ring + i * (kStep * 2 * D), token);
+                constexpr int kAhead = kStages - 1;
+                int pages[kB];
+#pragma unroll
+                for (int u = 0; u < kB; ++u) {
+                    pages[u] = next_page[u];
+                    next_page[u] = page_at(load_token + kStride + 16 * u);
+                }
+                load_pages(blocks[(i + kAhead) % kStages], pages, (i + kAhead) % kStages);
+                compute(blocks[i], ring + i * kStageBytes<D>, token);
                 token += kStride;
             }
         }
     }
     cp_async_wait<0>();
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (!p.cluster) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __syncthreads();
 
     // Join the four warps, in warp order.
@@ -471,85 +564,106 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
     }
     __syncthreads();
     constexpr int kQuads = D / 4;
-    const long long item = item_of(p, r, head, tile, split);
+    const int row0 = tile * kRows;
     for (int i = static_cast<int>(threadIdx.x); i < kRows * kQuads; i += kThreads) {
         const int row = i / kQuads, col = (i % kQuads) * 4;
         if (row >= n_rows) break;
-        float m = -INFINITY;
+        Merged x;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ml[w][row].x);
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float2 ml = s_ml[w][row];
-            if (ml.x == -INFINITY) continue;
-            const float alpha = ex2(ml.x - m);
-            l += ml.y * alpha;
-            const float4 v = *reinterpret_cast<const float4*>(&s_o[w][row][col]);
-            sum.x += v.x * alpha;
-            sum.y += v.y * alpha;
-            sum.z += v.z * alpha;
-            sum.w += v.w * alpha;
-        }
-        if (p.splits > 1) {
-            *reinterpret_cast<float4*>(p.part_o + (item * kRows + row) * D + col) = sum;
-            if (col == 0) p.part_ml[item * kRows + row] = make_float2(m, l);
+        for (int w = 0; w < kWarps; ++w) x.add(s_ml[w][row], *reinterpret_cast<const float4*>(&s_o[w][row][col]));
+        if (p.splits == 1) {
+            write_out<D, kBf16>(p, rq, head, row0 + row, col, x);
+        } else if (p.cluster) {
+            *reinterpret_cast<float4*>(smem + S::kCtaO + (row * D + col) * 4) = x.o;
+            if (col == 0) *reinterpret_cast<float2*>(smem + S::kCtaMl + row * 8) = make_float2(x.m, x.l);
         } else {
-            const float inv = l > 0.0f ? __frcp_rn(l) : 0.0f;  // a row without a key is 0
-            const int at = tile * kRows + row;
-            uint16_t* dst = p.out + (rq.first + at / p.group) * p.out_stride + (head * p.group + at % p.group) * D + col;
-            uint2 w;
-            w.x = out_bits<kBf16>(sum.x * inv) | static_cast<uint32_t>(out_bits<kBf16>(sum.y * inv)) << 16;
-            w.y = out_bits<kBf16>(sum.z * inv) | static_cast<uint32_t>(out_bits<kBf16>(sum.w * inv)) << 16;
-            *reinterpret_cast<uint2*>(dst) = w;
+            const long long item = item_of(p, r, head, tile, split);
+            *reinterpret_cast<float4*>(p.part_o + (item * kRows + row) * D + col) = x.o;
+            if (col == 0) p.part_ml[item * kRows + row] = make_float2(x.m, x.l);
         }
+    }
+    if (p.cluster) {
+        // CTA `split` of the cluster joins every splits-th 4 dims.
+        __syncwarp();
+        cluster_sync();
+        const uint32_t cta_o = smem_u32(smem + S::kCtaO), cta_ml = smem_u32(smem + S::kCtaMl);
+        for (int i = static_cast<int>(threadIdx.x) * p.splits + split; i < n_rows * kQuads; i += kThreads * p.splits) {
+            const int row = i / kQuads, col = (i % kQuads) * 4;
+            float2 ml[kMaxCluster];
+            float4 v[kMaxCluster];
+#pragma unroll
+            for (int s = 0; s < kMaxCluster; ++s) {
+                if (s < p.splits) {
+                    ml[s] = ld_shared_cluster_f2(mapa_shared(cta_ml + row * 8, s));
+                    v[s] = ld_shared_cluster_f4(mapa_shared(cta_o + (row * D + col) * 4, s));
+                }
+            }
+            Merged x;
+#pragma unroll
+            for (int s = 0; s < kMaxCluster; ++s)
+                if (s < p.splits) x.add(ml[s], v[s]);
+            write_out<D, kBf16>(p, rq, head, row0 + row, col, x);
+        }
+        __syncwarp();
+        cluster_sync();  // this CTA's shared memory stays until the others have read it
     }
 }
 
-// Joins the chunks of one (request, key head, row tile), in chunk order. One CTA each;
-// a thread owns 4 dims of a row.
+// Joins the rows' chunks from scratch. 256 threads share out (row, run of consecutive
+// chunks, 4 dims); the runs of a row are joined in order through shared memory. The host
+// chooses `join_runs` runs a row (a power of two, about 4 chunks each), so a CTA holds 256 /
+// (D / 4 * join_runs) rows, and `join_ctas` CTAs the rows of an item.
+constexpr int kJoinThreads = 256;
 template <int D, int NT, bool kBf16>
-__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     constexpr int kRows = 8 * NT;
     constexpr int kQuads = D / 4;
+    __shared__ float4 s_o[kJoinThreads];
+    __shared__ float2 s_ml[kJoinThreads / kQuads];
     int rest = static_cast<int>(blockIdx.x);
+    const int part = rest % p.join_ctas;
+    rest /= p.join_ctas;
     const int tile = rest % p.tiles;
     rest /= p.tiles;
     const int head = rest % p.heads_kv;
     const int r = rest / p.heads_kv;
     const Request rq = request_of(p, r);
     const int n_rows = min(kRows, rq.n * p.group - tile * kRows);
-    if (n_rows <= 0) return;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int runs = p.join_runs;
+    const int slot = static_cast<int>(threadIdx.x) / kQuads, quad = static_cast<int>(threadIdx.x) % kQuads;
+    const int run = slot % runs, row = part * (kJoinThreads / kQuads / runs) + slot / runs;
+    if (part * (kJoinThreads / kQuads / runs) >= n_rows) return;
     const int kv_end = max(rq.len - rq.n + (tile * kRows + n_rows - 1) / p.group + 1, 0);
     const int used = max(min((kv_end + p.chunk - 1) / p.chunk, p.splits), 1);
     const long long item = item_of(p, r, head, tile, 0);
-    for (int i = static_cast<int>(threadIdx.x); i < n_rows * kQuads; i += 256) {
-        const int row = i / kQuads, col = (i % kQuads) * 4;
-        float m = -INFINITY;
-        for (int s = 0; s < used; ++s) m = fmaxf(m, p.part_ml[(item + s) * kRows + row].x);
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float l = 0.0f;
-        for (int s = 0; s < used; ++s) {
-            const float2 ml = p.part_ml[(item + s) * kRows + row];
-            const float4 v = *reinterpret_cast<const float4*>(p.part_o + ((item + s) * kRows + row) * D + col);
-            if (ml.x == -INFINITY) continue;
-            const float alpha = ex2(ml.x - m);
-            l += ml.y * alpha;
-            sum.x += v.x * alpha;
-            sum.y += v.y * alpha;
-            sum.z += v.z * alpha;
-            sum.w += v.w * alpha;
+    const int each = (used + runs - 1) / runs;
+    const int last = row < n_rows ? min((run + 1) * each, used) : 0;
+    const float2* ml_at = p.part_ml + item * kRows + row;
+    const float* o_at = p.part_o + (item * kRows + row) * D + quad * 4;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    Merged x;
+    for (int s = run * each; s < last; s += 4) {
+        float2 ml[4];
+        float4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            ml[u] = make_float2(-INFINITY, 0.0f);
+            if (s + u < last) {
+                ml[u] = ml_at[static_cast<long long>(s + u) * kRows];
+                v[u] = *reinterpret_cast<const float4*>(o_at + static_cast<long long>(s + u) * kRows * D);
+            }
         }
-        const float inv = l > 0.0f ? __frcp_rn(l) : 0.0f;
-        const int at = tile * kRows + row;
-        uint16_t* dst = p.out + (rq.first + at / p.group) * p.out_stride + (head * p.group + at % p.group) * D + col;
-        uint2 w;
-        w.x = out_bits<kBf16>(sum.x * inv) | static_cast<uint32_t>(out_bits<kBf16>(sum.y * inv)) << 16;
-        w.y = out_bits<kBf16>(sum.z * inv) | static_cast<uint32_t>(out_bits<kBf16>(sum.w * inv)) << 16;
-        *reinterpret_cast<uint2*>(dst) = w;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x.add(ml[u], v[u]);
     }
+    if (runs > 1) {
+        s_o[threadIdx.x] = x.o;
+        if (quad == 0) s_ml[slot] = make_float2(x.m, x.l);
+        __syncthreads();
+        if (run == 0)
+            for (int k = 1; k < runs && k * each < used; ++k) x.add(s_ml[slot + k], s_o[threadIdx.x + k * kQuads]);
+    }
+    if (run == 0 && row < n_rows) write_out<D, kBf16>(p, rq, head, tile * kRows + row, quad * 4, x);
 }
 
 template <int D, int NT, bool kBf16, bool kChange>
@@ -557,23 +671,34 @@ cudaError_t launch_one(const Params& p, unsigned items, int device, cudaStream_t
     static std::atomic<bool> configured[host::kMaxDevices];
     auto kernel = paged_kernel<D, NT, kBf16, kChange>;
     if (!configured[device].load(std::memory_order_acquire)) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<D, NT>);
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D, NT>::kBytes);
         if (e != cudaSuccess) return e;
         configured[device].store(true, std::memory_order_release);
     }
-    kernel<<<items * p.splits, kThreads, kSmemBytes<D, NT>, stream>>>(p);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(items * p.splits);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Smem<D, NT>::kBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(p.splits);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.cluster ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 template <int D, int NT, bool kBf16>
 cudaError_t launch(const Params& p, bool change, unsigned items, int device, cudaStream_t stream) {
     cudaError_t err = change ? launch_one<D, NT, kBf16, true>(p, items, device, stream)
                              : launch_one<D, NT, kBf16, false>(p, items, device, stream);
-    if (err != cudaSuccess || p.splits == 1) return err;
+    if (err != cudaSuccess || p.part_o == nullptr) return err;
     // Programmatic dependent launch: the join's launch overlaps the last chunks.
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(items);
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(items * p.join_ctas);
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -651,25 +776,42 @@ inline cudaError_t paged_entry(bool bf16, const void* q, long long q_stride, voi
     p.scale = scale;
     p.softcap = softcap;
     p.slopes = slopes;
-    // Chunks: enough CTAs for several rounds of the GPU, at least 128 tokens each.
-    const long long want = (kCtasPerSm * static_cast<long long>(sm_count) + items - 1) / items;
-    const long long most = (max_seq_len + 127LL) / 128;
-    long long splits = want < most ? want : most;
-    if (splits < 1) splits = 1;
-    long long chunk = (max_seq_len + splits - 1) / splits;
-    chunk = (chunk + 63) / 64 * 64;
-    if (chunk < 64) chunk = 64;
-    splits = (max_seq_len + chunk - 1) / chunk;
-    p.splits = static_cast<int>(splits < 1 ? 1 : splits);
-    p.chunk = static_cast<int>(chunk);
+    const long long round = 64 * (128 / dim);  // a step of each warp
+    auto cut = [&](long long splits) {
+        long long chunk = (max_seq_len + splits - 1) / splits;
+        chunk = (chunk + round - 1) / round * round;
+        if (chunk < round) chunk = round;
+        splits = (max_seq_len + chunk - 1) / chunk;
+        p.splits = static_cast<int>(splits < 1 ? 1 : splits);
+        p.chunk = static_cast<int>(chunk);
+    };
+    if (items * kMaxCluster <= 4LL * sm_count && max_seq_len <= kMaxCluster * (TK_PAGED_CLUSTER_BYTES / (2 * dim))) {
+        // Short and few, all of it resident at once: one launch.
+        cut(kMaxCluster);
+        p.cluster = p.splits > 1;
+    } else {
+        // Enough CTAs for several rounds of the GPU (contexts are ragged, and a cluster would
+        // hold its SMs until its longest chunk ends), each with at least 128 KB of cache, or 64
+        // KB where one request has to fill the GPU.
+        const long long least = (n_requests == 1 ? 65536 : 131072) / (2 * dim);
+        const long long rounds = n_requests < TK_PAGED_ROUNDS ? n_requests : TK_PAGED_ROUNDS;
+        const long long want = rounds * 4LL * sm_count / items;
+        const long long most = (max_seq_len + least - 1) / least;
+        const long long splits = want < most ? want : most;
+        cut(splits < 1 ? 1 : splits);
+    }
     void* scratch = nullptr;
-    if (p.splits > 1) {
+    if (p.splits > 1 && !p.cluster) {
         const size_t n = static_cast<size_t>(items) * p.splits * 8 * nt;
         err = host::scratch_alloc(&scratch, n * (static_cast<size_t>(dim) * 4 + 8), device, stream);
         if (err != cudaSuccess) return err;
         p.part_o = static_cast<float*>(scratch);
         p.part_ml = reinterpret_cast<float2*>(p.part_o + n * dim);
     }
+    p.join_runs = 1;
+    while (p.join_runs * 4 < p.splits && p.join_runs * (dim / 4) < kJoinThreads) p.join_runs *= 2;
+    const int join_rows = kJoinThreads / (dim / 4) / p.join_runs;
+    p.join_ctas = static_cast<int>(((rows < 8 * nt ? rows : 8 * nt) + join_rows - 1) / join_rows);
     const bool change = softcap > 0.0f || slopes != nullptr;
     const unsigned count = static_cast<unsigned>(items);
     const int kind = (dim == 128 ? 4 : 0) + (nt == 2 ? 2 : 0) + (bf16 ? 1 : 0);
