@@ -21,6 +21,10 @@
 //  - the reference point of a row that has not met an allowed key stays -inf;
 //  - P is held as 2^(x - m + 7), so that binary16 keeps its 11 bits down to 2^-21 of
 //    the row's largest weight;
+//  - head_dim up to 64 leaves room in tensor memory for P beside S: S_{j+1} is multiplied
+//    while the softmax of S_j runs (see kApart);
+//  - the whole MMA warp runs the issuing loop and an elected lane issues, so that descriptors
+//    and addresses are warp-uniform: 5-11 % over one lane in a branch of its own;
 //  - with documents, warp 10 zeroes the V rows of padding (negative ids) in shared
 //    memory before the PV product reads them: 0 * NaN would be NaN.
 #pragma once
@@ -39,20 +43,37 @@ using attn::ex2;
 using attn::fma2;
 using attn::kBlockKV;
 using attn::kBlockQ;
-using attn::kKvSlots;
 using attn::kRegsControl;
 using attn::kRegsSoftmax;
 using attn::kThreads;
 using attn::kTmemCols;
 
 constexpr float kLog2e = 1.4426950408889634f;
+#ifndef TK_MASKED_GROUP_BYTES
+#define TK_MASKED_GROUP_BYTES (64LL << 20)
+#endif
 constexpr float kLift = 7.0f;  // P <= 2^(8 + kLift) = 2^15 < 65504
 
+// kApart (head_dim up to 64): tile g has S in columns [256g, 256g + 128), O in [+128, +192)
+// and P in [+192, +256). The softmax releases S as soon as its row is in registers (s_free),
+// so the next S is ready when it has finished with this one, and waits for PV_{j-1} (pv_done)
+// only before it writes P and rescales O. Otherwise P overwrites S, PV_j has to complete
+// before S_{j+1}, and each tile's chain S -> softmax -> PV -> S is serial. MEASURED_APART
 template <int kDPad, bool kBf16>
-struct Cfg : attn::Cfg<kDPad> {
+struct Cfg {
+    static constexpr bool kApart = kDPad == 64;
+    static constexpr int kTileBytes = kBlockQ * kDPad * 2;  // one Q / K / V tile
+    static constexpr int kBoxes = kDPad / 64;                // 64-column TMA boxes per tile
+    static constexpr int kSlots = kApart ? 8 : 4;            // K / V ring
+    static constexpr int kQBuffers = kApart ? 2 : 1;         // the next item's Q loads early
+    static constexpr int kQOffset = 0;                       // Q0, Q1 of each buffer
+    static constexpr int kKvOffset = kQBuffers * 2 * kTileBytes;
+    static constexpr int kBarOffset = kKvOffset + kSlots * kTileBytes;
+    static constexpr int kSmemBytes = kBarOffset + 512 + 1024;
+    static constexpr uint32_t kPOffset = kApart ? 192u : 0u; // P's columns in a tile's 256
     static constexpr uint32_t kFormat = kBf16 ? (1u << 7) | (1u << 10) : 0u;  // A and B alike
-    static constexpr uint32_t kIdescS = attn::Cfg<kDPad>::kIdescS | kFormat;
-    static constexpr uint32_t kIdescO = attn::Cfg<kDPad>::kIdescO | kFormat;
+    static constexpr uint32_t kIdescS = idesc_f16_f32(128, kBlockKV, 0, 0) | kFormat;
+    static constexpr uint32_t kIdescO = idesc_f16_f32(128, kDPad, 0, 1) | kFormat;
 };
 
 struct Params {
@@ -60,6 +81,7 @@ struct Params {
     int pairs;              // ceil(seq_q / 256)
     int heads_q, heads_kv, group;
     int num_items;          // batch * heads_q * pairs
+    int group_bh;           // (batch, head)s per group of items
     int* next_item;         // zeroed counter, or null: item w -> CTA w % grid
     int causal;
     const int* prefix;      // [batch] or null
@@ -79,6 +101,36 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, uint3
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
         " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+
+// tcgen05.mma and commit by one elected lane of a converged warp. With the whole warp in the
+// issuing loop its operands are warp-uniform.
+__device__ __forceinline__ void mma_ss_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void mma_ts_elect(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void commit_elect(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
         : "memory");
 }
 
@@ -214,9 +266,11 @@ __global__ void __launch_bounds__(kRunThreads) runs_kernel(const int* __restrict
 
 // ---- work items ---------------------------------------------------------------------
 
-// One (batch, head) and two 128-row query tiles; within a (batch, head), later pairs
-// first (under a causal mask they see more keys). Tile g works on key blocks
-// [b0[g], b1[g]) (empty if b0 >= b1); the item's loads cover [jb, je).
+// One (batch, head) and two 128-row query tiles. Items are numbered group by group of
+// (batch, head)s, and within a group the last pairs of rows of all its heads first: under a
+// causal mask those see the most keys, so the GPU runs out of work on the lightest items. A
+// group's K and V fit L2. Tile g works on key blocks [b0[g], b1[g]) (empty if b0 >= b1); the
+// item's loads cover [jb, je).
 struct Item {
     int batch, head, head_kv, q0;
     int b0[2], b1[2];
@@ -225,8 +279,11 @@ struct Item {
 
 __device__ __forceinline__ Item make_item(int w, const Params& p) {
     Item it;
-    const int pair = p.pairs - 1 - w % p.pairs;
-    const int bh = w / p.pairs;
+    const int first = w / (p.group_bh * p.pairs) * p.group_bh;  // of the group
+    const int heads = min(p.group_bh, p.num_items / p.pairs - first);
+    const int in_group = w - first * p.pairs;
+    const int pair = p.pairs - 1 - in_group / heads;
+    const int bh = first + in_group % heads;
     it.batch = bh / p.heads_q;
     it.head = bh % p.heads_q;
     it.head_kv = it.head / p.group;
@@ -264,17 +321,37 @@ __device__ __forceinline__ Item make_item(int w, const Params& p) {
 
 // ---- scores ---------------------------------------------------------------------------
 
-// Keys outside [lo, hi) (relative to the block) become -inf.
-__device__ __forceinline__ void mask_row(uint32_t (&r)[128], int lo, int hi) {
+// A block's 128 keys in four chunks of 32, for the rows of a warp: which chunks hold a masked
+// key (`edge`), and which some row sees at all (`live`). [lo, hi) is relative to the block.
+struct Chunks {
+    uint32_t edge, live;
+};
+
+__device__ __forceinline__ Chunks chunks_of(int lo, int hi) {
+    Chunks k{0, 0};
 #pragma unroll
-    for (int i = 0; i < 128; ++i)
-        if (i < lo || i >= hi) r[i] = 0xff800000u;
+    for (int c = 0; c < 4; ++c) {
+        if (__any_sync(0xffffffffu, lo > 32 * c || hi < 32 * c + 32)) k.edge |= 1u << c;
+        if (__any_sync(0xffffffffu, lo < 32 * c + 32 && hi > 32 * c && lo < hi)) k.live |= 1u << c;
+    }
+    return k;
 }
 
-// 2^(s c + a) of the row's 128 scores; writes them, rounded to 16 bits, over the first 64
-// columns of S, and returns their sum.
+// Keys outside [lo, hi) become -inf, in the chunks that hold some.
+__device__ __forceinline__ void mask_row(uint32_t (&r)[128], const Chunks& k, int lo, int hi) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        if (!(k.edge >> c & 1)) continue;
+#pragma unroll
+        for (int i = 32 * c; i < 32 * c + 32; ++i)
+            if (i < lo || i >= hi) r[i] = 0xff800000u;
+    }
+}
+
+// 2^(s c + a) of the row's 128 scores; writes them, rounded to 16 bits, to the 64 columns at
+// p_addr, and returns their sum. Chunks of 32 that no row of the warp sees are 0 at once.
 template <bool kBf16>
-__device__ __forceinline__ float exp_store(uint32_t s_addr, const uint32_t (&r)[128], float c, float a) {
+__device__ __forceinline__ float exp_store(uint32_t p_addr, const uint32_t (&r)[128], float c, float a, uint32_t live) {
     float2 acc[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) acc[t] = make_float2(0.0f, 0.0f);
@@ -282,6 +359,12 @@ __device__ __forceinline__ float exp_store(uint32_t s_addr, const uint32_t (&r)[
 #pragma unroll
     for (int chunk = 0; chunk < 4; ++chunk) {
         uint32_t pk[16];
+        if (!(live >> chunk & 1)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pk[i] = 0;
+            tmem_st_32x32b_x16(p_addr + 16 * chunk, pk);
+            continue;
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int idx = 32 * chunk + 2 * i;
@@ -290,29 +373,145 @@ __device__ __forceinline__ float exp_store(uint32_t s_addr, const uint32_t (&r)[
             acc[i & 3] = attn::add2(acc[i & 3], e);
             pk[i] = pack2<kBf16>(e.x, e.y);
         }
-        tmem_st_32x32b_x16(s_addr + 16 * chunk, pk);
+        tmem_st_32x32b_x16(p_addr + 16 * chunk, pk);
     }
     const float2 t = attn::add2(attn::add2(acc[0], acc[1]), attn::add2(acc[2], acc[3]));
     return t.x + t.y;
 }
 
-// softcap * tanh(s scale / softcap) in log2 units, in place:
-// tanh(x) = 1 - 2 / (1 + e^2x), which is 1 and -1 where the exponential is infinite or 0.
-__device__ __forceinline__ void cap_row(uint32_t (&r)[128], float over, float cap) {
-    const float in = over * 2.0f * kLog2e, out = cap * kLog2e;
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("{\n\t.reg .b64 ra, rb;\n\tmov.b64 ra, {%1, %2};\n\tmov.b64 rb, {%3, %4};\n\t"
+        "mul.rn.f32x2 %0, ra, rb;\n\t}"
+        : "=l"(d)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
+    return r;
+}
+
+// ---- softcap * tanh(s scale / softcap), in log2 units
+//
+// Where a warp's scores are small against the cap, tanh(y) = z Q(z^2) with z a multiple of y and
+// Q a polynomial (a least-squares fit of the relative error on Chebyshev nodes, reweighted
+// towards equal ripple), on the FMA pipe:
+//   kNear: |y| < 3/4,  z = 8/3 y, 5 coefficients, relative error 5.7e-7 (7.3e-7 in FP32)
+//   kMid:  |y| < 8/5,  z = 5/4 y, 9 coefficients, 2.5e-7 (6.5e-7 in FP32)
+// Both limits are |z| < 2, one bit of the exponent, so testing a row is an OR over it. Elsewhere
+// tanh(y) = 1 - 2 / (1 + e^2y), which is 1 and -1 where the exponential is infinite or 0: two MUFU
+// operations a score beside the softmax's own. MEASURED_CAP
+enum CapRange { kNear, kMid, kFar };
+
+template <CapRange kRange>
+struct CapPoly {
+    static constexpr int kTerms = kRange == kNear ? 5 : 9;
+    float2 co[kTerms];
+    __device__ __forceinline__ explicit CapPoly(float out) {
+        constexpr float near[5] = {3.74999791e-1f, -1.75754447e-2f, 9.83255915e-4f, -5.22008486e-5f, 1.89612661e-6f};
+        constexpr float mid[9] = {7.99999774e-1f, -1.70658499e-1f, 4.36336249e-2f, -1.11605870e-2f, 2.70939758e-3f, -5.68044372e-4f, 8.98020517e-5f, -8.98356757e-6f, 4.12556517e-7f};
 #pragma unroll
-    for (int i = 0; i < 128; ++i) {
-        const float e = ex2(__uint_as_float(r[i]) * in);
-        r[i] = __float_as_uint(fmaf(-2.0f * out, rcp_approx(1.0f + e), out));
+        for (int n = 0; n < kTerms; ++n) {
+            const float c = (kRange == kNear ? near[n < 5 ? n : 0] : mid[n]) * out;
+            co[n] = make_float2(c, c);
+        }
+    }
+    __device__ __forceinline__ float2 operator()(float2 z) const {  // Q(z^2)
+        const float2 u = mul2(z, z);
+        float2 q = fma2(co[kTerms - 1], u, co[kTerms - 2]);
+#pragma unroll
+        for (int n = kTerms - 3; n >= 0; --n) q = fma2(q, u, co[n]);
+        return q;
+    }
+};
+
+// r *= k; whether all of the warp's |r| are below 2 then.
+__device__ __forceinline__ bool scale_row(uint32_t (&r)[128], float k) {
+    const float2 k2 = make_float2(k, k);
+    uint32_t any[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 64; ++i) {
+        const float2 z = mul2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), k2);
+        r[2 * i] = __float_as_uint(z.x);
+        r[2 * i + 1] = __float_as_uint(z.y);
+        any[i & 3] |= r[2 * i] | r[2 * i + 1];
+    }
+    return !__any_sync(0xffffffffu, ((any[0] | any[1]) | (any[2] | any[3])) & 0x40000000u);
+}
+
+// Scores to z, and the range the warp's lie in. over = scale / softcap.
+__device__ __forceinline__ CapRange cap_range(uint32_t (&r)[128], float over) {
+    if (scale_row(r, 8.0f / 3.0f * over)) return kNear;
+    return scale_row(r, 15.0f / 32.0f) ? kMid : kFar;
+}
+
+// The capped score of one value in the scale of kMid and kFar (z = 5/4 y); out = softcap * log2(e).
+__device__ __forceinline__ float cap_far(float z, float out) {
+    return fmaf(-2.0f * out, rcp_approx(1.0f + ex2(z * (1.6f * kLog2e))), out);
+}
+
+// z to capped scores, in place.
+template <CapRange kRange>
+__device__ __forceinline__ void cap_row(uint32_t (&r)[128], float out) {
+    if constexpr (kRange == kFar) {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) r[i] = __float_as_uint(cap_far(__uint_as_float(r[i]), out));
+    } else {
+        const CapPoly<kRange> poly(out);
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+            const float2 z = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+            const float2 x = mul2(poly(z), z);
+            r[2 * i] = __float_as_uint(x.x);
+            r[2 * i + 1] = __float_as_uint(x.y);
+        }
     }
 }
 
-// s c - slope |pos - j|, in place; `from` = pos - first key of the block.
-__device__ __forceinline__ void bias_row(uint32_t (&r)[128], float c, float slope, int from) {
+// exp_store of capped scores straight from z: the argument's own multiply-add takes the last
+// product of the polynomial.
+template <bool kBf16, CapRange kRange>
+__device__ __forceinline__ float cap_exp_store(uint32_t p_addr, const uint32_t (&r)[128], float out, float a) {
+    const CapPoly<kRange> poly(out);
+    float2 acc[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[t] = make_float2(0.0f, 0.0f);
+    const float2 a2 = make_float2(a, a);
+#pragma unroll
+    for (int chunk = 0; chunk < 4; ++chunk) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int idx = 32 * chunk + 2 * i;
+            const float2 z = make_float2(__uint_as_float(r[idx]), __uint_as_float(r[idx + 1]));
+            const float2 x = fma2(z, poly(z), a2);
+            const float2 e = make_float2(ex2(x.x), ex2(x.y));
+            acc[i & 3] = attn::add2(acc[i & 3], e);
+            pk[i] = pack2<kBf16>(e.x, e.y);
+        }
+        tmem_st_32x32b_x16(p_addr + 16 * chunk, pk);
+    }
+    const float2 t = attn::add2(attn::add2(acc[0], acc[1]), attn::add2(acc[2], acc[3]));
+    return t.x + t.y;
+}
+
+// Scores r c - slope |pos - j| in log2 units, in place: leaves r with r c + base that score.
+// Where the block lies on one side of the rows of a warp, |pos - j| is linear in j: one
+// multiply-add a score by a constant of its column (slope / c), the row's part goes to base.
+// `from` = pos - first key of the block.
+__device__ __forceinline__ void bias_row(uint32_t (&r)[128], float& c, float& base, float slope, int from, bool left, bool right) {
     const float f = static_cast<float>(from);
+    if ((left || right) && c > 1e-12f) {
+        const float up = left ? slope : -slope;  // per key
+        const float up_c = __fdiv_rn(up, c);
+#pragma unroll
+        for (int i = 0; i < 128; ++i) r[i] = __float_as_uint(fmaf(up_c, static_cast<float>(i), __uint_as_float(r[i])));
+        base = -up * f;
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 128; ++i)
         r[i] = __float_as_uint(fmaf(fabsf(f - static_cast<float>(i)), -slope, __uint_as_float(r[i]) * c));
+    c = 1.0f;
 }
 
 // ---- kernel ---------------------------------------------------------------------------
@@ -327,38 +526,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t base = (raw_base + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (base - raw_base);
     const uint32_t bars = base + C::kBarOffset;
+    constexpr int kSlots = C::kSlots;
     auto kv_full = [&](int s) { return bars + 8u * s; };
-    auto kv_empty = [&](int s) { return bars + 8u * (kKvSlots + s); };
-    constexpr int kB = 2 * kKvSlots;
-    const uint32_t q_full = bars + 8u * kB;
-    const uint32_t q_empty = bars + 8u * (kB + 1);
+    auto kv_empty = [&](int s) { return bars + 8u * (kSlots + s); };
+    auto v_clean = [&](int s) { return bars + 8u * (2 * kSlots + s); };  // documents: V slot s has no padding rows left
+    constexpr int kB = 3 * kSlots;
+    auto q_full = [&](int b) { return bars + 8u * (kB + 16 + b); };
+    auto q_empty = [&](int b) { return bars + 8u * (kB + 18 + b); };
+    constexpr int kQ = C::kQBuffers;
     auto s_full = [&](int g) { return bars + 8u * (kB + 2 + g); };
     auto p_ready = [&](int g) { return bars + 8u * (kB + 4 + g); };
-    auto o_final = [&](int g) { return bars + 8u * (kB + 6 + g); };
+    auto o_final = [&](int g) { return bars + 8u * (kB + 6 + g); };  // kApart: pv_done, after every PV
     auto o_empty = [&](int g) { return bars + 8u * (kB + 8 + g); };
     auto item_full = [&](int s) { return bars + 8u * (kB + 10 + s); };
     auto item_empty = [&](int s) { return bars + 8u * (kB + 12 + s); };
-    auto v_clean = [&](int s) { return bars + 8u * (kB + 14 + s); };  // documents: V slot s has no padding rows left
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBarOffset + 8 * (kB + 14 + kKvSlots));
+    auto s_free = [&](int g) { return bars + 8u * (kB + 14 + g); };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBarOffset + 8 * (kB + 20));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* item_info = reinterpret_cast<volatile int*>(tmem_slot + 2);  // two entries
-    static_assert(8 * (kB + 14 + kKvSlots) + 16 <= 256, "barrier block");
+    static_assert(8 * (kB + 20) + 16 <= 512, "barrier block");
 
     const uint32_t warp = warp_id();
     const uint32_t lane = lane_id();
     const bool documents = p.rows != nullptr;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kKvSlots; ++s) {
+        for (int s = 0; s < kSlots; ++s) {
             mbar_init(kv_full(s), 1);
             mbar_init(kv_empty(s), 1);
             mbar_init(v_clean(s), 1);
         }
-        mbar_init(q_full, 1);
-        mbar_init(q_empty, 1);
         for (int g = 0; g < 2; ++g) {
+            mbar_init(q_full(g), 1);
+            mbar_init(q_empty(g), 1);
             mbar_init(s_full(g), 1);
             mbar_init(p_ready(g), 4);
+            mbar_init(s_free(g), 4);
             mbar_init(o_final(g), 1);
             mbar_init(o_empty(g), 4);
             mbar_init(item_full(g), 1);
@@ -410,17 +613,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ++items;
                     const Item it = make_item(wi, p);
                     if (it.jb >= it.je) continue;
-                    // Q of the previous item is free once all its S MMAs have completed.
-                    if (loaded > 0 &&
-                        !mbar_wait(q_empty, static_cast<uint32_t>(loaded - 1) & 1u, kFaultProducerWait, abort_flag)) {
+                    // A Q buffer is free once all S products of the item that had it have completed.
+                    const int qb = loaded % kQ;
+                    if (loaded >= kQ &&
+                        !mbar_wait(q_empty(qb), static_cast<uint32_t>(loaded / kQ - 1) & 1u, kFaultProducerWait, abort_flag)) {
                         ok = false;
                         break;
                     }
                     const int ntiles = it.q0 + kBlockQ < p.seq_q ? 2 : 1;
-                    mbar_arrive_expect_tx(q_full, ntiles * C::kTileBytes);
+                    mbar_arrive_expect_tx(q_full(qb), ntiles * C::kTileBytes);
                     for (int g = 0; g < ntiles; ++g)
                         for (int x = 0; x < C::kBoxes; ++x)
-                            tma_load_4d(base + C::kQOffset + g * C::kTileBytes + x * 16384, &map_q, q_full, x * 64,
+                            tma_load_4d(base + C::kQOffset + (2 * qb + g) * C::kTileBytes + x * 16384, &map_q, q_full(qb), x * 64,
                                         it.q0 + g * kBlockQ, it.head, it.batch);
                     ++loaded;
                     for (int j = it.jb; j < it.je && ok; ++j) {
@@ -435,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 tma_load_4d(dst + x * 16384, which == 0 ? &map_k : &map_v, kv_full(slot), x * 64,
                                             j * kBlockKV, it.head_kv, it.batch);
                             ++issued;
-                            if (++slot == kKvSlots) {
+                            if (++slot == kSlots) {
                                 slot = 0;
                                 phase ^= 1u;
                             }
@@ -444,14 +648,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!ok) break;
                 }
                 if (!ok) {
-                    // Let every issued load land before the CTA may exit: the last Q load
-                    // and the last (up to kKvSlots) K/V loads.
-                    if (loaded > 0) mbar_wait(q_full, static_cast<uint32_t>(loaded - 1) & 1u, kFaultDrainWait, nullptr);
+                    // Let every issued load land before the CTA may exit: the last Q loads
+                    // and the last (up to kSlots) K/V loads.
+                    for (int i = loaded > kQ ? loaded - kQ : 0; i < loaded; ++i)
+                        mbar_wait(q_full(i % kQ), static_cast<uint32_t>(i / kQ) & 1u, kFaultDrainWait, nullptr);
                     int s = slot;
                     uint32_t ph = phase;
-                    for (int i = 0; i < min(issued, kKvSlots); ++i) {
+                    for (int i = 0; i < min(issued, kSlots); ++i) {
                         if (--s < 0) {
-                            s = kKvSlots - 1;
+                            s = kSlots - 1;
                             ph ^= 1u;
                         }
                         mbar_wait(kv_full(s), ph, kFaultDrainWait, nullptr);
@@ -460,103 +665,142 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
         } else if (warp == 9) {
-            // ---------------- MMA issuer (one thread) ----------------
-            if (lane == 0) {
-                const uint32_t q_addr[2] = {base + C::kQOffset, base + C::kQOffset + C::kTileBytes};
+            // ---------------- MMA issuer (whole warp, an elected lane issues) ----------------
+            {
                 auto kv_addr = [&](int slot) { return base + C::kKvOffset + slot * C::kTileBytes; };
-                const uint64_t dq[2] = {sw128_desc(q_addr[0], 16, 1024), sw128_desc(q_addr[1], 16, 1024)};
+                // A step inside a tile is a plain add to its descriptor's low bits (16-byte units).
+                const uint64_t dq0 = sw128_desc(base + C::kQOffset, 16, 1024);
+                uint64_t dq = dq0;  // of the item's buffer
                 auto issue_s = [&](int g, uint32_t k_addr) {
                     const uint64_t dk = sw128_desc(k_addr, 16, 1024);
 #pragma unroll
                     for (int kk = 0; kk < kDPad / 16; ++kk) {
                         const uint64_t off = static_cast<uint64_t>(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
-                        mma_f16_ss<1>(tmem + 256u * g, dq[g] + off, dk + off, C::kIdescS, kk > 0 ? 1u : 0u);
+                        mma_ss_elect(tmem + 256u * g, dq + static_cast<uint64_t>(g * (C::kTileBytes >> 4)) + off, dk + off, C::kIdescS, kk > 0 ? 1u : 0u);
                     }
-                    mma_commit(s_full(g));
+                    commit_elect(s_full(g));
                 };
                 auto issue_pv = [&](int g, uint32_t v_addr, bool first) {
                     const uint64_t dv = sw128_desc(v_addr, 16384, 1024);
 #pragma unroll
                     for (int kk = 0; kk < kBlockKV / 16; ++kk)
-                        mma_f16_ts(tmem + 256u * g + 128u, tmem + 256u * g + kk * 8,
+                        mma_ts_elect(tmem + 256u * g + 128u, tmem + 256u * g + C::kPOffset + kk * 8,
                                    dv + static_cast<uint64_t>((kk * 2048) >> 4), C::kIdescO, (!first || kk > 0) ? 1u : 0u);
                 };
                 uint32_t pr_phase[2] = {0, 0};
                 int done[2] = {0, 0};  // items in which tile g has produced an output
+                int n_s[2] = {0, 0};   // kApart: S products of tile g
                 int kv_base = 0;       // K/V loads of the previous items
                 int loaded = 0;
                 bool ok = true;
                 auto o_free = [&](int g) {
                     return done[g] == 0 ||
-                           mbar_wait(o_empty(g), static_cast<uint32_t>(done[g] - 1) & 1u, kFaultAttnWait, abort_flag);
+                           mbar_wait_warp(o_empty(g), static_cast<uint32_t>(done[g] - 1) & 1u, kFaultAttnWait, abort_flag);
                 };
                 for (int items = 0, it_slot = 0; ok; it_slot ^= 1, ++items) {
-                    if (!mbar_wait(item_full(it_slot), static_cast<uint32_t>(items >> 1) & 1u, kFaultAttnWait, abort_flag))
+                    if (!mbar_wait_warp(item_full(it_slot), static_cast<uint32_t>(items >> 1) & 1u, kFaultAttnWait, abort_flag))
                         break;
                     const int wi = item_info[it_slot];
-                    mbar_arrive(item_empty(it_slot));
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(item_empty(it_slot));
                     if (wi < 0) break;
                     const Item it = make_item(wi, p);
                     if (it.jb >= it.je) continue;
-                    auto slot_of = [&](int load) { return (kv_base + load) % kKvSlots; };
-                    auto phase_of = [&](int load) { return static_cast<uint32_t>((kv_base + load) / kKvSlots) & 1u; };
+                    auto slot_of = [&](int load) { return (kv_base + load) % kSlots; };
+                    auto phase_of = [&](int load) { return static_cast<uint32_t>((kv_base + load) / kSlots) & 1u; };
                     auto act = [&](int g, int j) { return j >= it.b0[g] && j < it.b1[g]; };
                     auto wait_k = [&](int j) {
-                        return mbar_wait(kv_full(slot_of(2 * (j - it.jb))), phase_of(2 * (j - it.jb)), kFaultAttnWait, abort_flag);
+                        return mbar_wait_warp(kv_full(slot_of(2 * (j - it.jb))), phase_of(2 * (j - it.jb)), kFaultAttnWait, abort_flag);
                     };
                     auto wait_v = [&](int j) {
                         const int load = 2 * (j - it.jb) + 1;
-                        return mbar_wait(documents ? v_clean(slot_of(load)) : kv_full(slot_of(load)), phase_of(load),
+                        return mbar_wait_warp(documents ? v_clean(slot_of(load)) : kv_full(slot_of(load)), phase_of(load),
                                          kFaultAttnWait, abort_flag);
                     };
                     // PV of tile g, block j, once its probabilities are there.
                     auto pv = [&](int g, int j) {
-                        if (!mbar_wait(p_ready(g), pr_phase[g], kFaultAttnWait, abort_flag)) return false;
+                        if (!mbar_wait_warp(p_ready(g), pr_phase[g], kFaultAttnWait, abort_flag)) return false;
                         pr_phase[g] ^= 1u;
                         const bool first = j == it.b0[g];
                         if (first && !o_free(g)) return false;
                         tc_fence_after();
                         issue_pv(g, kv_addr(slot_of(2 * (j - it.jb) + 1)), first);
-                        if (j == it.b1[g] - 1) mma_commit(o_final(g));
+                        if (C::kApart || j == it.b1[g] - 1) commit_elect(o_final(g));
                         return true;
                     };
-                    ok = mbar_wait(q_full, static_cast<uint32_t>(loaded) & 1u, kFaultAttnWait, abort_flag);
+                    const int qb = loaded % kQ;
+                    ok = mbar_wait_warp(q_full(qb), static_cast<uint32_t>(loaded / kQ) & 1u, kFaultAttnWait, abort_flag);
+                    dq = dq0 + static_cast<uint64_t>(qb * (2 * C::kTileBytes >> 4));
                     ++loaded;
-                    if (ok && act(0, it.jb)) {
-                        ok = wait_k(it.jb);
-                        tc_fence_after();
-                        if (ok) issue_s(0, kv_addr(slot_of(0)));
-                    }
-                    for (int j = it.jb; j < it.je && ok; ++j) {
-                        ok = false;
-                        const int load = 2 * (j - it.jb);
-                        // PV1 of the block before, then its V is free.
-                        if (j > it.jb) {
-                            if (act(1, j - 1) && !pv(1, j - 1)) break;
-                            mma_commit(kv_empty(slot_of(load - 1)));
-                        }
-                        // S1, then K is free. K was waited for before S0, where tile 0 works on it.
-                        if (!act(0, j) && !wait_k(j)) break;
-                        if (act(1, j)) {
+                    if constexpr (C::kApart) {
+                        // Per step: S0_{j+1}, PV1_{j-1}, S1_{j+1}, PV0_j, each as soon as what it
+                        // needs is there; the tiles stay half a period apart.
+                        auto s_mma = [&](int g, int j) {
+                            if (n_s[g] > 0 &&
+                                !mbar_wait_warp(s_free(g), static_cast<uint32_t>(n_s[g] - 1) & 1u, kFaultAttnWait, abort_flag))
+                                return false;
+                            ++n_s[g];
                             tc_fence_after();
-                            issue_s(1, kv_addr(slot_of(load)));
+                            issue_s(g, kv_addr(slot_of(2 * (j - it.jb))));
+                            return true;
+                        };
+                        for (int j = it.jb - 1; j <= it.je && ok; ++j) {
+                            ok = false;
+                            const bool more = j + 1 < it.je;
+                            if (more && !wait_k(j + 1)) break;
+                            if (act(0, j + 1) && !s_mma(0, j + 1)) break;
+                            if (j > it.jb) {
+                                if (act(1, j - 1) && !pv(1, j - 1)) break;
+                                commit_elect(kv_empty(slot_of(2 * (j - 1 - it.jb) + 1)));
+                            }
+                            if (act(1, j + 1) && !s_mma(1, j + 1)) break;
+                            if (more) {
+                                commit_elect(kv_empty(slot_of(2 * (j + 1 - it.jb))));
+                                if (j + 1 == it.je - 1) commit_elect(q_empty(qb));
+                            }
+                            if (j >= it.jb && j < it.je) {
+                                if (!wait_v(j)) break;
+                                if (act(0, j) && !pv(0, j)) break;
+                            }
+                            ok = true;
                         }
-                        mma_commit(kv_empty(slot_of(load)));
-                        if (j == it.je - 1) mma_commit(q_empty);
-                        // PV0 and the next block's S0, back to back.
-                        if (!wait_v(j)) break;
-                        const bool next = act(0, j + 1);
-                        if (next && !wait_k(j + 1)) break;
-                        if (act(0, j) && !pv(0, j)) break;
-                        if (next) {
+                    } else {
+                        if (ok && act(0, it.jb)) {
+                            ok = wait_k(it.jb);
                             tc_fence_after();
-                            issue_s(0, kv_addr(slot_of(load + 2)));
+                            if (ok) issue_s(0, kv_addr(slot_of(0)));
                         }
-                        if (j == it.je - 1) {
-                            if (act(1, j) && !pv(1, j)) break;
-                            mma_commit(kv_empty(slot_of(load + 1)));
+                        for (int j = it.jb; j < it.je && ok; ++j) {
+                            ok = false;
+                            const int load = 2 * (j - it.jb);
+                            // PV1 of the block before, then its V is free.
+                            if (j > it.jb) {
+                                if (act(1, j - 1) && !pv(1, j - 1)) break;
+                                commit_elect(kv_empty(slot_of(load - 1)));
+                            }
+                            // S1, then K is free. K was waited for before S0, where tile 0 works on it.
+                            if (!act(0, j) && !wait_k(j)) break;
+                            if (act(1, j)) {
+                                tc_fence_after();
+                                issue_s(1, kv_addr(slot_of(load)));
+                            }
+                            commit_elect(kv_empty(slot_of(load)));
+                            if (j == it.je - 1) commit_elect(q_empty(qb));
+                            // PV0 and the next block's S0, back to back.
+                            if (!wait_v(j)) break;
+                            const bool next = act(0, j + 1);
+                            if (next && !wait_k(j + 1)) break;
+                            if (act(0, j) && !pv(0, j)) break;
+                            if (next) {
+                                tc_fence_after();
+                                issue_s(0, kv_addr(slot_of(load + 2)));
+                            }
+                            if (j == it.je - 1) {
+                                if (act(1, j) && !pv(1, j)) break;
+                                commit_elect(kv_empty(slot_of(load + 1)));
+                            }
+                            ok = true;
                         }
-                        ok = true;
                     }
 #pragma unroll
                     for (int g = 0; g < 2; ++g)
@@ -579,8 +823,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const Item it = make_item(wi, p);
                 for (int j = it.jb; j < it.je; ++j) {
                     const int load = kv_base + 2 * (j - it.jb) + 1;
-                    const int slot = load % kKvSlots;
-                    if (!mbar_wait_warp(kv_full(slot), static_cast<uint32_t>(load / kKvSlots) & 1u, kFaultAttnWait, abort_flag)) {
+                    const int slot = load % kSlots;
+                    if (!mbar_wait_warp(kv_full(slot), static_cast<uint32_t>(load / kSlots) & 1u, kFaultAttnWait, abort_flag)) {
                         ok = false;
                         break;
                     }
@@ -660,24 +904,67 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const bool need_mask = __any_sync(0xffffffffu, lo > kv0 || hi < kv0 + kBlockKV);
                 uint32_t r[128];
                 attn::load_row128(s_addr, r);
-                // Scores in log2 units are r * c; with a change of scores r already is.
-                float c = p.scale_log2;
+                if constexpr (C::kApart) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_free(g));
+                }
+                // Scores in log2 units are r * c + base.
+                float c = p.scale_log2, base = 0.0f;
+                const float cap_out = p.softcap * kLog2e;
+                // Capped scores without a mask or bias go from z to P in one pass: capping keeps
+                // the order, so the row's max is found on z.
+                CapRange range = kFar;
+                bool fused = false;
                 if constexpr (kChange) {
                     if (p.softcap > 0.0f) {
-                        cap_row(r, p.scale / p.softcap, p.softcap);
+                        range = cap_range(r, p.scale / p.softcap);
+                        fused = !need_mask && p.slopes == nullptr && range != kFar;
+                        if (!fused) {
+                            if (range == kNear) cap_row<kNear>(r, cap_out);
+                            else if (range == kMid) cap_row<kMid>(r, cap_out);
+                            else cap_row<kFar>(r, cap_out);
+                        }
                         c = 1.0f;
                     }
-                    // A non-positive scale (the max of r * c is not that of r) is applied here too.
-                    if (p.slopes != nullptr || p.softcap == 0.0f) bias_row(r, c, slope, pos - kv0);
-                    c = 1.0f;
+                    if (p.slopes != nullptr) {
+                        // Keys behind the row's position are masked, unless all of them are seen.
+                        const bool left = (p.causal && p.prefix == nullptr) || __all_sync(0xffffffffu, kv0 + kBlockKV - 1 <= pos);
+                        const bool right = __all_sync(0xffffffffu, kv0 >= pos);
+                        bias_row(r, c, base, slope, pos - kv0, left, right);
+                    } else if (c <= 0.0f) {  // the max of r * c is not that of r
+                        scale_row(r, c);
+                        c = 1.0f;
+                    }
                 }
-                if (need_mask) mask_row(r, lo - kv0, hi - kv0);
-                const float m_blk = attn::row_max128(r) * c;
+                Chunks chunks{0, 15};
+                if (need_mask) {
+                    chunks = chunks_of(lo - kv0, hi - kv0);
+                    mask_row(r, chunks, lo - kv0, hi - kv0);
+                }
+                const float r_max = attn::row_max128(r);
+                const float m_blk = kChange && fused ? cap_far(range == kNear ? 15.0f / 32.0f * r_max : r_max, cap_out) : fmaf(r_max, c, base);
                 // The point moves only when the max grows by more than 8, so P <= 2^(8 + kLift).
                 const float m_new = fmaxf(m_run, m_blk);
                 const float m_use = m_new > m_run + 8.0f ? m_new : m_run;
                 const float alpha = m_use == m_run ? 1.0f : ex2(m_run - m_use);
-                const float e_sum = exp_store<kBf16>(s_addr, r, c, kLift - (m_use == -INFINITY ? 0.0f : m_use));
+                if (C::kApart && j > b0) {
+                    // PV_{j-1} has read P and written O.
+                    if (!mbar_wait_warp(o_final(g), of_phase, kFaultAttnWait, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    of_phase ^= 1u;
+                    tc_fence_after();
+                }
+                const float a = kLift - (m_use == -INFINITY ? 0.0f : m_use);
+                float e_sum;
+                if (kChange && fused) {
+                    e_sum = range == kNear ? cap_exp_store<kBf16, kNear>(s_addr + C::kPOffset, r, cap_out, a)
+                                           : cap_exp_store<kBf16, kMid>(s_addr + C::kPOffset, r, cap_out, a);
+                } else {
+                    e_sum = exp_store<kBf16>(s_addr + C::kPOffset, r, c, base + a, chunks.live);
+                }
                 // tcgen05.ld/st are warp-collective: the rescale runs for the whole warp
                 // when any of its rows needs it.
                 if (j > b0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
@@ -910,6 +1197,15 @@ inline cudaError_t masked_entry(bool bf16, const void* q, const void* k, const v
     p.out_vec = (reinterpret_cast<uintptr_t>(out) & 15u) == 0 && (batch == 1 || vo.b % 8 == 0) && (heads == 1 || vo.h % 8 == 0) &&
                 (seq_q == 1 || vo.s % 8 == 0);
     const int grid = p.num_items < sm_count ? p.num_items : sm_count;
+    // Query heads whose K and V take about a quarter of L2, whole key heads, but at least two
+    // items for each SM.
+    long long at_once = p.group;
+    if (causal != 0 || doc_ids != nullptr) {
+        at_once = (TK_MASKED_GROUP_BYTES / (4LL * seq_kv * dim)) * p.group;
+        const long long fill = (2LL * sm_count + pairs - 1) / pairs;
+        if (at_once < fill) at_once = (fill + p.group - 1) / p.group * p.group;
+    }
+    p.group_bh = static_cast<int>(at_once < bh ? at_once : bh);
 
     // One scratch buffer: the item counter, the documents' tiles and rows, copies of
     // operands whose rows TMA cannot address.
