@@ -85,7 +85,7 @@ struct Params {
     int* next_item;         // zeroed counter, or null: item w -> CTA w % grid
     int causal;
     const int* prefix;      // [batch] or null
-    const int2* rows;       // documents: [batch, seq] (lo, hi) of each row, before the causal cut; or null
+    const int2* rows;       // documents: [batch, seq] (lo, hi) of each row; or null
     const int4* tiles;      // documents: [batch, 2 pairs] (lo, hi, holds padding, 0) of each 128 rows
     float scale;            // of the raw product
     float scale_log2;       // scale * log2(e)
@@ -146,21 +146,22 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 
 // ---- documents --------------------------------------------------------------------
 
-// For every position of a packed row: the run of equal ids that holds it (empty where
-// the id is negative). One CTA per batch row; 8 positions a thread, 8192 a step: a
-// running maximum of run starts going forward, a running minimum of run ends going
-// back. Then the intervals' hull for each 128 rows. Also zeroes the item counter.
+// For every position of a packed row: the run of equal ids that holds it (empty where the id
+// is negative), cut at the position itself under a causal mask; then the intervals' hull
+// for each 128 rows. One CTA per 1024 positions: a running maximum of run starts, and unless
+// causal a running minimum of run ends, inside them; what it needs of the positions outside
+// it looks for 4096 at a time. Also zeroes the item counter. 8192 positions: 16 us in one
+// CTA, MEASURED_RUNS us in eight.
 constexpr int kRunThreads = 1024;
-constexpr int kRunEach = 8;
-constexpr int kRunStep = kRunThreads * kRunEach;
+constexpr int kRunLook = 4;  // positions a thread looks at in a search step
 
 template <bool kMax>
 __device__ __forceinline__ int extreme(int a, int b) { return kMax ? max(a, b) : min(a, b); }
 
-// Exclusive running max (kMax, from thread 0 up) or min (from the last thread down) over
-// the CTA; `all` is the extreme of every thread's value.
+// Inclusive running max (kMax, from thread 0 up) or min (from the last thread down) over the CTA;
+// `all` is the extreme of every thread's value.
 template <bool kMax>
-__device__ __forceinline__ int block_running(int v, int none, int* warp_values, int& all) {
+__device__ __forceinline__ int block_running(int v, int* warp_values, int& all) {
     const int lane = static_cast<int>(lane_id());
     const int warp = static_cast<int>(threadIdx.x >> 5);
     int x = v;
@@ -170,98 +171,99 @@ __device__ __forceinline__ int block_running(int v, int none, int* warp_values, 
         if (kMax ? lane >= o : lane + o < 32) x = extreme<kMax>(x, other);
     }
     if (lane == (kMax ? 31 : 0)) warp_values[warp] = x;
-    int before = kMax ? __shfl_up_sync(0xffffffffu, x, 1) : __shfl_down_sync(0xffffffffu, x, 1);
-    if (lane == (kMax ? 0 : 31)) before = none;
     __syncthreads();
-    int w = warp_values[lane];
-    int y = w;
+    int y = warp_values[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int other = kMax ? __shfl_up_sync(0xffffffffu, y, o) : __shfl_down_sync(0xffffffffu, y, o);
         if (kMax ? lane >= o : lane + o < 32) y = extreme<kMax>(y, other);
     }
     all = __shfl_sync(0xffffffffu, y, kMax ? 31 : 0);
-    int outer = __shfl_sync(0xffffffffu, y, kMax ? max(warp - 1, 0) : min(warp + 1, 31));
-    if (warp == (kMax ? 0 : 31)) outer = none;
+    const int outer = __shfl_sync(0xffffffffu, y, kMax ? max(warp - 1, 0) : min(warp + 1, 31));
     __syncthreads();
-    return extreme<kMax>(before, outer);
+    return warp == (kMax ? 0 : 31) ? x : extreme<kMax>(x, outer);
 }
 
 __global__ void __launch_bounds__(kRunThreads) runs_kernel(const int* __restrict__ ids, int seq, int n_tiles, int causal,
                                                            int2* rows, int4* tiles, int* next_item) {
     __shared__ int warp_values[32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tid = static_cast<int>(threadIdx.x);
-    ids += static_cast<long long>(blockIdx.x) * seq;
-    rows += static_cast<long long>(blockIdx.x) * seq;
-    tiles += static_cast<long long>(blockIdx.x) * n_tiles;
-    if (blockIdx.x == 0 && tid == 0 && next_item != nullptr) *next_item = 0;
-    int carry = 0;
-    for (int base = 0; base < seq; base += kRunStep) {
-        const int s0 = base + tid * kRunEach;
-        int id[kRunEach], before = s0 > 0 && s0 < seq ? ids[s0 - 1] : 0;
-        int last = -1;
+    const int s0 = static_cast<int>(blockIdx.x) * kRunThreads;
+    const int s = s0 + tid;
+    ids += static_cast<long long>(blockIdx.y) * seq;
+    rows += static_cast<long long>(blockIdx.y) * seq;
+    tiles += static_cast<long long>(blockIdx.y) * n_tiles;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0 && next_item != nullptr) *next_item = 0;
+    const bool there = s < seq;
+    const int id = there ? ids[s] : -1;
+    const bool starts = there && (s == 0 || ids[s - 1] != id);
+    const bool ends = there && (s == seq - 1 || ids[s + 1] != id);
+    int all;
+    int start = block_running<true>(starts ? s : -1, warp_values, all);
+    if (s0 < seq && s0 > 0 && __syncthreads_or(tid == 0 && !starts)) {
+        // The first run began before: look back for its start.
+        int found = -1;
+        for (int hi = s0; found < 0; hi -= kRunThreads * kRunLook) {
+            int best = -1;
 #pragma unroll
-        for (int i = 0; i < kRunEach; ++i) {
-            id[i] = s0 + i < seq ? ids[s0 + i] : -1;
-            if (s0 + i < seq && (s0 + i == 0 || id[i] != (i > 0 ? id[i - 1] : before))) last = s0 + i;
-        }
-        int all;
-        int start = max(block_running<true>(last, -1, warp_values, all), carry);
-#pragma unroll
-        for (int i = 0; i < kRunEach; ++i) {
-            if (s0 + i < seq) {
-                if (id[i] != (i > 0 ? id[i - 1] : before)) start = s0 + i;
-                rows[s0 + i].x = id[i] >= 0 ? start : 0;
+            for (int i = 0; i < kRunLook; ++i) {
+                const int k = hi - 1 - (i * kRunThreads + tid);
+                if (k >= 0 && (k == 0 || ids[k - 1] != ids[k])) best = max(best, k);
             }
+            block_running<true>(best, warp_values, found);
         }
-        carry = max(carry, all);
+        start = max(start, found);
     }
-    carry = seq;
-    for (int base = (seq - 1) / kRunStep * kRunStep; base >= 0; base -= kRunStep) {
-        const int s0 = base + tid * kRunEach;
-        int id[kRunEach];
-        const int after = s0 + kRunEach < seq ? ids[s0 + kRunEach] : 0;
-        int first = INT_MAX;  // smallest run end (exclusive) in these positions
+    int end = s + 1;
+    if (causal == 0) {
+        end = block_running<false>(ends ? s + 1 : INT_MAX, warp_values, all);
+        const int next = min(s0 + kRunThreads, seq);
+        if (__syncthreads_or(s == next - 1 && !ends)) {
+            // The last run goes on: look for its end.
+            int found = INT_MAX;
+            for (int lo = next; found == INT_MAX; lo += kRunThreads * kRunLook) {
+                int best = INT_MAX;
 #pragma unroll
-        for (int i = kRunEach - 1; i >= 0; --i) {
-            id[i] = s0 + i < seq ? ids[s0 + i] : -1;
-            if (s0 + i < seq && (s0 + i == seq - 1 || id[i] != (i < kRunEach - 1 ? id[i + 1] : after))) first = s0 + i + 1;
-        }
-        int all;
-        int end = min(block_running<false>(first, INT_MAX, warp_values, all), carry);
-#pragma unroll
-        for (int i = kRunEach - 1; i >= 0; --i) {
-            if (s0 + i < seq) {
-                if (s0 + i == seq - 1 || id[i] != (i < kRunEach - 1 ? id[i + 1] : after)) end = s0 + i + 1;
-                rows[s0 + i].y = id[i] >= 0 ? end : 0;
+                for (int i = 0; i < kRunLook; ++i) {
+                    const int k = lo + i * kRunThreads + tid;
+                    if (k < seq && (k == seq - 1 || ids[k + 1] != ids[k])) best = min(best, k + 1);
+                }
+                block_running<false>(best, warp_values, found);
             }
+            end = min(end, found);
         }
-        carry = min(carry, all);
     }
+    const bool sees = there && id >= 0;
+    if (there) rows[s] = sees ? make_int2(start, end) : make_int2(0, 0);
+    // Hull of each 128 rows: four warps.
+    __shared__ int4 warp_hull[32];
+    int lo = sees ? start : INT_MAX, hi = sees ? end : 0, pad = there && id < 0 ? 1 : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        pad |= __shfl_xor_sync(0xffffffffu, pad, o);
+    }
+    if (lane_id() == 0) warp_hull[tid >> 5] = make_int4(lo, hi, pad, 0);
     __syncthreads();
-    const int lane = static_cast<int>(lane_id());
-    for (int tile = tid >> 5; tile < n_tiles; tile += kRunThreads / 32) {
-        int lo = INT_MAX, hi = 0, pad = 0;
+    const int tile = s0 / kBlockQ + tid;
+    if (tid < kRunThreads / kBlockQ && tile < n_tiles) {
+        int4 h = warp_hull[4 * tid];
 #pragma unroll
-        for (int i = 0; i < kBlockQ / 32; ++i) {
-            const int s = tile * kBlockQ + i * 32 + lane;
-            if (s >= seq) continue;
-            const int2 r = rows[s];
-            if (r.x < r.y) {
-                lo = min(lo, r.x);
-                hi = max(hi, causal ? min(r.y, s + 1) : r.y);
-            } else {
-                pad = 1;
-            }
+        for (int i = 1; i < 4; ++i) {
+            const int4 x = warp_hull[4 * tid + i];
+            h.x = min(h.x, x.x);
+            h.y = max(h.y, x.y);
+            h.z |= x.z;
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            pad |= __shfl_xor_sync(0xffffffffu, pad, o);
-        }
-        if (lane == 0) tiles[tile] = make_int4(lo, hi, pad, 0);
+        tiles[tile] = h;
     }
+}
+
+__global__ void zero_kernel(int* counter) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    *counter = 0;
 }
 
 // ---- work items ---------------------------------------------------------------------
@@ -500,7 +502,7 @@ __device__ __forceinline__ float cap_exp_store(uint32_t p_addr, const uint32_t (
 // `from` = pos - first key of the block.
 __device__ __forceinline__ void bias_row(uint32_t (&r)[128], float& c, float& base, float slope, int from, bool left, bool right) {
     const float f = static_cast<float>(from);
-    if ((left || right) && c > 1e-12f) {
+    if ((left || right) && c > 1e-12f) {  // else also where the scale is not positive: the max of r c is not that of r
         const float up = left ? slope : -slope;  // per key
         const float up_c = __fdiv_rn(up, c);
 #pragma unroll
@@ -516,7 +518,16 @@ __device__ __forceinline__ void bias_row(uint32_t (&r)[128], float& c, float& ba
 
 // ---- kernel ---------------------------------------------------------------------------
 
-template <int kDPad, bool kBf16, bool kChange>
+// What is done to the scores: kernels of their own, since each pass over a row is unrolled to
+// 128 scores and the instruction cache feels it.
+enum Kind {
+    kPlain,        // a positive scale, folded into the exponent
+    kCap,
+    kBias,         // slopes, or a non-positive scale
+    kCapBias,
+};
+
+template <int kDPad, bool kBf16, Kind kKind>
 __global__ void __launch_bounds__(kThreads, 1)
     masked_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const Params p) {
@@ -578,6 +589,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    // The kernel before zeroes the counter and finds the documents (programmatic dependent launch).
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     if (warp >= 8) {
         setmaxnreg_dec<kRegsControl>();
@@ -882,14 +895,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (documents) {
                     const int2 r = __ldg(p.rows + (static_cast<long long>(it.batch) * p.seq_q + q_row));
                     lo = r.x;
-                    hi = p.causal ? min(r.y, pos + 1) : r.y;
+                    hi = r.y;
                 } else if (p.causal) {
                     hi = pos + 1;
                     if (p.prefix != nullptr) hi = min(max(hi, __ldg(p.prefix + it.batch)), p.seq_kv);
                 }
             }
             float slope = 0.0f;
-            if (kChange && p.slopes != nullptr) slope = __ldg(p.slopes + it.head) * kLog2e;
+            if ((kKind == kBias || kKind == kCapBias) && p.slopes != nullptr) slope = __ldg(p.slopes + it.head) * kLog2e;
             float m_run = -INFINITY;  // reference point, log2 units
             float l_run = 0.0f;       // running sum of 2^(x - m_run + kLift)
             const int b0 = it.b0[g], b1 = it.b1[g];
@@ -916,26 +929,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // the order, so the row's max is found on z.
                 CapRange range = kFar;
                 bool fused = false;
-                if constexpr (kChange) {
-                    if (p.softcap > 0.0f) {
-                        range = cap_range(r, p.scale / p.softcap);
-                        fused = !need_mask && p.slopes == nullptr && range != kFar;
-                        if (!fused) {
-                            if (range == kNear) cap_row<kNear>(r, cap_out);
-                            else if (range == kMid) cap_row<kMid>(r, cap_out);
-                            else cap_row<kFar>(r, cap_out);
-                        }
-                        c = 1.0f;
+                if constexpr (kKind == kCap || kKind == kCapBias) {
+                    range = cap_range(r, p.scale / p.softcap);
+                    fused = kKind == kCap && !need_mask && range != kFar;
+                    if (!fused) {
+                        if (range == kNear) cap_row<kNear>(r, cap_out);
+                        else if (range == kMid) cap_row<kMid>(r, cap_out);
+                        else cap_row<kFar>(r, cap_out);
                     }
-                    if (p.slopes != nullptr) {
-                        // Keys behind the row's position are masked, unless all of them are seen.
-                        const bool left = (p.causal && p.prefix == nullptr) || __all_sync(0xffffffffu, kv0 + kBlockKV - 1 <= pos);
-                        const bool right = __all_sync(0xffffffffu, kv0 >= pos);
-                        bias_row(r, c, base, slope, pos - kv0, left, right);
-                    } else if (c <= 0.0f) {  // the max of r * c is not that of r
-                        scale_row(r, c);
-                        c = 1.0f;
-                    }
+                    c = 1.0f;
+                }
+                if constexpr (kKind == kBias || kKind == kCapBias) {
+                    // Keys behind the row's position are masked, unless all of them are seen.
+                    const bool left = (p.causal && p.prefix == nullptr) || __all_sync(0xffffffffu, kv0 + kBlockKV - 1 <= pos);
+                    const bool right = __all_sync(0xffffffffu, kv0 >= pos);
+                    bias_row(r, c, base, slope, pos - kv0, left, right);
                 }
                 Chunks chunks{0, 15};
                 if (need_mask) {
@@ -943,7 +951,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mask_row(r, chunks, lo - kv0, hi - kv0);
                 }
                 const float r_max = attn::row_max128(r);
-                const float m_blk = kChange && fused ? cap_far(range == kNear ? 15.0f / 32.0f * r_max : r_max, cap_out) : fmaf(r_max, c, base);
+                const float m_blk = kKind == kCap && fused ? cap_far(range == kNear ? 15.0f / 32.0f * r_max : r_max, cap_out) : fmaf(r_max, c, base);
                 // The point moves only when the max grows by more than 8, so P <= 2^(8 + kLift).
                 const float m_new = fmaxf(m_run, m_blk);
                 const float m_use = m_new > m_run + 8.0f ? m_new : m_run;
@@ -959,7 +967,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 const float a = kLift - (m_use == -INFINITY ? 0.0f : m_use);
                 float e_sum;
-                if (kChange && fused) {
+                if (kKind == kCap && fused) {
                     e_sum = range == kNear ? cap_exp_store<kBf16, kNear>(s_addr + C::kPOffset, r, cap_out, a)
                                            : cap_exp_store<kBf16, kMid>(s_addr + C::kPOffset, r, cap_out, a);
                 } else {
@@ -1069,19 +1077,40 @@ __global__ void gather_rows_kernel(const uint16_t* src, long long sb, long long 
     }
 }
 
-template <int kDPad, bool kBf16, bool kChange>
-cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int device, int grid,
-                   cudaStream_t stream) {
+template <int kDPad, bool kBf16, Kind kKind>
+cudaError_t launch_kind(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, bool after, int device,
+                        int grid, cudaStream_t stream) {
     using C = Cfg<kDPad, kBf16>;
     static std::atomic<bool> configured[host::kMaxDevices];
-    auto kernel = masked_kernel<kDPad, kBf16, kChange>;
+    auto kernel = masked_kernel<kDPad, kBf16, kKind>;
     if (!configured[device].load(std::memory_order_acquire)) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
         if (e != cudaSuccess) return e;
         configured[device].store(true, std::memory_order_release);
     }
-    kernel<<<static_cast<unsigned>(grid), kThreads, C::kSmemBytes, stream>>>(mq, mk, mv, p);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = after ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, p);
+}
+
+// after: a kernel of this call, launched right before, that this one depends on.
+template <int kDPad, bool kBf16>
+cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, bool after, int device,
+                   int grid, cudaStream_t stream) {
+    const bool bias = p.slopes != nullptr || (p.softcap == 0.0f && !(p.scale > 0.0f));
+    if (p.softcap > 0.0f)
+        return bias ? launch_kind<kDPad, kBf16, kCapBias>(mq, mk, mv, p, after, device, grid, stream)
+                    : launch_kind<kDPad, kBf16, kCap>(mq, mk, mv, p, after, device, grid, stream);
+    return bias ? launch_kind<kDPad, kBf16, kBias>(mq, mk, mv, p, after, device, grid, stream)
+                : launch_kind<kDPad, kBf16, kPlain>(mq, mk, mv, p, after, device, grid, stream);
 }
 
 // Strides of a dimension of size 1 are never used; the others have to be positive.
@@ -1139,7 +1168,7 @@ inline cudaError_t masked_entry(bool bf16, const void* q, const void* k, const v
     if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || batch <= 0 || heads <= 0 || heads_kv <= 0 ||
         heads % heads_kv != 0 || seq_q <= 0 || seq_kv <= 0 || (dim != 16 && dim != 32 && dim != 64 && dim != 128) ||
         (causal != 0 && causal != 1) || !(scale - scale == 0.0f) || !(softcap >= 0.0f) || !(softcap - softcap == 0.0f) ||
-        (doc_ids != nullptr && (prefix != nullptr || seq_q != seq_kv)) || (prefix != nullptr && causal == 0)) {
+        (doc_ids != nullptr && (prefix != nullptr || seq_q != seq_kv || batch > 65535)) || (prefix != nullptr && causal == 0)) {
         return cudaErrorInvalidValue;
     }
     const long long bh = static_cast<long long>(batch) * heads;
@@ -1246,28 +1275,24 @@ inline cudaError_t masked_entry(bool bf16, const void* q, const void* k, const v
     if (doc_ids != nullptr) {
         p.tiles = reinterpret_cast<const int4*>(scratch + tiles_at);
         p.rows = reinterpret_cast<const int2*>(scratch + rows_at);
-        runs_kernel<<<static_cast<unsigned>(batch), kRunThreads, 0, stream>>>(
-            doc_ids, seq_q, 2 * pairs, causal, reinterpret_cast<int2*>(scratch + rows_at),
-            reinterpret_cast<int4*>(scratch + tiles_at), p.next_item);
+        const dim3 blocks(static_cast<unsigned>((256LL * pairs + kRunThreads - 1) / kRunThreads), static_cast<unsigned>(batch));
+        runs_kernel<<<blocks, kRunThreads, 0, stream>>>(doc_ids, seq_q, 2 * pairs, causal,
+                                                        reinterpret_cast<int2*>(scratch + rows_at),
+                                                        reinterpret_cast<int4*>(scratch + tiles_at), p.next_item);
     } else if (counted) {
-        err = cudaMemsetAsync(scratch, 0, sizeof(int), stream);
+        zero_kernel<<<1, 1, 0, stream>>>(p.next_item);
     }
+    const bool after = doc_ids != nullptr || counted;
     CUtensorMap mq, mk, mv;
-    if (err == cudaSuccess && !(make_map(&mq, vq, batch, heads, seq_q, dim) && make_map(&mk, vk, batch, heads_kv, seq_kv, dim) &&
-                                make_map(&mv, vv, batch, heads_kv, seq_kv, dim))) {
+    if (!(make_map(&mq, vq, batch, heads, seq_q, dim) && make_map(&mk, vk, batch, heads_kv, seq_kv, dim) &&
+          make_map(&mv, vv, batch, heads_kv, seq_kv, dim))) {
         err = cudaErrorInvalidValue;
-    }
-    if (err == cudaSuccess) {
-        const bool change = softcap > 0.0f || slopes != nullptr || !(scale > 0.0f);
-        switch ((dim == 128 ? 4 : 0) + (bf16 ? 2 : 0) + (change ? 1 : 0)) {
-            case 0: err = launch<64, false, false>(mq, mk, mv, p, device, grid, stream); break;
-            case 1: err = launch<64, false, true>(mq, mk, mv, p, device, grid, stream); break;
-            case 2: err = launch<64, true, false>(mq, mk, mv, p, device, grid, stream); break;
-            case 3: err = launch<64, true, true>(mq, mk, mv, p, device, grid, stream); break;
-            case 4: err = launch<128, false, false>(mq, mk, mv, p, device, grid, stream); break;
-            case 5: err = launch<128, false, true>(mq, mk, mv, p, device, grid, stream); break;
-            case 6: err = launch<128, true, false>(mq, mk, mv, p, device, grid, stream); break;
-            default: err = launch<128, true, true>(mq, mk, mv, p, device, grid, stream); break;
+    } else {
+        switch ((dim == 128 ? 2 : 0) + (bf16 ? 1 : 0)) {
+            case 0: err = launch<64, false>(mq, mk, mv, p, after, device, grid, stream); break;
+            case 1: err = launch<64, true>(mq, mk, mv, p, after, device, grid, stream); break;
+            case 2: err = launch<128, false>(mq, mk, mv, p, after, device, grid, stream); break;
+            default: err = launch<128, true>(mq, mk, mv, p, after, device, grid, stream); break;
         }
     }
     if (scratch != nullptr) cudaFreeAsync(scratch, stream);
