@@ -134,6 +134,9 @@ __device__ __forceinline__ void commit_elect(uint32_t bar) {
         : "memory");
 }
 
+// A value that all lanes hold alike, in a form the compiler knows to be warp-uniform.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 template <bool kBf16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     if constexpr (kBf16) {
@@ -273,10 +276,12 @@ __global__ void zero_kernel(int* counter) {
 // causal mask those see the most keys, so the GPU runs out of work on the lightest items. A
 // group's K and V fit L2. Tile g works on key blocks [b0[g], b1[g]) (empty if b0 >= b1); the
 // item's loads cover [jb, je).
+// The TMA thread works an item out and leaves it in shared memory for the other warps.
 struct Item {
-    int batch, head, head_kv, q0;
+    int batch, head, q0;
     int b0[2], b1[2];
     int jb, je;
+    int none;  // no item: the end
 };
 
 __device__ __forceinline__ Item make_item(int w, const Params& p) {
@@ -288,7 +293,6 @@ __device__ __forceinline__ Item make_item(int w, const Params& p) {
     const int bh = first + in_group % heads;
     it.batch = bh / p.heads_q;
     it.head = bh % p.heads_q;
-    it.head_kv = it.head / p.group;
     it.q0 = pair * 2 * kBlockQ;
     it.jb = INT_MAX;
     it.je = 0;
@@ -318,6 +322,7 @@ __device__ __forceinline__ Item make_item(int w, const Params& p) {
         }
     }
     if (it.je == 0) it.jb = 0;
+    it.none = 0;
     return it;
 }
 
@@ -351,8 +356,12 @@ __device__ __forceinline__ void mask_row(uint32_t (&r)[128], const Chunks& k, in
 }
 
 // 2^(s c + a) of the row's 128 scores; writes them, rounded to 16 bits, to the 64 columns at
-// p_addr, and returns their sum. Chunks of 32 that no row of the warp sees are 0 at once.
-template <bool kBf16>
+// p_addr, and returns their sum. kSkip: chunks of 32 that no row of the warp sees are 0 at once,
+// for a branch at each chunk. Where blocks are mostly seen whole the branches cost more (unmasked
+// head_dim 64: 363 against 325 us); with documents they pay (138 against 148 us), and so do they
+// for capped scores, whose whole blocks go another way. Both forms in one kernel lose to
+// either alone there (391 against 355 us): each is 64 pairs of code.
+template <bool kBf16, bool kSkip>
 __device__ __forceinline__ float exp_store(uint32_t p_addr, const uint32_t (&r)[128], float c, float a, uint32_t live) {
     float2 acc[4];
 #pragma unroll
@@ -361,7 +370,7 @@ __device__ __forceinline__ float exp_store(uint32_t p_addr, const uint32_t (&r)[
 #pragma unroll
     for (int chunk = 0; chunk < 4; ++chunk) {
         uint32_t pk[16];
-        if (!(live >> chunk & 1)) {
+        if (kSkip && !(live >> chunk & 1)) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) pk[i] = 0;
             tmem_st_32x32b_x16(p_addr + 16 * chunk, pk);
@@ -527,7 +536,7 @@ enum Kind {
     kCapBias,
 };
 
-template <int kDPad, bool kBf16, Kind kKind>
+template <int kDPad, bool kBf16, Kind kKind, bool kDocs>
 __global__ void __launch_bounds__(kThreads, 1)
     masked_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const Params p) {
@@ -554,12 +563,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto s_free = [&](int g) { return bars + 8u * (kB + 14 + g); };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBarOffset + 8 * (kB + 20));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* item_info = reinterpret_cast<volatile int*>(tmem_slot + 2);  // two entries
-    static_assert(8 * (kB + 20) + 16 <= 512, "barrier block");
+    Item* item_ring = reinterpret_cast<Item*>(tmem_slot + 2);  // two entries
+    static_assert(8 * (kB + 20) + 8 + 2 * sizeof(Item) <= 512, "barrier block");
 
     const uint32_t warp = warp_id();
     const uint32_t lane = lane_id();
-    const bool documents = p.rows != nullptr;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kSlots; ++s) {
@@ -576,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(o_final(g), 1);
             mbar_init(o_empty(g), 4);
             mbar_init(item_full(g), 1);
-            mbar_init(item_empty(g), documents ? 10 : 9);  // the MMA thread, eight softmax warps, warp 10
+            mbar_init(item_empty(g), kDocs ? 10 : 9);  // the MMA thread, eight softmax warps, warp 10
         }
         *abort_flag = 0;
         fence_barrier_init();
@@ -588,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(*tmem_slot)));
     // The kernel before zeroes the counter and finds the documents (programmatic dependent launch).
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
@@ -612,7 +620,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         w = p.next_item != nullptr ? static_cast<int>(gridDim.x) + atomicAdd(p.next_item, 1)
                                                    : w + static_cast<int>(gridDim.x);
                     }
-                    const int wi = w < p.num_items ? w : -1;
+                    Item it;
+                    if (w < p.num_items) it = make_item(w, p);
+                    else it.none = 1;
                     // Entry it_slot was last used two items ago.
                     if (items >= 2 &&
                         !mbar_wait(item_empty(it_slot), static_cast<uint32_t>((items - 2) >> 1) & 1u,
@@ -620,11 +630,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         ok = false;
                         break;
                     }
-                    item_info[it_slot] = wi;
+                    item_ring[it_slot] = it;
                     mbar_arrive(item_full(it_slot));
-                    if (wi < 0) break;
+                    if (it.none) break;
                     ++items;
-                    const Item it = make_item(wi, p);
                     if (it.jb >= it.je) continue;
                     // A Q buffer is free once all S products of the item that had it have completed.
                     const int qb = loaded % kQ;
@@ -650,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             mbar_arrive_expect_tx(kv_full(slot), C::kTileBytes);
                             for (int x = 0; x < C::kBoxes; ++x)
                                 tma_load_4d(dst + x * 16384, which == 0 ? &map_k : &map_v, kv_full(slot), x * 64,
-                                            j * kBlockKV, it.head_kv, it.batch);
+                                            j * kBlockKV, it.head / p.group, it.batch);
                             ++issued;
                             if (++slot == kSlots) {
                                 slot = 0;
@@ -713,11 +722,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int items = 0, it_slot = 0; ok; it_slot ^= 1, ++items) {
                     if (!mbar_wait_warp(item_full(it_slot), static_cast<uint32_t>(items >> 1) & 1u, kFaultAttnWait, abort_flag))
                         break;
-                    const int wi = item_info[it_slot];
+                    Item it = item_ring[it_slot];
+                    it.jb = uniform(it.jb);
+                    it.je = uniform(it.je);
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        it.b0[g] = uniform(it.b0[g]);
+                        it.b1[g] = uniform(it.b1[g]);
+                    }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(item_empty(it_slot));
-                    if (wi < 0) break;
-                    const Item it = make_item(wi, p);
+                    if (uniform(it.none)) break;
                     if (it.jb >= it.je) continue;
                     auto slot_of = [&](int load) { return (kv_base + load) % kSlots; };
                     auto phase_of = [&](int load) { return static_cast<uint32_t>((kv_base + load) / kSlots) & 1u; };
@@ -727,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     };
                     auto wait_v = [&](int j) {
                         const int load = 2 * (j - it.jb) + 1;
-                        return mbar_wait_warp(documents ? v_clean(slot_of(load)) : kv_full(slot_of(load)), phase_of(load),
+                        return mbar_wait_warp(kDocs ? v_clean(slot_of(load)) : kv_full(slot_of(load)), phase_of(load),
                                          kFaultAttnWait, abort_flag);
                     };
                     // PV of tile g, block j, once its probabilities are there.
@@ -822,18 +837,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             __syncwarp();
-        } else if (warp == 10 && documents) {
+        } else if (kDocs && warp == 10) {
             // ---------------- padding rows of V become 0 ----------------
             int kv_base = 0;
             bool ok = true;
             for (int items = 0, it_slot = 0; ok; it_slot ^= 1, ++items) {
                 if (!mbar_wait_warp(item_full(it_slot), static_cast<uint32_t>(items >> 1) & 1u, kFaultAttnWait, abort_flag))
                     break;
-                const int wi = item_info[it_slot];
+                const Item it = item_ring[it_slot];
                 __syncwarp();
                 if (lane == 0) mbar_arrive(item_empty(it_slot));
-                if (wi < 0) break;
-                const Item it = make_item(wi, p);
+                if (it.none) break;
                 for (int j = it.jb; j < it.je; ++j) {
                     const int load = kv_base + 2 * (j - it.jb) + 1;
                     const int slot = load % kSlots;
@@ -878,13 +892,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int it_slot = 0, items = 0; ok; it_slot ^= 1, ++items) {
             if (!mbar_wait_warp(item_full(it_slot), static_cast<uint32_t>(items >> 1) & 1u, kFaultAttnWait, abort_flag))
                 break;
-            const int wi = item_info[it_slot];
+            const int none = item_ring[it_slot].none, batch = item_ring[it_slot].batch, head = item_ring[it_slot].head;
+            const int q0 = item_ring[it_slot].q0 + g * kBlockQ;
+            const int b0 = uniform(item_ring[it_slot].b0[g]), b1 = uniform(item_ring[it_slot].b1[g]);
             __syncwarp();
             if (lane == 0) mbar_arrive(item_empty(it_slot));
-            if (wi < 0) break;
-            const Item it = make_item(wi, p);
-            const int q_row = it.q0 + g * kBlockQ + row_in_tile;
-            if (it.q0 + g * kBlockQ >= p.seq_q) continue;
+            if (uniform(none)) break;
+            const int q_row = q0 + row_in_tile;
+            if (uniform(q0) >= p.seq_q) continue;
             const int pos = q_row + p.seq_kv - p.seq_q;
             // The row's keys [lo, hi). Rows past the end take every key, so that they never
             // make their warp compute a mask; they are not stored.
@@ -892,20 +907,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (q_row < p.seq_q) {
                 lo = 0;
                 hi = p.seq_kv;
-                if (documents) {
-                    const int2 r = __ldg(p.rows + (static_cast<long long>(it.batch) * p.seq_q + q_row));
+                if constexpr (kDocs) {
+                    const int2 r = __ldg(p.rows + (static_cast<long long>(batch) * p.seq_q + q_row));
                     lo = r.x;
                     hi = r.y;
                 } else if (p.causal) {
                     hi = pos + 1;
-                    if (p.prefix != nullptr) hi = min(max(hi, __ldg(p.prefix + it.batch)), p.seq_kv);
+                    if (p.prefix != nullptr) hi = min(max(hi, __ldg(p.prefix + batch)), p.seq_kv);
                 }
             }
             float slope = 0.0f;
-            if ((kKind == kBias || kKind == kCapBias) && p.slopes != nullptr) slope = __ldg(p.slopes + it.head) * kLog2e;
+            if ((kKind == kBias || kKind == kCapBias) && p.slopes != nullptr) slope = __ldg(p.slopes + head) * kLog2e;
             float m_run = -INFINITY;  // reference point, log2 units
             float l_run = 0.0f;       // running sum of 2^(x - m_run + kLift)
-            const int b0 = it.b0[g], b1 = it.b1[g];
             for (int j = b0; j < b1; ++j) {
                 if (!mbar_wait_warp(s_full(g), sf_phase, kFaultAttnWait, abort_flag)) {
                     ok = false;
@@ -971,7 +985,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     e_sum = range == kNear ? cap_exp_store<kBf16, kNear>(s_addr + C::kPOffset, r, cap_out, a)
                                            : cap_exp_store<kBf16, kMid>(s_addr + C::kPOffset, r, cap_out, a);
                 } else {
-                    e_sum = exp_store<kBf16>(s_addr + C::kPOffset, r, c, base + a, chunks.live);
+                    constexpr bool kSkip = kDocs || kKind == kCap || kKind == kCapBias;
+                    e_sum = exp_store<kBf16, kSkip>(s_addr + C::kPOffset, r, c, base + a, chunks.live);
                 }
                 // tcgen05.ld/st are warp-collective: the rescale runs for the whole warp
                 // when any of its rows needs it.
@@ -996,7 +1011,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (!ok) break;
             const bool row_ok = q_row < p.seq_q;
-            uint16_t* orow = p.out + it.batch * p.out_b + it.head * p.out_h + static_cast<long long>(q_row) * p.out_s;
+            uint16_t* orow = p.out + batch * p.out_b + head * p.out_h + static_cast<long long>(q_row) * p.out_s;
             if (b0 >= b1) {
                 // No row of the tile sees a key: nothing was multiplied.
                 if (row_ok) {
@@ -1077,12 +1092,12 @@ __global__ void gather_rows_kernel(const uint16_t* src, long long sb, long long 
     }
 }
 
-template <int kDPad, bool kBf16, Kind kKind>
-cudaError_t launch_kind(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, bool after, int device,
+template <int kDPad, bool kBf16, Kind kKind, bool kDocs>
+cudaError_t launch_kernel(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, bool after, int device,
                         int grid, cudaStream_t stream) {
     using C = Cfg<kDPad, kBf16>;
     static std::atomic<bool> configured[host::kMaxDevices];
-    auto kernel = masked_kernel<kDPad, kBf16, kKind>;
+    auto kernel = masked_kernel<kDPad, kBf16, kKind, kDocs>;
     if (!configured[device].load(std::memory_order_acquire)) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
         if (e != cudaSuccess) return e;
@@ -1099,6 +1114,13 @@ cudaError_t launch_kind(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
     cfg.attrs = attr;
     cfg.numAttrs = after ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, p);
+}
+
+template <int kDPad, bool kBf16, Kind kKind>
+cudaError_t launch_kind(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, bool after, int device,
+                        int grid, cudaStream_t stream) {
+    return p.rows != nullptr ? launch_kernel<kDPad, kBf16, kKind, true>(mq, mk, mv, p, after, device, grid, stream)
+                             : launch_kernel<kDPad, kBf16, kKind, false>(mq, mk, mv, p, after, device, grid, stream);
 }
 
 // after: a kernel of this call, launched right before, that this one depends on.
