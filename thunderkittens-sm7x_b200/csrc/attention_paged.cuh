@@ -190,6 +190,7 @@ struct Rows {
     float slope[NT][2];   // log2 units
     int pos[NT][2];       // position, -1 for a row that is not there
     float m[NT][2];       // reference point
+    float off[NT][2];     // kLift - m; 0 while there is no point
     float l[NT][2];       // this lane's part of the sum
 };
 
@@ -366,6 +367,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
             rows.slope[nt][c] = kChange && p.slopes != nullptr && in_tile < n_rows
                                     ? __ldg(p.slopes + head * p.group + row % p.group) * kLog2e : 0.0f;
             rows.m[nt][c] = -INFINITY;
+            rows.off[nt][c] = 0.0f;
             rows.l[nt][c] = 0.0f;
         }
     }
@@ -448,6 +450,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
                     const float now = fmaxf(rows.m[nt][c], mx);
                     const float alpha = now == -INFINITY ? 1.0f : ex2(rows.m[nt][c] - now);
                     rows.m[nt][c] = now;
+                    rows.off[nt][c] = now == -INFINITY ? 0.0f : kLift - now;
                     rows.l[nt][c] *= alpha;
 #pragma unroll
                     for (int i = 0; i < kM; ++i) {
@@ -481,10 +484,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
             for (int nt = 0; nt < NT; ++nt) {
                 float e[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float m = rows.m[nt][c & 1];
-                    e[c] = ex2(s[u][nt][c] + (m == -INFINITY ? 0.0f : kLift - m));
-                }
+                for (int c = 0; c < 4; ++c) e[c] = ex2(s[u][nt][c] + rows.off[nt][c & 1]);
                 rows.l[nt][0] += e[0] + e[2];
                 rows.l[nt][1] += e[1] + e[3];
                 b[nt][0] = transpose_8x8(attn::pack_half2(e[0] * vr, e[1] * vr));
@@ -791,9 +791,11 @@ inline cudaError_t paged_entry(bool bf16, const void* q, long long q_stride, voi
         p.cluster = p.splits > 1;
     } else {
         // Enough CTAs for several rounds of the GPU (contexts are ragged, and a cluster would
-        // hold its SMs until its longest chunk ends), each with at least 128 KB of cache, or 64
-        // KB where one request has to fill the GPU.
-        const long long least = (n_requests == 1 ? 65536 : 131072) / (2 * dim);
+        // hold its SMs until its longest chunk ends), each of at least 1024 tokens, or 64 KB of
+        // cache where one request has to fill the GPU. 512 or 2048 tokens instead of 1024: 16
+        // requests of 17 to 4096 tokens, 16 heads of 64, 32.4 or 33.6 us against 31.5; 32 of up to
+        // 1024, 8 heads of 128, 16.5 or 15.3 against 15.3.
+        const long long least = n_requests == 1 ? 32768 / dim : 1024;
         const long long rounds = n_requests < TK_PAGED_ROUNDS ? n_requests : TK_PAGED_ROUNDS;
         const long long want = rounds * 4LL * sm_count / items;
         const long long most = (max_seq_len + least - 1) / least;

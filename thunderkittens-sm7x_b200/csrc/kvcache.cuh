@@ -397,7 +397,23 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a <= 3.402823466e38f ? a : 0.0f;
 }
 
-// The same for a pair of 16-bit values, as bits (whose order is that of the magnitudes).
+// The larger of each of two 16-bit values; a NaN gives way.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (kBf16) asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// Whether neither of two 16-bit magnitudes is infinite or NaN.
+template <bool kBf16>
+__device__ __forceinline__ bool all_finite(uint32_t pair) {
+    constexpr uint32_t inf = kBf16 ? 0x7f80u : 0x7c00u;
+    return (pair & 0xffffu) < inf && (pair >> 16) < inf;
+}
+
+// |x| of a pair of 16-bit values, 0 for those that are not finite.
 template <bool kBf16>
 __device__ __forceinline__ uint32_t finite_magnitudes(uint32_t pair) {
     const uint32_t a = pair & 0x7fff7fffu;
@@ -419,27 +435,28 @@ __device__ __forceinline__ bool exact_reciprocal(float s) {
 // page. One warp (or, kCta, the four warps of a CTA together) takes one run of one
 // head: the largest |x| of the run sets the scale (never below the page's own, if the
 // page already held tokens before the run's first place), the tokens already there move
-// to it if it grew, and the run is stored. Grid: (token chunks, heads, keys / values). A
-// run belongs to the CTA that holds its first token; it may end behind that CTA's chunk,
+// to it if it grew, and the run is stored. Grid: (token chunks x heads, keys / values),
+// heads fastest: the heads of a token lie side by side, and read at about the same time they
+// share DRAM pages. A run belongs to the CTA that holds its first token; it may end behind that CTA's chunk,
 // so the CTA looks at one slot before its chunk and a page's worth behind it.
 //
 // What bounds it: 2 bytes read and 1 written per element; at a few tokens, the chain
 // slots -> values -> scale -> bytes.
 template <int kDim, bool kBf16, bool kCta>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, kCta ? 8 : 1) append_kernel(const AppendParams p) {
     constexpr int kLanes = kDim / 8;                      // threads that read one token, 16 bytes each
     constexpr int kGroup = kCta ? kAppendThreads : 32;    // threads that work on one run
     constexpr int kRows = kGroup / kLanes;                // tokens per step
     constexpr int kHeld = 8;                              // steps held in registers
     __shared__ long long s_slots[1 + kMostChunk + kMostPage];
     __shared__ float s_max[kAppendWarps];
-    const bool values = blockIdx.z != 0;
-    const int head = static_cast<int>(blockIdx.y);
+    const bool values = blockIdx.y != 0;
+    const int head = static_cast<int>(blockIdx.x) % p.heads;
     const int tid = static_cast<int>(threadIdx.x);
     const int lane = static_cast<int>(lane_id());
     const int warp = tid >> 5;
     const int in_group = kCta ? tid : lane;
-    const int t0 = static_cast<int>(blockIdx.x) * p.chunk;
+    const int t0 = static_cast<int>(blockIdx.x) / p.heads * p.chunk;
     const int count = min(p.chunk, p.n_tokens - t0);
     const uint16_t* x = (values ? p.x[1] : p.x[0]) + head * kDim;
     const long long stride = values ? p.stride[1] : p.stride[0];
@@ -488,18 +505,40 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
             const float old = place > 0 ? scales[tile] : 0.0f;
             const uint16_t* rows = x + static_cast<long long>(t0 + begin) * stride + col;
             uint4 held[kHeld];
-            uint32_t top = 0;  // two 16-bit maxima
-            for (int j0 = 0; j0 < n; j0 += kRows * kHeld) {
+            const long long step = kRows * stride;
+            auto load = [&](int j0) {
+                const uint16_t* at = rows + (j0 + sub) * stride;
+                if (j0 + kRows * kHeld <= n) {
 #pragma unroll
-                for (int u = 0; u < kHeld; ++u) {
-                    const int j = j0 + u * kRows + sub;
-                    held[u] = j < n ? __ldg(reinterpret_cast<const uint4*>(rows + j * stride)) : make_uint4(0, 0, 0, 0);
+                    for (int u = 0; u < kHeld; ++u) held[u] = __ldg(reinterpret_cast<const uint4*>(at + u * step));
+                } else {
+#pragma unroll
+                    for (int u = 0; u < kHeld; ++u)
+                        held[u] = j0 + u * kRows + sub < n ? __ldg(reinterpret_cast<const uint4*>(at + u * step)) : make_uint4(0, 0, 0, 0);
                 }
+            };
+            // Largest magnitudes of the even and the odd elements.
+            uint32_t top = 0;
+            for (int j0 = 0; j0 < n; j0 += kRows * kHeld) {
+                load(j0);
 #pragma unroll
                 for (int u = 0; u < kHeld; ++u) {
-                    const uint32_t w[4] = {held[u].x, held[u].y, held[u].z, held[u].w};
+                    const uint32_t a = max_pair<kBf16>(held[u].x & 0x7fff7fffu, held[u].y & 0x7fff7fffu);
+                    const uint32_t b = max_pair<kBf16>(held[u].z & 0x7fff7fffu, held[u].w & 0x7fff7fffu);
+                    top = max_pair<kBf16>(top, max_pair<kBf16>(a, b));
+                }
+            }
+            if (__any_sync(0xffffffffu, !all_finite<kBf16>(top))) {
+                // Infinities and NaN do not set the scale: once more without them.
+                top = 0;
+                for (int j0 = 0; j0 < n; j0 += kRows * kHeld) {
+                    if (n > kRows * kHeld) load(j0);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) top = __vmaxu2(top, finite_magnitudes<kBf16>(w[c]));
+                    for (int u = 0; u < kHeld; ++u) {
+                        const uint32_t w[4] = {held[u].x, held[u].y, held[u].z, held[u].w};
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) top = max_pair<kBf16>(top, finite_magnitudes<kBf16>(w[c]));
+                    }
                 }
             }
             const float2 tops = pair_to_float2<kBf16>(top);
@@ -528,14 +567,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
             }
             auto store = [&](auto over) {
                 for (int j0 = 0; j0 < n; j0 += kRows * kHeld) {
-                    if (n > kRows * kHeld) {  // else the registers still hold the run
-#pragma unroll
-                        for (int u = 0; u < kHeld; ++u) {
-                            const int j = j0 + u * kRows + sub;
-                            if (j < n) held[u] = __ldg(reinterpret_cast<const uint4*>(rows + j * stride));
-                        }
-                    }
+                    if (n > kRows * kHeld) load(j0);  // else the registers still hold the run
                     uint8_t* at = bytes + (place + j0 + sub) * kDim + col;
+                    const bool full = j0 + kRows * kHeld <= n;
 #pragma unroll
                     for (int u = 0; u < kHeld; ++u) {
                         const uint32_t w[4] = {held[u].x, held[u].y, held[u].z, held[u].w};
@@ -545,7 +579,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
                             const float2 f = pair_to_float2<kBf16>(w[c]);
                             b[c] = to_e4m3x2(over(f.x), over(f.y));
                         }
-                        if (j0 + u * kRows + sub < n)
+                        if (full || j0 + u * kRows + sub < n)
                             *reinterpret_cast<uint2*>(at + u * kRows * kDim) =
                                 make_uint2(__byte_perm(b[0], b[1], 0x5410), __byte_perm(b[2], b[3], 0x5410));
                     }
@@ -612,7 +646,9 @@ inline cudaError_t append_entry(bool bf16, const void* k, const void* v, long lo
     // of up to a page, one at a time by the whole CTA.
     const bool cta = n_tokens > 1024;
     p.chunk = cta ? (n_tokens <= 8192 ? 16 : kMostChunk) : kAppendWarps;
-    const dim3 grid(static_cast<unsigned>((n_tokens + p.chunk - 1) / p.chunk), static_cast<unsigned>(heads), 2);
+    const long long ctas = (n_tokens + p.chunk - 1LL) / p.chunk * heads;
+    if (ctas > INT_MAX) return cudaErrorInvalidValue;
+    const dim3 grid(static_cast<unsigned>(ctas), 2);
     switch ((dim == 128 ? 4 : 0) + (bf16 ? 2 : 0) + (cta ? 1 : 0)) {
         case 0: append_kernel<64, false, false><<<grid, kAppendThreads, 0, stream>>>(p); break;
         case 1: append_kernel<64, false, true><<<grid, kAppendThreads, 0, stream>>>(p); break;

@@ -78,7 +78,7 @@ class TkError(RuntimeError):
 
 
 def build() -> None:
-    """Compile libtk_b200.so for sm_100a (nvcc cross-compiles without a GPU)."""
+    """Compile libtk_b200.so for sm_100a (nvcc cross-compiles without a GPU) and _ops.so."""
     subprocess.run(["make", "-s", "-C", PKG_ROOT], check=True)
 
 
@@ -287,75 +287,39 @@ def attention(q, k, v, *, scale, causal=False, out=None, stream=None):
 
 # ---- attention of language models, and the paged 8-bit cache ---------------------------
 #
-# The smallest calls take a few microseconds on the GPU, less than Python takes to look
-# at a dozen tensors with care. So each helper tests all that it requires in one chain of
-# cheap comparisons, and works out which of them failed only when one did.
+# These helpers go through _ops.so (csrc/torch_ops.cpp), which checks the tensors, allocates
+# what is not given and calls the C ABI on their device and its current stream.
 
-_torch = None
-_raw_stream = None
-_Strides = C.c_int64 * 12
+_ops = None
 
 
-def _import_torch():
-    global _torch, _raw_stream
+def _load_ops():
+    """The built extension module. Raises if it was not built: there is no fallback."""
+    global _ops
+    import importlib.machinery
+    import importlib.util
+
+    import torch  # noqa: F401  (its libraries have to be there first)
+    path = os.path.join(HERE, "_ops.so")
+    if not os.path.exists(path):
+        raise RuntimeError(f"{path} is missing: run `make -C {PKG_ROOT}` (no fallback exists)")
+    lib()
+    loader = importlib.machinery.ExtensionFileLoader("_ops", path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_ops", loader))
+    loader.exec_module(module)
+    module.set_error(TkError)
+    _ops = module
+    return module
+
+
+def _on(stream, t):
+    """Makes a call's stream current, with its device, while the call allocates and launches."""
     import torch
-    # The handle of a device's current stream without a Stream object around it (0.1 us against 4).
-    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
-    _torch = torch
-    return torch
-
-
-def _require(ok, message):
-    if not ok:
-        raise ValueError(message)
-
-
-def _half_type(t, name):
-    _require(t.dtype in (_torch.float16, _torch.bfloat16), f"{name} must be float16 or bfloat16, got {t.dtype}")
-
-
-def _vector(t, name, dtype, shape):
-    """None, or a contiguous tensor of this type and shape."""
-    _require(t is None or (t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous()),
-             f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}" +
-             ("" if t is None else f", got {t.dtype} {tuple(t.shape)}"))
-
-
-def _same_device(device, **tensors):
-    _require(device.type == "cuda", f"tensors must be on a CUDA device, got {device}")
-    for name, t in tensors.items():
-        _require(t is None or t.device == device, f"{name} is on {getattr(t, 'device', None)}, expected {device}")
-
-
-class _Launch:
-    """Makes `device`, and on it the stream of a call, current while the call allocates its
-    outputs and launches, so that the outputs belong to that stream."""
-
-    def __init__(self, device, stream):
-        self.device = _torch.cuda.device(device)
-        if isinstance(stream, int):
-            stream = _torch.cuda.ExternalStream(stream, device=device)
-        _require(stream is None or stream.device == device, f"stream is on {getattr(stream, 'device', None)}, tensors on {device}")
-        self.scope = None if stream is None else _torch.cuda.stream(stream)
-
-    def __enter__(self):
-        self.device.__enter__()
-        if self.scope is not None:
-            self.scope.__enter__()
-
-    def __exit__(self, *exc):
-        if self.scope is not None:
-            self.scope.__exit__(*exc)
-        self.device.__exit__(*exc)
-
-
-def _on(call, device, stream, *args):
-    """call(stream handle, *args) on the device's current stream, or on `stream`."""
-    i = device.index
-    if stream is None and i == _torch.cuda.current_device():
-        return call(_raw_stream(i), *args)
-    with _Launch(device, stream):
-        return call(_raw_stream(i), *args)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=t.device)
+    if stream.device != t.device:
+        raise ValueError(f"stream is on {stream.device}, tensors on {t.device}")
+    return torch.cuda.stream(stream)
 
 
 def attention_masked(q, k, v, *, scale, causal=False, softcap=0.0, alibi_slopes=None, doc_ids=None, prefix_lens=None,
@@ -367,49 +331,11 @@ def attention_masked(q, k, v, *, scale, causal=False, softcap=0.0, alibi_slopes=
     same type, its strides ordered as q's if `out` is not given. alibi_slopes: float32 [Hq];
     doc_ids: int32 [B, Sq] (each run of equal ids a document, negative: padding);
     prefix_lens: int32 [B] (with causal). A row that may see no key is 0."""
-    torch = _torch or _import_torch()
-    kind, device, kshape = q.dtype, q.device, k.shape
-    if not (q.dim() == 4 and k.dim() == 4 and (kind is torch.float16 or kind is torch.bfloat16)
-            and device.type == "cuda" and k.dtype is kind and v.dtype is kind and k.device == device and v.device == device
-            and v.shape == kshape and q.size(0) == kshape[0] and q.size(3) == kshape[3]
-            and (out is None or (out.dtype is kind and out.shape == q.shape and out.device == device))):
-        _masked_complaint(q, k, v, out)
-    b, h, sq, d = q.shape
-    for t, name, dtype, shape in ((alibi_slopes, "alibi_slopes", torch.float32, (h,)), (doc_ids, "doc_ids", torch.int32, (b, sq)),
-                                  (prefix_lens, "prefix_lens", torch.int32, (b,))):
-        if t is not None:
-            _vector(t, name, dtype, shape)
-            _require(t.device == device, f"{name} is on {t.device}, expected {device}")
-
-    def call(handle, out):
-        if out is None:
-            out = torch.empty_like(q)
-        if q.is_contiguous() and k.is_contiguous() and v.is_contiguous() and out.is_contiguous():
-            strides = None
-        else:
-            (qb, qh, qs, q1), (kb, kh, ks, k1) = q.stride(), k.stride()
-            (vb, vh, vs, v1), (ob, oh, os_, o1) = v.stride(), out.stride()
-            _require(d == 1 or (q1 == 1 and k1 == 1 and v1 == 1 and o1 == 1), "the last strides of q, k, v and out must be 1")
-            strides = _Strides(qb, qh, qs, kb, kh, ks, vb, vh, vs, ob, oh, os_)
-        name = "tk_attention_masked_f16" if kind is torch.float16 else "tk_attention_masked_bf16"
-        code = getattr(_lib or lib(), name)(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), strides, b, h, kshape[1], sq, kshape[2], d, scale, softcap,
-            alibi_slopes if alibi_slopes is None else alibi_slopes.data_ptr(), doc_ids if doc_ids is None else doc_ids.data_ptr(),
-            prefix_lens if prefix_lens is None else prefix_lens.data_ptr(), 1 if causal else 0, handle)
-        if code:
-            raise TkError(name, code)
-        return out
-
-    return _on(call, device, stream, out)
-
-
-def _masked_complaint(q, k, v, out):
-    _half_type(q, "q")
-    _require(q.dim() == 4 and k.dim() == 4 and v.shape == k.shape, "q, k, v must be [B, H, S, D], k and v alike")
-    _require(k.shape[0] == q.shape[0] and k.shape[3] == q.shape[3], f"k has shape {tuple(k.shape)}, q {tuple(q.shape)}")
-    _require(k.dtype == q.dtype and v.dtype == q.dtype, "q, k, v must have one type")
-    _same_device(q.device, k=k, v=v, out=out)
-    raise ValueError("out must have q's type and shape")
+    call = (_ops or _load_ops()).attention_masked
+    if stream is None:
+        return call(q, k, v, scale, causal, softcap, alibi_slopes, doc_ids, prefix_lens, out)
+    with _on(stream, q):
+        return call(q, k, v, scale, causal, softcap, alibi_slopes, doc_ids, prefix_lens, out)
 
 
 def kv_plan(cached_lens, new_lens, block_table, free_pages, n_free, *, page_size, max_tokens, lens_out=None, seq_lens=None,
@@ -417,121 +343,24 @@ def kv_plan(cached_lens, new_lens, block_table, free_pages, n_free, *, page_size
     """Places for the new tokens of a step (tk_kv_plan): fills block_table in place and returns
     (lens, seq_lens, starts, slots, n_free). cached_lens, new_lens: int32 [R]; block_table: int32
     [R, max_pages]; free_pages: int32; n_free: int32 [1]. lens_out may be cached_lens and
-    n_free_out n_free, for a state that moves on in place. Outputs that are not given come as
-    parts of one new buffer."""
-    torch = _torch or _import_torch()
-    i32, device = torch.int32, cached_lens.device
-    if not (device.type == "cuda" and cached_lens.dim() == 1 and block_table.dim() == 2 and n_free.numel() == 1
-            and cached_lens.shape == new_lens.shape and block_table.size(0) == cached_lens.size(0)
-            and cached_lens.dtype is i32 and new_lens.dtype is i32 and block_table.dtype is i32 and free_pages.dtype is i32
-            and n_free.dtype is i32 and cached_lens.is_contiguous() and new_lens.is_contiguous() and block_table.is_contiguous()
-            and free_pages.is_contiguous() and new_lens.device == device and block_table.device == device
-            and free_pages.device == device and n_free.device == device):
-        _plan_complaint(cached_lens, new_lens, block_table, free_pages, n_free)
-    r, width = block_table.shape
-    _require(max_tokens >= 0, "max_tokens must not be negative")
-    for t, name, dtype, n in ((lens_out, "lens_out", i32, r), (seq_lens, "seq_lens", i32, r), (starts, "starts", i32, r + 1),
-                              (slots, "slots", torch.int64, max_tokens), (n_free_out, "n_free_out", i32, 1)):
-        if t is not None:
-            _vector(t, name, dtype, (n,))
-            _require(t.device == device, f"{name} is on {t.device}, expected {device}")
-
-    def call(handle, lens_out, seq_lens, starts, slots, n_free_out):
-        if lens_out is None or seq_lens is None or starts is None or slots is None or n_free_out is None:
-            # Slots first: they need 8-byte alignment.
-            parts = torch.empty(2 * max_tokens + 3 * r + 2, dtype=i32, device=device).split((2 * max_tokens, r, r, r + 1, 1))
-            slots = parts[0].view(torch.int64) if slots is None else slots
-            lens_out = parts[1] if lens_out is None else lens_out
-            seq_lens = parts[2] if seq_lens is None else seq_lens
-            starts = parts[3] if starts is None else starts
-            n_free_out = parts[4] if n_free_out is None else n_free_out
-        code = (_lib or lib()).tk_kv_plan(
-            cached_lens.data_ptr(), new_lens.data_ptr(), r, page_size, block_table.data_ptr(), width, free_pages.data_ptr(),
-            free_pages.numel(), n_free.data_ptr(), lens_out.data_ptr(), seq_lens.data_ptr(), starts.data_ptr(), slots.data_ptr(),
-            max_tokens, n_free_out.data_ptr(), handle)
-        if code:
-            raise TkError("tk_kv_plan", code)
-        return lens_out, seq_lens, starts, slots, n_free_out
-
-    return _on(call, device, stream, lens_out, seq_lens, starts, slots, n_free_out)
-
-
-def _plan_complaint(cached_lens, new_lens, block_table, free_pages, n_free):
-    i32 = _torch.int32
-    _require(cached_lens.dim() == 1, "cached_lens must be [R]")
-    r = cached_lens.shape[0]
-    _vector(cached_lens, "cached_lens", i32, (r,))
-    _vector(new_lens, "new_lens", i32, (r,))
-    _require(block_table.dim() == 2, "block_table must be [R, max_pages]")
-    _vector(block_table, "block_table", i32, (r, block_table.shape[1]))
-    _vector(free_pages, "free_pages", i32, free_pages.shape)
-    _vector(n_free, "n_free", i32, (1,))
-    _same_device(cached_lens.device, new_lens=new_lens, block_table=block_table, free_pages=free_pages, n_free=n_free)
-
-
-def _cache_complaint(device, k_cache, v_cache, k_scale, v_scale):
-    _require(k_cache.dim() == 4, "k_cache must be [pages, Hkv, page_size, D]")
-    shape = k_cache.shape
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _require(t.element_size() == 1, f"{name} must hold bytes (uint8 or float8_e4m3fn)")
-        _vector(t, name, t.dtype, shape)
-    _vector(k_scale, "k_scale", _torch.float32, shape[:2])
-    _vector(v_scale, "v_scale", _torch.float32, shape[:2])
-    _same_device(device, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
-
-
-def _cache_ok(torch, device, k_cache, v_cache, k_scale, v_scale):
-    f32, shape = torch.float32, k_cache.shape
-    return (len(shape) == 4 and v_cache.shape == shape and k_cache.element_size() == 1 and v_cache.element_size() == 1
-            and k_scale.dtype is f32 and v_scale.dtype is f32 and k_scale.shape == shape[:2] and v_scale.shape == shape[:2]
-            and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()
-            and k_cache.device == device and v_cache.device == device and k_scale.device == device and v_scale.device == device)
-
-
-def _tokens(t, name, heads, dim):
-    """Elements between the tokens of a packed [T, heads, dim] tensor."""
-    if t.is_contiguous():
-        return heads * dim
-    token, head, one = t.stride()
-    _require(one == 1 and (heads == 1 or head == dim), f"the heads of a token of {name} must be adjacent")
-    return token if t.size(0) > 1 else heads * dim
+    n_free_out n_free, for a state that moves on in place. 32-bit outputs that are not given come
+    as parts of one new buffer."""
+    call = (_ops or _load_ops()).kv_plan
+    args = (cached_lens, new_lens, block_table, free_pages, n_free, page_size, max_tokens, lens_out, seq_lens, starts, slots, n_free_out)
+    if stream is None:
+        return call(*args)
+    with _on(stream, cached_lens):
+        return call(*args)
 
 
 def kv_append(k, v, slots, k_cache, v_cache, k_scale, v_scale, *, stream=None):
     """Quantises packed tokens k, v [T, Hkv, D] (float16 or bfloat16) into the cache at slots
     (int64 [T], -1: skipped), in place (tk_kv_append_e4m3_*)."""
-    torch = _torch or _import_torch()
-    kind, device = k.dtype, k.device
-    if not ((kind is torch.float16 or kind is torch.bfloat16) and v.dtype is kind and k.dim() == 3 and v.shape == k.shape
-            and device.type == "cuda" and v.device == device and slots.device == device and slots.dtype is torch.int64
-            and slots.dim() == 1 and slots.size(0) == k.size(0) and slots.is_contiguous()
-            and _cache_ok(torch, device, k_cache, v_cache, k_scale, v_scale)
-            and k.size(1) == k_cache.size(1) and k.size(2) == k_cache.size(3)):
-        _append_complaint(k, v, slots, k_cache, v_cache, k_scale, v_scale)
-    n, heads, dim = k.shape
-    if n == 0:
-        return
-    k_stride, v_stride = _tokens(k, "k", heads, dim), _tokens(v, "v", heads, dim)
-
-    def call(handle):
-        name = "tk_kv_append_e4m3_f16" if kind is torch.float16 else "tk_kv_append_e4m3_bf16"
-        code = getattr(_lib or lib(), name)(
-            k.data_ptr(), v.data_ptr(), k_stride, v_stride, slots.data_ptr(), n, heads, dim, k_cache.data_ptr(),
-            v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k_cache.size(0), k_cache.size(2), handle)
-        if code:
-            raise TkError(name, code)
-
-    _on(call, device, stream)
-
-
-def _append_complaint(k, v, slots, k_cache, v_cache, k_scale, v_scale):
-    _half_type(k, "k")
-    _cache_complaint(k.device, k_cache, v_cache, k_scale, v_scale)
-    _require(k.dim() == 3 and tuple(k.shape[1:]) == (k_cache.shape[1], k_cache.shape[3]),
-             f"k must be [T, {k_cache.shape[1]}, {k_cache.shape[3]}], got {tuple(k.shape)}")
-    _require(v.dtype == k.dtype and v.shape == k.shape, "k and v must have one type and shape")
-    _vector(slots, "slots", _torch.int64, (k.shape[0],))
-    _same_device(k.device, v=v, slots=slots)
+    call = (_ops or _load_ops()).kv_append
+    if stream is None:
+        return call(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+    with _on(stream, k):
+        return call(k, v, slots, k_cache, v_cache, k_scale, v_scale)
 
 
 def attention_paged(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, starts, *, scale, softcap=0.0,
@@ -540,52 +369,10 @@ def attention_paged(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens
     (tk_attention_paged_e4m3_*); returns [T, Hq, D] of q's type. max_query_len: at least the most
     query tokens of a request; max_seq_len: about the longest context (default: what the block
     table can hold). Rows behind the last request are left as they were in `out`."""
-    torch = _torch or _import_torch()
-    kind, device, i32 = q.dtype, q.device, torch.int32
-    if not ((kind is torch.float16 or kind is torch.bfloat16) and q.dim() == 3 and device.type == "cuda"
-            and _cache_ok(torch, device, k_cache, v_cache, k_scale, v_scale) and q.size(2) == k_cache.size(3)
-            and block_table.dim() == 2 and block_table.dtype is i32 and seq_lens.dtype is i32 and starts.dtype is i32
-            and seq_lens.dim() == 1 and starts.dim() == 1 and seq_lens.size(0) == block_table.size(0)
-            and starts.size(0) == block_table.size(0) + 1 and block_table.is_contiguous() and seq_lens.is_contiguous()
-            and starts.is_contiguous() and block_table.device == device and seq_lens.device == device and starts.device == device
-            and (out is None or (out.dtype is kind and out.shape == q.shape and out.device == device))):
-        _paged_complaint(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, starts, out)
-    n, h, dim = q.shape
-    r, width = block_table.shape
-    pages, hkv, page, _ = k_cache.shape
-    if alibi_slopes is not None:
-        _vector(alibi_slopes, "alibi_slopes", torch.float32, (h,))
-        _require(alibi_slopes.device == device, f"alibi_slopes is on {alibi_slopes.device}, expected {device}")
-    q_stride = _tokens(q, "q", h, dim)
-
-    def call(handle, out):
-        if out is None:
-            out, out_stride = torch.empty((n, h, dim), dtype=kind, device=device), h * dim
-        else:
-            out_stride = _tokens(out, "out", h, dim)
-        if n == 0 or r == 0:
-            return out
-        name = "tk_attention_paged_e4m3_f16" if kind is torch.float16 else "tk_attention_paged_e4m3_bf16"
-        code = getattr(_lib or lib(), name)(
-            q.data_ptr(), q_stride, out.data_ptr(), out_stride, n, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-            v_scale.data_ptr(), pages, page, block_table.data_ptr(), width, seq_lens.data_ptr(), starts.data_ptr(), r, h, hkv, dim,
-            max_query_len, width * page if max_seq_len is None else max_seq_len, scale, softcap,
-            alibi_slopes if alibi_slopes is None else alibi_slopes.data_ptr(), handle)
-        if code:
-            raise TkError(name, code)
-        return out
-
-    return _on(call, device, stream, out)
-
-
-def _paged_complaint(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, starts, out):
-    _half_type(q, "q")
-    _cache_complaint(q.device, k_cache, v_cache, k_scale, v_scale)
-    _require(q.dim() == 3 and q.shape[2] == k_cache.shape[3], f"q must be [T, Hq, {k_cache.shape[3]}], got {tuple(q.shape)}")
-    _require(block_table.dim() == 2, "block_table must be [R, max_pages]")
-    r = block_table.shape[0]
-    _vector(block_table, "block_table", _torch.int32, block_table.shape)
-    _vector(seq_lens, "seq_lens", _torch.int32, (r,))
-    _vector(starts, "starts", _torch.int32, (r + 1,))
-    _same_device(q.device, block_table=block_table, seq_lens=seq_lens, starts=starts, out=out)
-    raise ValueError("out must have q's type and shape")
+    call = (_ops or _load_ops()).attention_paged
+    args = (q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, starts, scale, softcap, alibi_slopes, max_query_len,
+            max_seq_len, out)
+    if stream is None:
+        return call(*args)
+    with _on(stream, q):
+        return call(*args)
