@@ -243,8 +243,8 @@ TK_API cudaError_t tk_attention_forward_gqa_f16(const void* q, const void* k, co
  *     nothing, and whose K and V may hold anything (NaN included).
  * Elements are binary16 (_f16) or bfloat16 (_bf16), out alike. Probabilities are
  * rounded to that type before the PV product, everything between is FP32.
- * head_dim in {16, 32, 64, 128}; seq_q, seq_kv >= 1; any finite scale; softcap >= 0
- * (0: none).
+ * head_dim in {16, 32, 64, 128}; seq_q, seq_kv >= 1; |scale| <= 1e30; softcap 0 (none)
+ * or 1e-6 to 1e30; with doc_ids, batch at most 65535.
  * strides (host): 12 values in elements, (batch, head, row) of Q, K, V and out in
  * turn, or NULL for contiguous tensors; the elements of a row are adjacent. Strides of
  * dimensions larger than 1 must be positive, and out's rows must not share elements.
@@ -274,7 +274,7 @@ TK_API cudaError_t tk_attention_masked_bf16(const void* q, const void* k, const 
 
 /* Places for the new tokens of a step, from request lengths, on the GPU. Request r
  * holds cached_lens[r] tokens and adds new_lens[r] (negative values count as 0).
- *   - It is taken if new_lens[r] > 0, its row has room (max_pages), its tokens end
+ *   - It is taken if new_lens[r] > 0, its row has room (max_pages, and 2^31 - 1 tokens), its tokens end
  *     at or before max_tokens, and it needs no new page or the pages needed up to and
  *     including it (in request order, requests that fail the other conditions not
  *     counted) are at most *n_free.
@@ -332,8 +332,9 @@ TK_API cudaError_t tk_kv_append_e4m3_bf16(const void* k, const void* v, int64_t 
  * are left as they were). max_seq_len only sets how the work is split and should be near
  * the largest seq_lens; results are right for any. head_dim 64 or 128; page_size 16, 32,
  * 64 or 128; q and out 16-byte aligned with strides that are multiples of 8, caches
- * 32-byte aligned; n_requests * heads_kv * ceil(max_query_len * heads_q / heads_kv / 16)
- * at most 2^24. Long contexts take scratch for their chunks' partial sums. */
+ * 32-byte aligned; max_pages * page_size at most 2^30; scale and softcap as for
+ * tk_attention_masked; n_requests * heads_kv * ceil(max_query_len * heads_q / heads_kv
+ * / 16) at most 2^24. Long contexts take scratch for their chunks' partial sums. */
 TK_API cudaError_t tk_attention_paged_e4m3_f16(
     const void* q, int64_t q_stride, void* out, int64_t out_stride, int n_tokens, const void* k_cache,
     const void* v_cache, const float* k_scale, const float* v_scale, int n_pages, int page_size,

@@ -30,9 +30,9 @@ GOOD = [16384, 4096, 64, 8192, 4096, 64, 8192, 4096, 64, 16384, 4096, 64]
 
 @pytest.mark.parametrize("over", [
     dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(batch=0), dict(heads=0), dict(heads_kv=0), dict(heads=5), dict(sq=0),
-    dict(skv=0), dict(d=48), dict(d=256), dict(scale=math.nan), dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.nan), dict(cap=math.inf),
-    dict(causal=2), dict(ids=5 * MB, prefix=6 * MB), dict(ids=5 * MB, skv=65), dict(prefix=5 * MB, causal=0), dict(out=MB), dict(out=2 * MB + 64),
-    dict(ids=4 * MB + 4), dict(prefix=4 * MB), dict(slopes=4 * MB), dict(batch=2 ** 31 - 1, heads=4), dict(sq=2 ** 31 - 1, skv=2 ** 31 - 1),
+    dict(skv=0), dict(d=48), dict(d=256), dict(scale=math.nan), dict(scale=math.inf), dict(scale=-3e38), dict(cap=-1.0), dict(cap=math.nan), dict(cap=math.inf), dict(cap=1e-9),
+    dict(cap=3e38), dict(causal=2), dict(ids=5 * MB, prefix=6 * MB), dict(ids=5 * MB, skv=65), dict(prefix=5 * MB, causal=0), dict(out=MB), dict(out=2 * MB + 64),
+    dict(ids=4 * MB + 4), dict(ids=5 * MB, batch=65536, heads=2), dict(prefix=4 * MB), dict(slopes=4 * MB), dict(batch=2 ** 31 - 1, heads=4), dict(sq=2 ** 31 - 1, skv=2 ** 31 - 1),
     dict(strides=GOOD[:2] + [0] + GOOD[3:]), dict(strides=GOOD[:4] + [-64] + GOOD[5:]), dict(strides=GOOD[:11] + [32]),
     dict(strides=GOOD[:10] + [64, 64]), dict(strides=GOOD[:9] + [4096, 4096, 64], batch=2), dict(strides=[2 ** 62] + GOOD[1:], batch=3),
 ], ids=lambda d: ",".join(f"{k}" for k in d))
@@ -91,7 +91,8 @@ def paged(**over):
 @pytest.mark.parametrize("over", [
     dict(q=None), dict(out=None), dict(kc=None), dict(vc=None), dict(ksc=None), dict(vsc=None), dict(table=None), dict(lens=None),
     dict(starts=None), dict(n=-1), dict(pages=0), dict(width=0), dict(r=-1), dict(heads=0), dict(heads_kv=0), dict(heads=5), dict(dim=32),
-    dict(page=8), dict(page=256), dict(mq=-1), dict(ms=-1), dict(scale=math.nan), dict(scale=-math.inf), dict(cap=-0.5), dict(cap=math.inf),
+    dict(page=8), dict(page=256), dict(mq=-1), dict(ms=-1), dict(scale=math.nan), dict(scale=-math.inf), dict(cap=-0.5), dict(cap=math.inf), dict(cap=1e-30),
+    dict(width=2 ** 26),
     dict(qs=504), dict(os=516), dict(q=MB + 2), dict(out=2 * MB + 8), dict(kc=3 * MB + 16), dict(out=MB), dict(out=3 * MB), dict(out=4 * MB),
     dict(out=5 * MB), dict(out=7 * MB), dict(out=8 * MB), dict(out=9 * MB), dict(slopes=2 * MB), dict(mq=2 ** 31 - 1),
 ], ids=lambda d: ",".join(f"{k}={v}" for k, v in d.items()))

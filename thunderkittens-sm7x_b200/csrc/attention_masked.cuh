@@ -1189,7 +1189,7 @@ inline cudaError_t masked_entry(bool bf16, const void* q, const void* k, const v
                                 const float* slopes, const int* doc_ids, const int* prefix, int causal, cudaStream_t stream) {
     if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || batch <= 0 || heads <= 0 || heads_kv <= 0 ||
         heads % heads_kv != 0 || seq_q <= 0 || seq_kv <= 0 || (dim != 16 && dim != 32 && dim != 64 && dim != 128) ||
-        (causal != 0 && causal != 1) || !(scale - scale == 0.0f) || !(softcap >= 0.0f) || !(softcap - softcap == 0.0f) ||
+        (causal != 0 && causal != 1) || !host::scores_ok(scale, softcap) ||
         (doc_ids != nullptr && (prefix != nullptr || seq_q != seq_kv || batch > 65535)) || (prefix != nullptr && causal == 0)) {
         return cudaErrorInvalidValue;
     }

@@ -57,6 +57,7 @@ template <int D>
 constexpr int kStageBytes = kStep<D> * 2 * D;
 constexpr int kStages = 3;
 constexpr int kMaxCluster = 8;
+constexpr long long kMostTokens = 1LL << 30;  // of a context: positions and steps stay far below 2^31
 #ifndef TK_PAGED_ROUNDS
 #define TK_PAGED_ROUNDS 6
 #endif
@@ -103,8 +104,7 @@ struct Request {
 __device__ __forceinline__ Request request_of(const Params& p, int r) {
     Request q;
     const int a = max(p.starts[r], 0), b = min(p.starts[r + 1], p.n_tokens);
-    const long long most = static_cast<long long>(p.width) * p.page;
-    q.len = static_cast<int>(min(static_cast<long long>(max(p.seq_lens[r], 0)), most));
+    q.len = min(max(p.seq_lens[r], 0), p.width * p.page);
     q.first = a;
     q.n = max(b - a, 0);
     return q;
@@ -717,7 +717,7 @@ inline cudaError_t paged_entry(bool bf16, const void* q, long long q_stride, voi
         table == nullptr || seq_lens == nullptr || starts == nullptr || n_tokens < 0 || n_pages <= 0 || width <= 0 ||
         n_requests < 0 || heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv != 0 || (dim != 64 && dim != 128) ||
         (page != 16 && page != 32 && page != 64 && page != 128) || max_query_len < 0 || max_seq_len < 0 ||
-        !(scale - scale == 0.0f) || !(softcap >= 0.0f) || !(softcap - softcap == 0.0f)) {
+        !host::scores_ok(scale, softcap) || static_cast<long long>(width) * page > kMostTokens) {
         return cudaErrorInvalidValue;
     }
     const long long row = static_cast<long long>(heads_q) * dim;
@@ -739,6 +739,7 @@ inline cudaError_t paged_entry(bool bf16, const void* q, long long q_stride, voi
         host::ranges_overlap(out, out_bytes, starts, (static_cast<size_t>(n_requests) + 1) * 4) ||
         (slopes != nullptr && host::ranges_overlap(out, out_bytes, slopes, static_cast<size_t>(heads_q) * 4)))
         return cudaErrorInvalidValue;
+    if (max_seq_len > width * page) max_seq_len = width * page;  // no context is longer
     const int group = heads_q / heads_kv;
     const long long rows = static_cast<long long>(max_query_len) * group;
     const int nt = rows > 8 ? 2 : 1;

@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
         const long long end = tokens + block_scan(n, part.warp_sums, sum);
         const long long whole = static_cast<long long>(c) + n;
         const int have = static_cast<int>((static_cast<long long>(c) + p.page - 1) / p.page);
-        const bool fits = n > 0 && whole <= static_cast<long long>(p.width) * p.page && end <= p.max_tokens;
+        const bool fits = n > 0 && whole <= min(static_cast<long long>(p.width) * p.page, static_cast<long long>(INT_MAX)) && end <= p.max_tokens;
         const int need = fits ? static_cast<int>((whole + p.page - 1) / p.page) - have : 0;
         const long long upto = pages + block_scan(need, part.warp_sums, page_sum);
         const bool taken = fits && (need == 0 || upto <= n_free);

@@ -152,6 +152,14 @@ inline cudaError_t scratch_pool_bytes(int device, uint64_t* reserved, uint64_t* 
     return cudaMemPoolGetAttribute(sp.pools[device], cudaMemPoolAttrUsedMemCurrent, used);
 }
 
+// Softmax scale and score cap of the attention entry points with score changes: a finite
+// scale (in log2 units too), and a cap that is 0 (none) or leaves the factors scale / cap
+// and cap * log2(e) finite and normal.
+inline bool scores_ok(float scale, float softcap) {
+    const bool scale_ok = scale >= -1e30f && scale <= 1e30f;
+    return scale_ok && (softcap == 0.0f || (softcap >= 1e-6f && softcap <= 1e30f));
+}
+
 inline bool ranges_overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
     const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
     return a0 < b0 + b_bytes && b0 < a0 + a_bytes;

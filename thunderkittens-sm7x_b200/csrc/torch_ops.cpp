@@ -152,6 +152,7 @@ PyObject* attention_masked(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int hkv = fits_int(k.size(1), "k"), skv = fits_int(k.size(2), "k");
         const float scale = static_cast<float>(number(a[3], "scale"));
         const int causal = PyObject_IsTrue(a[4]);
+        if (causal < 0) return nullptr;
         const float cap = static_cast<float>(number(a[5], "softcap"));
         const auto slopes = maybe(a[6], "alibi_slopes"), ids = maybe(a[7], "doc_ids"), prefix = maybe(a[8], "prefix_lens");
         auto out = maybe(a[9], "out");
