@@ -78,15 +78,17 @@ struct Cfg {
 
 struct Params {
     int seq_q, seq_kv, head_dim;
-    int pairs;              // ceil(seq_q / 256)
+    int item_tiles;         // query tiles of an item: 2, or 1 where that fills the GPU better
+    int per_head;           // items of a (batch, head): ceil(seq_q / (128 item_tiles))
+    int tile_stride;        // 128-row tiles of a batch row in `tiles`
     int heads_q, heads_kv, group;
-    int num_items;          // batch * heads_q * pairs
+    int num_items;          // batch * heads_q * per_head
     int group_bh;           // (batch, head)s per group of items
     int* next_item;         // zeroed counter, or null: item w -> CTA w % grid
     int causal;
     const int* prefix;      // [batch] or null
     const int2* rows;       // documents: [batch, seq] (lo, hi) of each row; or null
-    const int4* tiles;      // documents: [batch, 2 pairs] (lo, hi, holds padding, 0) of each 128 rows
+    const int4* tiles;      // documents: [batch, tile_stride] (lo, hi, holds padding, 0) of each 128 rows
     float scale;            // of the raw product
     float scale_log2;       // scale * log2(e)
     float softcap;          // 0: none
@@ -271,14 +273,15 @@ __global__ void zero_kernel(int* counter) {
 
 // ---- work items ---------------------------------------------------------------------
 
-// One (batch, head) and two 128-row query tiles. Items are numbered group by group of
-// (batch, head)s, and within a group the last pairs of rows of all its heads first: under a
+// One (batch, head) and one or two 128-row query tiles. Items are numbered group by group of
+// (batch, head)s, and within a group the last rows of all its heads first: under a
 // causal mask those see the most keys, so the GPU runs out of work on the lightest items. A
 // group's K and V fit L2. Tile g works on key blocks [b0[g], b1[g]) (empty if b0 >= b1); the
 // item's loads cover [jb, je).
 // The TMA thread works an item out and leaves it in shared memory for the other warps.
 struct Item {
     int batch, head, q0;
+    int tiles;  // of 128 query rows: 1 or 2
     int b0[2], b1[2];
     int jb, je;
     int none;  // no item: the end
@@ -286,23 +289,24 @@ struct Item {
 
 __device__ __forceinline__ Item make_item(int w, const Params& p) {
     Item it;
-    const int first = w / (p.group_bh * p.pairs) * p.group_bh;  // of the group
-    const int heads = min(p.group_bh, p.num_items / p.pairs - first);
-    const int in_group = w - first * p.pairs;
-    const int pair = p.pairs - 1 - in_group / heads;
+    const int first = w / (p.group_bh * p.per_head) * p.group_bh;  // of the group
+    const int heads = min(p.group_bh, p.num_items / p.per_head - first);
+    const int in_group = w - first * p.per_head;
+    const int part = p.per_head - 1 - in_group / heads;
     const int bh = first + in_group % heads;
     it.batch = bh / p.heads_q;
     it.head = bh % p.heads_q;
-    it.q0 = pair * 2 * kBlockQ;
+    it.q0 = part * p.item_tiles * kBlockQ;
+    it.tiles = it.q0 + kBlockQ < p.seq_q ? p.item_tiles : 1;
     it.jb = INT_MAX;
     it.je = 0;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
         const int r0 = it.q0 + g * kBlockQ;
         int lo = 0, hi = 0;
-        if (r0 < p.seq_q) {
+        if (g < it.tiles) {
             if (p.tiles != nullptr) {
-                const int4 t = __ldg(p.tiles + (static_cast<long long>(it.batch) * 2 * p.pairs + 2 * pair + g));
+                const int4 t = __ldg(p.tiles + (static_cast<long long>(it.batch) * p.tile_stride + part * p.item_tiles + g));
                 lo = t.x;
                 hi = t.y;
             } else {
@@ -642,9 +646,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         ok = false;
                         break;
                     }
-                    const int ntiles = it.q0 + kBlockQ < p.seq_q ? 2 : 1;
-                    mbar_arrive_expect_tx(q_full(qb), ntiles * C::kTileBytes);
-                    for (int g = 0; g < ntiles; ++g)
+                    mbar_arrive_expect_tx(q_full(qb), it.tiles * C::kTileBytes);
+                    for (int g = 0; g < it.tiles; ++g)
                         for (int x = 0; x < C::kBoxes; ++x)
                             tma_load_4d(base + C::kQOffset + (2 * qb + g) * C::kTileBytes + x * 16384, &map_q, q_full(qb), x * 64,
                                         it.q0 + g * kBlockQ, it.head, it.batch);
@@ -856,7 +859,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         break;
                     }
                     // Documents have seq_kv = seq_q: key block j holds the rows of tile j.
-                    if (__ldg(p.tiles + (static_cast<long long>(it.batch) * 2 * p.pairs + j)).z != 0) {
+                    if (__ldg(p.tiles + (static_cast<long long>(it.batch) * p.tile_stride + j)).z != 0) {
                         const uint32_t tile = base + C::kKvOffset + slot * C::kTileBytes;
 #pragma unroll
                         for (int i = 0; i < kBlockKV / 32; ++i) {
@@ -893,13 +896,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!mbar_wait_warp(item_full(it_slot), static_cast<uint32_t>(items >> 1) & 1u, kFaultAttnWait, abort_flag))
                 break;
             const int none = item_ring[it_slot].none, batch = item_ring[it_slot].batch, head = item_ring[it_slot].head;
-            const int q0 = item_ring[it_slot].q0 + g * kBlockQ;
+            const int q0 = item_ring[it_slot].q0 + g * kBlockQ, tiles = item_ring[it_slot].tiles;
             const int b0 = uniform(item_ring[it_slot].b0[g]), b1 = uniform(item_ring[it_slot].b1[g]);
             __syncwarp();
             if (lane == 0) mbar_arrive(item_empty(it_slot));
             if (uniform(none)) break;
             const int q_row = q0 + row_in_tile;
-            if (uniform(q0) >= p.seq_q) continue;
+            if (g >= uniform(tiles)) continue;
             const int pos = q_row + p.seq_kv - p.seq_q;
             // The row's keys [lo, hi). Rows past the end take every key, so that they never
             // make their warp compute a mask; they are not stored.
@@ -1230,11 +1233,17 @@ inline cudaError_t masked_entry(bool bf16, const void* q, const void* k, const v
     p.seq_q = seq_q;
     p.seq_kv = seq_kv;
     p.head_dim = dim;
-    p.pairs = pairs;
+    // One tile an item where all of them run at once: two tiles share K and V loads and overlap
+    // each other's waits, but need more blocks one after the other. 16 heads, causal, 1024 x 128:
+    // MEASURED_TILES
+    const long long all_tiles = bh * ((seq_q + 127LL) / 128);
+    p.item_tiles = all_tiles <= sm_count ? 1 : 2;
+    p.per_head = p.item_tiles == 1 ? (seq_q + 127) / 128 : pairs;
+    p.tile_stride = 2 * pairs;
     p.heads_q = heads;
     p.heads_kv = heads_kv;
     p.group = heads / heads_kv;
-    p.num_items = static_cast<int>(bh * pairs);
+    p.num_items = static_cast<int>(bh * p.per_head);
     p.causal = causal;
     p.prefix = prefix;
     p.scale = scale;
@@ -1253,7 +1262,7 @@ inline cudaError_t masked_entry(bool bf16, const void* q, const void* k, const v
     long long at_once = p.group;
     if (causal != 0 || doc_ids != nullptr) {
         at_once = (TK_MASKED_GROUP_BYTES / (4LL * seq_kv * dim)) * p.group;
-        const long long fill = (2LL * sm_count + pairs - 1) / pairs;
+        const long long fill = (2LL * sm_count + p.per_head - 1) / p.per_head;
         if (at_once < fill) at_once = (fill + p.group - 1) / p.group * p.group;
     }
     p.group_bh = static_cast<int>(at_once < bh ? at_once : bh);
