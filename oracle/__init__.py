@@ -46,11 +46,16 @@ def ref_root() -> str:
     return os.environ.get("REF_ROOT") or os.path.join(os.path.dirname(os.path.dirname(HERE)), "reference")
 
 
+def have_ref() -> bool:
+    """Whether the reference's sources are there (not merely an empty directory of that name)."""
+    return os.path.isfile(os.path.join(ref_root(), "src", "gemm.cu"))
+
+
 def build(ref: bool = False) -> None:
     """Compile the oracle (and, if asked and the reference tree exists, _ref)."""
     targets = ["all"]
     root = ref_root()
-    if ref and os.path.isdir(root):
+    if ref and have_ref():
         targets += ["ref", "legacy", f"REF_ROOT={root}"]
     subprocess.run(["make", "-s", "-C", HERE, *targets], check=True)
 
