@@ -4,7 +4,7 @@
 //
 // It computes nothing. It exists because the smallest of these calls take a few
 // microseconds on the GPU, and looking at a dozen tensors from Python takes longer than
-// that (kv_append of 64 tokens: 11 us in Python with ctypes, PYTHON_MEASURED us here).
+// that (kv_append of 64 tokens: 11 us in Python with ctypes, 4.9 us here).
 //
 // Built as the extension module tk_b200/_ops.so against the installed torch; the library
 // itself, libtk_b200.so, needs neither torch nor Python.
