@@ -128,6 +128,24 @@ def test_document_layouts(layout):
 
 
 @pytest.mark.parametrize("kind", [F16, BF16], ids=["f16", "bf16"])
+def test_many_items_without_keys(kind):
+    """One CTA after another meets runs of items that see nothing: 96 heads of 8 query pairs, most of
+    them padding, so that each takes several, in either size of the pipeline."""
+    s = 2048
+    ids = np.full((1, s), -1, np.int32)
+    ids[0, 130:200] = 1
+    ids[0, 1900:1930] = 2
+    for d in (64, 128):
+        q, k, v = make(1, 96, s, d, kind, 70), make(1, 96, s, d, kind, 71), make(1, 96, s, d, kind, 72)
+        for causal in (False, True):
+            out = torch.full_like(q, float("nan"))
+            tk_b200.attention_masked(q, k, v, scale=0.1, causal=causal, doc_ids=torch.from_numpy(ids).cuda(), out=out)
+            held(q, k, v, out, scale=0.1, causal=causal, ids=ids, heads=range(0, 96, 19))
+            assert torch.count_nonzero(out[:, :, 200:1900]) == 0 and torch.count_nonzero(out[:, :, :130]) == 0
+    assert tk_b200.device_status() == 0
+
+
+@pytest.mark.parametrize("kind", [F16, BF16], ids=["f16", "bf16"])
 def test_padding_may_hold_anything(kind):
     """NaN and infinities in Q, K and V at padding positions reach no other row."""
     s, d = 500, 128

@@ -180,7 +180,7 @@ __device__ __forceinline__ void plan_rest(const PlanParams& p, long long tokens,
     for (long long t = tokens + rank * kPlanThreads + threadIdx.x; t < p.max_tokens; t += ctas * kPlanThreads) p.slots[t] = -1;
 }
 
-// One CTA, requests 1024 at a time:
+// Requests 1024 at a time:
 //
 //   need_r  = ceil((c_r + n_r) / page) - ceil(c_r / page)
 //   taken_r = n_r > 0, the row and the slots are wide enough, and need_r = 0 or
@@ -188,15 +188,19 @@ __device__ __forceinline__ void plan_rest(const PlanParams& p, long long tokens,
 //   page k of the call = free_pages[n_free - 1 - k]
 //
 // Two prefix sums (new tokens, pages needed), the lengths, and with kFill the entries and
-// slots too. Without it plan_fill_kernel follows with as many CTAs as the slots need. It
-// works from this kernel's outputs alone, so no scratch is passed between the two.
+// slots too: then every CTA computes the sums for itself, CTA 0 writes the lengths, and the
+// CTAs share out the rest. That needs inputs that CTA 0 does not overwrite. Where lens_out is
+// `cached` (a state that moves on in place) and there is more to fill than one CTA should, one
+// CTA does the sums without kFill, and plan_fill_kernel follows, which works from that kernel's
+// outputs alone, so that no scratch is passed between the two.
 // What bounds both: the launches and the chain lengths -> sums -> entries; the bytes are a
 // few MB at most (8 a slot). 1024 requests with 385,000 tokens: 39 us when one cluster of
-// 8 CTAs did all of it (8 SMs wait for their page numbers), 12.5 us in two kernels.
+// 8 CTAs did all of it (8 SMs wait for their page numbers), 12.4 us in two kernels, 8.6 in one.
 template <bool kFill>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
     __shared__ PlanPart part;
     const int tid = static_cast<int>(threadIdx.x);
+    const int rank = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
     if constexpr (!kFill) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int n_free = *p.n_free;
     n_free = n_free < 0 ? 0 : (n_free > p.free_capacity ? p.free_capacity : n_free);
@@ -219,8 +223,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
         const long long upto = pages + block_scan(need, part.warp_sums, page_sum);
         const bool taken = fits && (need == 0 || upto <= n_free);
         if (taken && need > 0) atomicMax(&part.used, static_cast<int>(upto));
-        if (r < p.n_requests) {
-            // Each thread has read its own request: lens_out may be `cached`.
+        if (rank == 0 && r < p.n_requests) {
+            // Each thread has read its own request: with one CTA lens_out may be `cached`.
             p.lens_out[r] = taken ? static_cast<int>(whole) : c;
             p.seq_lens[r] = taken ? static_cast<int>(whole) : 0;
             p.starts[r] = clamp_int(end - n);
@@ -234,17 +238,17 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
             part.base[tid] = static_cast<int>(upto - need) - have;
             part.taken[tid] = taken ? 1 : 0;
             __syncthreads();
-            plan_fill(p, part, r0, min(kPlanThreads, p.n_requests - r0), tokens, sum, pages, page_sum, n_free, 0, 1);
+            plan_fill(p, part, r0, min(kPlanThreads, p.n_requests - r0), tokens, sum, pages, page_sum, n_free, rank, ctas);
             __syncthreads();  // the shared arrays are rewritten by the next 1024 requests
         }
         tokens += sum;
         pages += page_sum;
     }
     __syncthreads();
-    if constexpr (kFill) plan_rest(p, tokens, 0, 1);
-    if (tid == 0) {
+    if constexpr (kFill) plan_rest(p, tokens, rank, ctas);
+    if (rank == 0 && tid == 0) {
         p.starts[p.n_requests] = clamp_int(tokens);
-        *p.n_free_out = n_free - part.used;  // read by this CTA alone, at its start
+        *p.n_free_out = n_free - part.used;  // may be n_free with one CTA: read at its start
     }
 }
 
@@ -303,9 +307,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_fill_kernel(const PlanParam
     plan_rest(p, tokens, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
 }
 
-// Up to this many slots and requests in one kernel of one CTA.
-constexpr int kPlanOneCta = 4096;
-
 inline cudaError_t plan_entry(const int* cached, const int* fresh, int n_requests, int page, int* table, int width,
                               const int* free_pages, int free_capacity, const int* n_free, int* lens_out, int* seq_lens,
                               int* starts, int64_t* slots, int max_tokens, int* n_free_out, cudaStream_t stream) {
@@ -335,16 +336,17 @@ inline cudaError_t plan_entry(const int* cached, const int* fresh, int n_request
     static_cast<void>(cudaGetLastError());
     PlanParams p{cached, fresh, n_requests, page, table, width, free_pages, free_capacity, n_free,
                  lens_out, seq_lens, starts, slots, max_tokens, n_free_out};
-    if (max_tokens <= kPlanOneCta && n_requests <= kPlanOneCta) {
-        plan_kernel<true><<<1, kPlanThreads, 0, stream>>>(p);
+    // A warp writes 128 slots at a time.
+    const long long want = (max_tokens + 4095LL) / 4096;
+    const unsigned ctas = static_cast<unsigned>(want < 1 ? 1 : (want < sm_count ? want : sm_count));
+    if (ctas == 1 || (lens_out != cached && n_free_out != n_free)) {
+        plan_kernel<true><<<ctas, kPlanThreads, 0, stream>>>(p);
         return cudaGetLastError();
     }
     plan_kernel<false><<<1, kPlanThreads, 0, stream>>>(p);
-    // A warp writes 128 slots at a time; programmatic dependent launch: this launch overlaps
-    // the first kernel.
-    const int want = (max_tokens + 4095) / 4096;
+    // Programmatic dependent launch: this launch overlaps the first kernel.
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(want < 1 ? 1 : (want < sm_count ? want : sm_count)));
+    cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kPlanThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
