@@ -409,8 +409,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int w = 4 * c + i;
-                    const uint32_t a0 = kv::from_e4m3x2(near[i] & 0xffffu), a2 = kv::from_e4m3x2(near[i] >> 16);
-                    const uint32_t a1 = kv::from_e4m3x2(far[i] & 0xffffu), a3 = kv::from_e4m3x2(far[i] >> 16);
+                    uint32_t a0, a1, a2, a3;
+                    kv::from_e4m3x4(near[i], a0, a2);
+                    kv::from_e4m3x4(far[i], a1, a3);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma_16816(s[u][nt], a0, a1, a2, a3, q[nt][2 * w], q[nt][2 * w + 1]);
                 }
@@ -519,9 +520,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const uint32_t pick = half == 0 ? 0x5140u : 0x7362u;
-                    const uint32_t near = __byte_perm(v[0][i], v[1][i], pick), far = __byte_perm(v[2][i], v[3][i], pick);
-                    const uint32_t a0 = kv::from_e4m3x2(near & 0xffffu), a1 = kv::from_e4m3x2(near >> 16);
-                    const uint32_t a2 = kv::from_e4m3x2(far & 0xffffu), a3 = kv::from_e4m3x2(far >> 16);
+                    uint32_t a0, a1, a2, a3;
+                    kv::from_e4m3x4(__byte_perm(v[0][i], v[1][i], pick), a0, a1);
+                    kv::from_e4m3x4(__byte_perm(v[2][i], v[3][i], pick), a2, a3);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][2 * i + half], a0, a1, a2, a3, b[nt][0], b[nt][1]);
                 }

@@ -39,6 +39,14 @@ __device__ __forceinline__ uint32_t from_e4m3x2(uint32_t two) {
     return r;
 }
 
+// Four e4m3 bytes to binary16: bytes 0 and 1 in lo, 2 and 3 in hi.
+__device__ __forceinline__ void from_e4m3x4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(four));
+}
+
 __device__ __forceinline__ float2 half2_bits_to_float2(uint32_t bits) {
     return __half22float2(*reinterpret_cast<const __half2*>(&bits));
 }
