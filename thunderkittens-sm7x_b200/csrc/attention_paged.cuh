@@ -270,9 +270,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
     const int lane = static_cast<int>(lane_id());
     const int warp = static_cast<int>(threadIdx.x >> 5);
     const int g = lane >> 2, t = lane & 3;
+    // x: items; y: chunks, so that first all first chunks start, then all second ones, and so on:
+    // those that ragged contexts do not reach come last.
     int rest = static_cast<int>(blockIdx.x);
-    const int split = rest % p.splits;
-    rest /= p.splits;
+    const int split = static_cast<int>(blockIdx.y);
     const int tile = rest % p.tiles;
     rest /= p.tiles;
     const int head = rest % p.heads_kv;
@@ -433,7 +434,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
                     const int j = token + 16 * u + g + (c >> 1) * 8;
                     if constexpr (kChange) {
                         if (cap > 0.0f) x = cap * tanh_of(x * over_cap);
-                        x = fmaf(static_cast<float>(j - rows.pos[nt][c & 1]), rows.slope[nt][c & 1], x * kLog2e);
+                        const float far = static_cast<float>(token + 16 * u + g - rows.pos[nt][c & 1]) + (c >> 1) * 8.0f;
+                        x = fmaf(far, rows.slope[nt][c & 1], x * kLog2e);
                     }
                     // Without a page a block's tokens are not there, whatever the ring holds.
                     if (partial && (!bl[u].on || j >= end || j > rows.pos[nt][c & 1])) x = -INFINITY;
@@ -684,14 +686,14 @@ cudaError_t launch_one(const Params& p, unsigned items, int device, cudaStream_t
         configured[device].store(true, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(items * p.splits);
+    cfg.gridDim = dim3(items, static_cast<unsigned>(p.splits));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = Smem<D, NT>::kBytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(p.splits);
-    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = static_cast<unsigned>(p.splits);
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = p.cluster ? 1 : 0;
