@@ -36,7 +36,7 @@ def check_plan(cached, new, page, width, n_pages, n_free, max_tokens, seed=0, in
     want_table = table.copy()
     lens, seq, starts, slots, left = plain64.plan(cached, new, page, want_table, free, n_free, max_tokens)
     d_cached, d_new, d_table, d_free, d_n = ints(cached), ints(new), ints(table).reshape(len(cached), width), ints(free), ints([n_free])
-    kw = dict(lens_out=d_cached, n_free_out=d_n) if in_place else {}
+    kw = dict(lens_out=d_cached, n_free_out=d_n) if in_place is True else dict(lens_out=d_cached) if in_place == "lens" else {}
     got = tk_b200.kv_plan(d_cached, d_new, d_table, d_free, d_n, page_size=page, max_tokens=max_tokens, **kw)
     torch.cuda.synchronize()
     assert np.array_equal(d_table.cpu().numpy(), want_table)
@@ -47,11 +47,11 @@ def check_plan(cached, new, page, width, n_pages, n_free, max_tokens, seed=0, in
         assert d_cached.cpu().tolist() == list(cached) and d_n.item() == n_free
 
 
-@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("in_place", [False, True, "lens"])
 @pytest.mark.parametrize("requests,page,longest,prompt", [(1, 16, 1, 1), (1, 1, 40, 7), (5, 7, 100, 30), (64, 32, 4096, 1),
                                                           (1024, 16, 300, 5), (1025, 16, 100, 1), (2500, 128, 1000, 40), (37, 64, 9, 1000)])
 def test_plan(requests, page, longest, prompt, in_place):
-    """One CTA and the cluster, one group of requests and several, places to spare."""
+    """One CTA and many, one kernel and two (in place), one group of requests and several."""
     g = np.random.default_rng(requests)
     cached = g.integers(0, longest, requests).tolist()
     new = g.integers(0, prompt + 1, requests).tolist()
@@ -70,11 +70,12 @@ def test_plan_runs_out():
             check_plan(cached, new, 16, 4, 60, n_free, max_tokens, seed=n_free + 9)
     check_plan(cached, new, 16, 4, 60, 20, 200, holes=True)
     check_plan(cached, new, 16, 4, 60, 10 ** 6, 200)  # more than the list holds: what it holds
-    # the cluster, and a second group of requests after the pages ran out
+    # many CTAs, and a second group of requests after the pages ran out
     g = np.random.default_rng(3)
     cached, new = g.integers(0, 50, 2300).tolist(), g.integers(0, 60, 2300).tolist()
     for n_free in (0, 700, 3000):
-        check_plan(cached, new, 16, 6, 9000, n_free, 40000, in_place=True)
+        for in_place in (False, True):
+            check_plan(cached, new, 16, 6, 9000, n_free, 40000, in_place=in_place)
 
 
 def test_plan_of_nothing():

@@ -373,14 +373,15 @@ __device__ __forceinline__ void mask_row(uint32_t (&r)[128], const Chunks& k, in
 // head_dim 64: 363 against 325 us); with documents they pay (138 against 148 us), and so do they
 // for capped scores, whose whole blocks go another way. Both forms in one kernel lose to
 // either alone there (391 against 355 us): each is 64 pairs of code.
-template <bool kBf16, bool kSkip>
-__device__ __forceinline__ float exp_store(uint32_t p_addr, const uint32_t (&r)[128], float c, float a, uint32_t live) {
+template <bool kBf16, bool kSkip, class Mid>
+__device__ __forceinline__ float exp_store(uint32_t p_addr, const uint32_t (&r)[128], float c, float a, uint32_t live, Mid&& mid) {
     float2 acc[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) acc[t] = make_float2(0.0f, 0.0f);
     const float2 c2 = make_float2(c, c), a2 = make_float2(a, a);
 #pragma unroll
     for (int chunk = 0; chunk < 4; ++chunk) {
+        if (chunk == 2) mid();
         uint32_t pk[16];
         if (kSkip && !(live >> chunk & 1)) {
 #pragma unroll
@@ -493,8 +494,8 @@ __device__ __forceinline__ void cap_row(uint32_t (&r)[128], float out) {
 
 // exp_store of capped scores straight from z: the argument's own multiply-add takes the last
 // product of the polynomial.
-template <bool kBf16, CapRange kRange>
-__device__ __forceinline__ float cap_exp_store(uint32_t p_addr, const uint32_t (&r)[128], float out, float a) {
+template <bool kBf16, CapRange kRange, class Mid>
+__device__ __forceinline__ float cap_exp_store(uint32_t p_addr, const uint32_t (&r)[128], float out, float a, Mid&& mid) {
     const CapPoly<kRange> poly(out);
     float2 acc[4];
 #pragma unroll
@@ -502,6 +503,7 @@ __device__ __forceinline__ float cap_exp_store(uint32_t p_addr, const uint32_t (
     const float2 a2 = make_float2(a, a);
 #pragma unroll
     for (int chunk = 0; chunk < 4; ++chunk) {
+        if (chunk == 2) mid();
         uint32_t pk[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -559,6 +561,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t base = (raw_base + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (base - raw_base);
     const uint32_t bars = base + C::kBarOffset;
+    // Where P overwrites S, its first 64 keys are announced while the others' exponentials run (on
+    // s_free, which is not used otherwise), and PV begins on them: 6 % at head_dim 128 (unmasked
+    // bfloat16, 2 x 32 heads, 4096: 474 to 443 us). With capped scores it loses 2 %.
+    constexpr bool kEarly = !C::kApart && (kKind == kPlain || kKind == kBias);
     constexpr int kSlots = C::kSlots;
     auto kv_full = [&](int s) { return bars + 8u * s; };
     auto kv_empty = [&](int s) { return bars + 8u * (kSlots + s); };
@@ -714,10 +720,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     commit_elect(s_full(g));
                 };
-                auto issue_pv = [&](int g, uint32_t v_addr, bool first) {
+                auto issue_pv = [&](int g, uint32_t v_addr, bool first, int k0, int k1) {
                     const uint64_t dv = sw128_desc(v_addr, 16384, 1024);
 #pragma unroll
-                    for (int kk = 0; kk < kBlockKV / 16; ++kk)
+                    for (int kk = k0; kk < k1; ++kk)
                         mma_ts_elect(tmem + 256u * g + 128u, tmem + 256u * g + C::kPOffset + kk * 8,
                                    dv + static_cast<uint64_t>((kk * 2048) >> 4), C::kIdescO, (!first || kk > 0) ? 1u : 0u);
                 };
@@ -759,12 +765,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                     };
                     // PV of tile g, block j, once its probabilities are there.
                     auto pv = [&](int g, int j) {
+                        const bool first = j == it.b0[g];
+                        const uint32_t v = kv_addr(slot_of(2 * (j - it.jb) + 1));
+                        if constexpr (kEarly) {
+                            if (!mbar_wait_warp(s_free(g), pr_phase[g], kFaultAttnWait, abort_flag)) return false;
+                            if (first && !o_free(g)) return false;
+                            tc_fence_after();
+                            issue_pv(g, v, first, 0, 4);
+                        }
                         if (!mbar_wait_warp(p_ready(g), pr_phase[g], kFaultAttnWait, abort_flag)) return false;
                         pr_phase[g] ^= 1u;
-                        const bool first = j == it.b0[g];
-                        if (first && !o_free(g)) return false;
+                        if (!kEarly && first && !o_free(g)) return false;
                         tc_fence_after();
-                        issue_pv(g, kv_addr(slot_of(2 * (j - it.jb) + 1)), first);
+                        if constexpr (kEarly) issue_pv(g, v, false, 4, 8);
+                        else issue_pv(g, v, first, 0, 8);
                         if (C::kApart || j == it.b1[g] - 1) commit_elect(o_final(g));
                         return true;
                     };
@@ -991,29 +1005,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                     of_phase ^= 1u;
                     tc_fence_after();
                 }
+                // tcgen05.ld/st are warp-collective: the rescale runs for the whole warp when any of
+                // its rows needs it. PV_{j-1} has completed (in-order tcgen05, or waited for).
+                auto rescale = [&]() {
+                    if (j > b0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+#pragma unroll
+                        for (int x = 0; x < kDPad / 16; ++x) {
+                            uint32_t o[16];
+                            tmem_ld_32x32b_x16(o_addr + 16 * x, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_st_32x32b_x16(o_addr + 16 * x, o);
+                        }
+                    }
+                };
+                if constexpr (kEarly) rescale();
+                auto mid = [&]() {
+                    if constexpr (kEarly) {
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(s_free(g));
+                    }
+                };
                 const float a = kLift - (m_use == -INFINITY ? 0.0f : m_use);
                 float e_sum;
                 if (kKind == kCap && fused) {
-                    e_sum = range == kNear ? cap_exp_store<kBf16, kNear>(s_addr + C::kPOffset, r, cap_out, a)
-                                           : cap_exp_store<kBf16, kMid>(s_addr + C::kPOffset, r, cap_out, a);
+                    e_sum = range == kNear ? cap_exp_store<kBf16, kNear>(s_addr + C::kPOffset, r, cap_out, a, mid)
+                                           : cap_exp_store<kBf16, kMid>(s_addr + C::kPOffset, r, cap_out, a, mid);
                 } else {
                     constexpr bool kSkip = kDocs || kKind == kCap || kKind == kCapBias;
-                    e_sum = exp_store<kBf16, kSkip>(s_addr + C::kPOffset, r, c, base + a, chunks.live);
+                    e_sum = exp_store<kBf16, kSkip>(s_addr + C::kPOffset, r, c, base + a, chunks.live, mid);
                 }
-                // tcgen05.ld/st are warp-collective: the rescale runs for the whole warp
-                // when any of its rows needs it.
-                if (j > b0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-                    // PV_{j-1} has completed (in-order tcgen05).
-#pragma unroll
-                    for (int x = 0; x < kDPad / 16; ++x) {
-                        uint32_t o[16];
-                        tmem_ld_32x32b_x16(o_addr + 16 * x, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                        tmem_st_32x32b_x16(o_addr + 16 * x, o);
-                    }
-                }
+                if constexpr (!kEarly) rescale();
                 l_run = l_run * alpha + e_sum;
                 m_run = m_use;
                 tmem_wait_st();
