@@ -200,7 +200,8 @@ __device__ __forceinline__ int block_running(int v, int* warp_values, int& all) 
 __global__ void __launch_bounds__(kRunThreads) runs_kernel(const int* __restrict__ ids, int seq, int n_tiles, int causal,
                                                            int2* rows, int4* tiles, int* next_item) {
     __shared__ int warp_values[32];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    grid_release();
+    grid_wait();
     const int tid = static_cast<int>(threadIdx.x);
     const int s0 = static_cast<int>(blockIdx.x) * kRunThreads;
     const int s = s0 + tid;
@@ -275,7 +276,8 @@ __global__ void __launch_bounds__(kRunThreads) runs_kernel(const int* __restrict
 }
 
 __global__ void zero_kernel(int* counter) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    grid_release();
+    grid_wait();
     *counter = 0;
 }
 
@@ -616,8 +618,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(*tmem_slot)));
-    // The kernel before zeroes the counter and finds the documents (programmatic dependent launch).
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // The kernel before zeroes the counter and finds the documents.
+    grid_wait();
 
     if (warp >= 8) {
         setmaxnreg_dec<kRegsControl>();
@@ -1130,7 +1132,7 @@ __global__ void gather_rows_kernel(const uint16_t* src, long long sb, long long 
 }
 
 template <int kDPad, bool kBf16, Kind kKind, bool kDocs>
-cudaError_t launch_kernel(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, bool after, int device,
+cudaError_t launch_kernel(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int device,
                         int grid, cudaStream_t stream) {
     using C = Cfg<kDPad, kBf16>;
     static std::atomic<bool> configured[host::kMaxDevices];
@@ -1140,36 +1142,25 @@ cudaError_t launch_kernel(const CUtensorMap& mq, const CUtensorMap& mk, const CU
         if (e != cudaSuccess) return e;
         configured[device].store(true, std::memory_order_release);
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = C::kSmemBytes;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = after ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, p);
+    return host::launch_overlapped(kernel, dim3(static_cast<unsigned>(grid)), kThreads, C::kSmemBytes, stream, mq, mk, mv, p);
 }
 
 template <int kDPad, bool kBf16, Kind kKind>
-cudaError_t launch_kind(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, bool after, int device,
+cudaError_t launch_kind(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int device,
                         int grid, cudaStream_t stream) {
-    return p.rows != nullptr ? launch_kernel<kDPad, kBf16, kKind, true>(mq, mk, mv, p, after, device, grid, stream)
-                             : launch_kernel<kDPad, kBf16, kKind, false>(mq, mk, mv, p, after, device, grid, stream);
+    return p.rows != nullptr ? launch_kernel<kDPad, kBf16, kKind, true>(mq, mk, mv, p, device, grid, stream)
+                             : launch_kernel<kDPad, kBf16, kKind, false>(mq, mk, mv, p, device, grid, stream);
 }
 
-// after: a kernel of this call, launched right before, that this one depends on.
 template <int kDPad, bool kBf16>
-cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, bool after, int device,
+cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int device,
                    int grid, cudaStream_t stream) {
     const bool bias = p.slopes != nullptr || (p.softcap == 0.0f && !(p.scale > 0.0f));
     if (p.softcap > 0.0f)
-        return bias ? launch_kind<kDPad, kBf16, kCapBias>(mq, mk, mv, p, after, device, grid, stream)
-                    : launch_kind<kDPad, kBf16, kCap>(mq, mk, mv, p, after, device, grid, stream);
-    return bias ? launch_kind<kDPad, kBf16, kBias>(mq, mk, mv, p, after, device, grid, stream)
-                : launch_kind<kDPad, kBf16, kPlain>(mq, mk, mv, p, after, device, grid, stream);
+        return bias ? launch_kind<kDPad, kBf16, kCapBias>(mq, mk, mv, p, device, grid, stream)
+                    : launch_kind<kDPad, kBf16, kCap>(mq, mk, mv, p, device, grid, stream);
+    return bias ? launch_kind<kDPad, kBf16, kBias>(mq, mk, mv, p, device, grid, stream)
+                : launch_kind<kDPad, kBf16, kPlain>(mq, mk, mv, p, device, grid, stream);
 }
 
 // Strides of a dimension of size 1 are never used; the others have to be positive.
@@ -1342,23 +1333,24 @@ inline cudaError_t masked_entry(bool bf16, const void* q, const void* k, const v
         p.tiles = reinterpret_cast<const int4*>(scratch + tiles_at);
         p.rows = reinterpret_cast<const int2*>(scratch + rows_at);
         const dim3 blocks(static_cast<unsigned>((256LL * pairs + kRunThreads - 1) / kRunThreads), static_cast<unsigned>(batch));
-        runs_kernel<<<blocks, kRunThreads, 0, stream>>>(doc_ids, seq_q, 2 * pairs, causal,
-                                                        reinterpret_cast<int2*>(scratch + rows_at),
-                                                        reinterpret_cast<int4*>(scratch + tiles_at), p.next_item);
+        err = host::launch_overlapped(runs_kernel, blocks, kRunThreads, 0, stream, doc_ids, seq_q, 2 * pairs, causal,
+                                      reinterpret_cast<int2*>(scratch + rows_at), reinterpret_cast<int4*>(scratch + tiles_at),
+                                      p.next_item);
     } else if (counted) {
-        zero_kernel<<<1, 1, 0, stream>>>(p.next_item);
+        err = host::launch_overlapped(zero_kernel, dim3(1), 1, 0, stream, p.next_item);
     }
-    const bool after = doc_ids != nullptr || counted;
     CUtensorMap mq, mk, mv;
-    if (!(make_map(&mq, vq, batch, heads, seq_q, dim) && make_map(&mk, vk, batch, heads_kv, seq_kv, dim) &&
+    if (err != cudaSuccess) {
+        // nothing more is launched
+    } else if (!(make_map(&mq, vq, batch, heads, seq_q, dim) && make_map(&mk, vk, batch, heads_kv, seq_kv, dim) &&
           make_map(&mv, vv, batch, heads_kv, seq_kv, dim))) {
         err = cudaErrorInvalidValue;
     } else {
         switch ((dim == 128 ? 2 : 0) + (bf16 ? 1 : 0)) {
-            case 0: err = launch<64, false>(mq, mk, mv, p, after, device, grid, stream); break;
-            case 1: err = launch<64, true>(mq, mk, mv, p, after, device, grid, stream); break;
-            case 2: err = launch<128, false>(mq, mk, mv, p, after, device, grid, stream); break;
-            default: err = launch<128, true>(mq, mk, mv, p, after, device, grid, stream); break;
+            case 0: err = launch<64, false>(mq, mk, mv, p, device, grid, stream); break;
+            case 1: err = launch<64, true>(mq, mk, mv, p, device, grid, stream); break;
+            case 2: err = launch<128, false>(mq, mk, mv, p, device, grid, stream); break;
+            default: err = launch<128, true>(mq, mk, mv, p, device, grid, stream); break;
         }
     }
     if (scratch != nullptr) cudaFreeAsync(scratch, stream);

@@ -285,6 +285,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
     const int begin = split * p.chunk;
     const int* table = p.table + static_cast<long long>(r) * p.width;
     int page_of[kStages][kB];
+    grid_wait();
 #pragma unroll
     for (int i = 0; i < kStages; ++i) {
 #pragma unroll
@@ -552,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
         }
     }
     cp_async_wait<0>();
-    if (!p.cluster) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (!p.cluster) grid_release();
     __syncthreads();
 
     // Join the four warps, in warp order.
@@ -642,7 +643,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     const int runs = p.join_runs;
     const int slot = static_cast<int>(threadIdx.x) / kQuads, quad = static_cast<int>(threadIdx.x) % kQuads;
     const int run = slot % runs, row = part * (kJoinThreads / kQuads / runs) + slot / runs;
-    if (part * (kJoinThreads / kQuads / runs) >= n_rows) return;
+    if (part * (kJoinThreads / kQuads / runs) >= n_rows) {
+        grid_wait();  // also where there is nothing to do: this grid must not end before the one it follows
+        return;
+    }
     const int kv_end = max(rq.len - rq.n + (tile * kRows + n_rows - 1) / p.group + 1, 0);
     const int used = max(min((kv_end + p.chunk - 1) / p.chunk, p.splits), 1);
     const long long item = item_of(p, r, head, tile, 0);
@@ -650,7 +654,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     const int last = row < n_rows ? min((run + 1) * each, used) : 0;
     const float2* ml_at = p.part_ml + item * kRows + row;
     const float* o_at = p.part_o + (item * kRows + row) * D + quad * 4;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    grid_wait();
     Merged x;
     for (int s = run * each; s < last; s += 4) {
         float2 ml[4];
@@ -685,18 +689,22 @@ cudaError_t launch_one(const Params& p, unsigned items, int device, cudaStream_t
         if (e != cudaSuccess) return e;
         configured[device].store(true, std::memory_order_release);
     }
+    const dim3 grid(items, static_cast<unsigned>(p.splits));
+    if (!p.cluster) return host::launch_overlapped(kernel, grid, kThreads, Smem<D, NT>::kBytes, stream, p);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(items, static_cast<unsigned>(p.splits));
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = Smem<D, NT>::kBytes;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1;
     attr[0].val.clusterDim.y = static_cast<unsigned>(p.splits);
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = p.cluster ? 1 : 0;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
@@ -705,17 +713,7 @@ cudaError_t launch(const Params& p, bool change, unsigned items, int device, cud
     cudaError_t err = change ? launch_one<D, NT, kBf16, true>(p, items, device, stream)
                              : launch_one<D, NT, kBf16, false>(p, items, device, stream);
     if (err != cudaSuccess || p.part_o == nullptr) return err;
-    // Programmatic dependent launch: the join's launch overlaps the last chunks.
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(items * p.join_ctas);
-    cfg.blockDim = dim3(kJoinThreads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, join_kernel<D, NT, kBf16>, p);
+    return host::launch_overlapped(join_kernel<D, NT, kBf16>, dim3(items * p.join_ctas), kJoinThreads, 0, stream, p);
 }
 
 inline cudaError_t paged_entry(bool bf16, const void* q, long long q_stride, void* out, long long out_stride, int n_tokens,

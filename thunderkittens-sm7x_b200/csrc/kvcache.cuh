@@ -209,7 +209,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     __shared__ PlanPart part;
     const int tid = static_cast<int>(threadIdx.x);
     const int rank = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
-    if constexpr (!kFill) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if constexpr (!kFill) grid_release();
+    grid_wait();
     int n_free = *p.n_free;
     n_free = n_free < 0 ? 0 : (n_free > p.free_capacity ? p.free_capacity : n_free);
     if (tid == 0) part.used = 0;
@@ -266,7 +267,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
 __global__ void __launch_bounds__(kPlanThreads) plan_fill_kernel(const PlanParams p) {
     __shared__ PlanPart part;
     const int tid = static_cast<int>(threadIdx.x);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    grid_wait();
     // The pages taken in all: free_pages counts from the n_free before the call.
     long long used = 0;
     for (int r0 = 0; r0 < p.n_requests; r0 += kPlanThreads) {
@@ -348,23 +349,12 @@ inline cudaError_t plan_entry(const int* cached, const int* fresh, int n_request
     const long long want = (max_tokens + 4095LL) / 4096;
     const unsigned ctas = static_cast<unsigned>(want < 1 ? 1 : (want < sm_count ? want : sm_count));
     if (ctas == 1 || (lens_out != cached && n_free_out != n_free)) {
-        plan_kernel<true><<<ctas, kPlanThreads, 0, stream>>>(p);
-        return cudaGetLastError();
+        err = host::launch_overlapped(plan_kernel<true>, dim3(ctas), kPlanThreads, 0, stream, p);
+        return err != cudaSuccess ? err : cudaGetLastError();
     }
-    plan_kernel<false><<<1, kPlanThreads, 0, stream>>>(p);
-    // Programmatic dependent launch: this launch overlaps the first kernel.
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(kPlanThreads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    err = cudaLaunchKernelEx(&cfg, plan_fill_kernel, p);
-    if (err != cudaSuccess) return err;
-    return cudaGetLastError();
+    err = host::launch_overlapped(plan_kernel<false>, dim3(1), kPlanThreads, 0, stream, p);
+    if (err == cudaSuccess) err = host::launch_overlapped(plan_fill_kernel, dim3(ctas), kPlanThreads, 0, stream, p);
+    return err != cudaSuccess ? err : cudaGetLastError();
 }
 
 // ---------------------------------------------------------------------------
@@ -477,6 +467,7 @@ __global__ void __launch_bounds__(kAppendThreads, kCta ? 8 : 1) append_kernel(co
     float* scales = values ? p.scale[1] : p.scale[0];
     const long long n_slots = p.n_pages * p.page;
     const int sub = in_group / kLanes, col = (in_group % kLanes) * 8;
+    grid_wait();
 
     // s_slots[1 + i]: slot of token t0 + i, -1 where there is no such token or place.
     for (int i = tid; i < 1 + count + p.page; i += kAppendThreads) {
@@ -663,16 +654,16 @@ inline cudaError_t append_entry(bool bf16, const void* k, const void* v, long lo
     if (ctas > INT_MAX) return cudaErrorInvalidValue;
     const dim3 grid(static_cast<unsigned>(ctas), 2);
     switch ((dim == 128 ? 4 : 0) + (bf16 ? 2 : 0) + (cta ? 1 : 0)) {
-        case 0: append_kernel<64, false, false><<<grid, kAppendThreads, 0, stream>>>(p); break;
-        case 1: append_kernel<64, false, true><<<grid, kAppendThreads, 0, stream>>>(p); break;
-        case 2: append_kernel<64, true, false><<<grid, kAppendThreads, 0, stream>>>(p); break;
-        case 3: append_kernel<64, true, true><<<grid, kAppendThreads, 0, stream>>>(p); break;
-        case 4: append_kernel<128, false, false><<<grid, kAppendThreads, 0, stream>>>(p); break;
-        case 5: append_kernel<128, false, true><<<grid, kAppendThreads, 0, stream>>>(p); break;
-        case 6: append_kernel<128, true, false><<<grid, kAppendThreads, 0, stream>>>(p); break;
-        default: append_kernel<128, true, true><<<grid, kAppendThreads, 0, stream>>>(p); break;
+        case 0: err = host::launch_overlapped(append_kernel<64, false, false>, grid, kAppendThreads, 0, stream, p); break;
+        case 1: err = host::launch_overlapped(append_kernel<64, false, true>, grid, kAppendThreads, 0, stream, p); break;
+        case 2: err = host::launch_overlapped(append_kernel<64, true, false>, grid, kAppendThreads, 0, stream, p); break;
+        case 3: err = host::launch_overlapped(append_kernel<64, true, true>, grid, kAppendThreads, 0, stream, p); break;
+        case 4: err = host::launch_overlapped(append_kernel<128, false, false>, grid, kAppendThreads, 0, stream, p); break;
+        case 5: err = host::launch_overlapped(append_kernel<128, false, true>, grid, kAppendThreads, 0, stream, p); break;
+        case 6: err = host::launch_overlapped(append_kernel<128, true, false>, grid, kAppendThreads, 0, stream, p); break;
+        default: err = host::launch_overlapped(append_kernel<128, true, true>, grid, kAppendThreads, 0, stream, p); break;
     }
-    return cudaGetLastError();
+    return err != cudaSuccess ? err : cudaGetLastError();
 }
 
 }  // namespace kv

@@ -152,6 +152,25 @@ inline cudaError_t scratch_pool_bytes(int device, uint64_t* reserved, uint64_t* 
     return cudaMemPoolGetAttribute(sp.pools[device], cudaMemPoolAttrUsedMemCurrent, used);
 }
 
+// Launches a kernel that begins with griddepcontrol.wait as a programmatic dependent of what is
+// before it on the stream: its launch then overlaps the end of that kernel. The wait comes before
+// the first access to global memory in every thread that makes one, so the order of the stream
+// holds as for any launch.
+template <class... P, class... A>
+cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // Softmax scale and score cap of the attention entry points with score changes: a finite
 // scale (in log2 units too), and a cap that is 0 (none) or leaves the factors scale / cap
 // and cap * log2(e) finite and normal.

@@ -441,6 +441,12 @@ __device__ __forceinline__ void setmaxnreg_dec() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegs));
 }
 
+// Programmatic dependent launch. grid_wait: until the kernels before this one on the stream are
+// complete and their writes visible (at once in an ordinary launch). grid_release: the kernel
+// launched after this one may start and run up to its own wait.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // 1 / x to about 1 ulp; 0 for an infinite x.
 __device__ __forceinline__ float rcp_approx(float x) {
     float y;
