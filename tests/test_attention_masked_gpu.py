@@ -80,6 +80,63 @@ def test_softcap(cap, spread, kind):
     held(q, k, v, out, scale=0.09, causal=True, cap=cap)
 
 
+@pytest.mark.parametrize("cap,scale", [(1e7, 0.09), (1e25, 0.09), (1e30, 1e-3), (300.0, 1e-9), (1e-5, 0.09), (5.0, 1e4), (2.0, -0.09), (2.0, 0.0)])
+def test_softcap_of_any_size(cap, scale):
+    """A cap far above the scores changes nothing; one far below them leaves their signs."""
+    q, k, v = make(1, 2, 300, 64, F16, 60, 4.0), make(1, 2, 300, 64, F16, 61), make(1, 2, 300, 64, F16, 62)
+    out = tk_b200.attention_masked(q, k, v, scale=scale, causal=True, softcap=cap)
+    held(q, k, v, out, scale=scale, causal=True, cap=0.0 if cap > 1e6 else cap)
+    assert tk_b200.device_status() == 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("spread", [1.0, 12.0, 60.0])
+def test_softcap_of_mixed_rows(spread, d):
+    """Rows and keys of very different sizes: small and large scores change places along a row."""
+    q, k, v = make(1, 2, 600, d, BF16, 63), make(1, 1, 900, d, BF16, 64), make(1, 1, 900, d, BF16, 65)
+    size = torch.ones(900, device="cuda")
+    size[130:140] = spread
+    size[600:610] = spread
+    k, q = k * size[:, None].to(BF16), q * torch.linspace(0, 4, 600, device="cuda")[:, None].to(BF16)
+    out = tk_b200.attention_masked(q, k, v, scale=0.1, causal=True, softcap=6.0)
+    held(q, k, v, out, scale=0.1, causal=True, cap=6.0)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cap", [50.0, 0.7])
+def test_softcap_under_masks(cap, d):
+    """Documents with padding that holds NaN, a prefix, and rows before the first key."""
+    s = 400
+    ids = documents(1, s, 70)
+    ids[0, 100:240] = -1
+    q, k, v = make(1, 4, s, d, F16, 71, 3.0), make(1, 2, s, d, F16, 72), make(1, 2, s, d, F16, 73)
+    for causal in (False, True):
+        held(q, k, v, tk_b200.attention_masked(q, k, v, scale=0.1, causal=causal, softcap=cap, doc_ids=torch.from_numpy(ids).cuda()),
+             scale=0.1, causal=causal, cap=cap, ids=ids)
+    prefix = [130]
+    held(q, k, v, tk_b200.attention_masked(q, k, v, scale=0.1, causal=True, softcap=cap, prefix_lens=torch.tensor(prefix, dtype=torch.int32).cuda()),
+         scale=0.1, causal=True, cap=cap, prefix=prefix)
+    few = k[:, :, :150], v[:, :, :150]
+    held(q, *few, tk_b200.attention_masked(q, *few, scale=0.1, causal=True, softcap=cap), scale=0.1, causal=True, cap=cap)
+    pad = torch.from_numpy(ids[0] < 0).cuda()
+    for t in (q, k, v):
+        t[:, :, pad] = float("nan")
+    held(q, k, v, tk_b200.attention_masked(q, k, v, scale=0.1, causal=True, softcap=cap, doc_ids=torch.from_numpy(ids).cuda()),
+         scale=0.1, causal=True, cap=cap, ids=ids)
+
+
+@pytest.mark.parametrize("cap", [0.0, 50.0, 0.5])
+@pytest.mark.parametrize("key", [38, 135, 299])
+def test_nan_key(key, cap):
+    """A NaN key: rows that see it are NaN, those before it are as without it."""
+    q, k, v = make(1, 2, 300, 64, F16, 66, 3.0), make(1, 2, 300, 64, F16, 67), make(1, 2, 300, 64, F16, 68)
+    bad = k.clone()
+    bad[:, :, key] = float("nan")
+    out = tk_b200.attention_masked(q, bad, v, scale=0.125, causal=True, softcap=cap)
+    assert out[:, :, key:].isnan().all()
+    held(q[:, :, :key], k[:, :, :key], v[:, :, :key], out[:, :, :key], scale=0.125, causal=True, cap=cap)
+
+
 @pytest.mark.parametrize("cap", [0.0, 20.0])
 @pytest.mark.parametrize("causal", [False, True])
 def test_slopes(causal, cap):

@@ -30,9 +30,9 @@
 // What bounds it: the softmax, as in attention.cuh. A block of 128 keys takes a warp 1024 MUFU
 // cycles for its exponentials, two warps share each MUFU, and of the rest (loads from tensor
 // memory, max, sums, packing, masks, biases, caps) only part overlaps. Measured on B200, causal,
-// burst clocks: 2 x 32 heads on 2 x 8, 4096 x 128, no change of scores 257 us (1,070 TFLOP/s), softcap
-// 346 us (MUFU floor 115); 11 documents with slopes, 32 heads, 8192 x 64, 121 us (floor 32: 6 blocks an
-// item leave its start and end in sight); 64 heads, a prefix, 1001 rows on 2777 keys, 95 us (256
+// burst clocks: 2 x 32 heads on 2 x 8, 4096 x 128, no change of scores 246 us (1,120 TFLOP/s), softcap
+// 348 us (MUFU floor 115); 11 documents with slopes, 32 heads, 8192 x 64, 122 us (floor 32: 6 blocks an
+// item leave its start and end in sight); 64 heads, a prefix, 1001 rows on 2777 keys, 88 us (256
 // items on 148 SMs: two rounds).
 #pragma once
 
@@ -418,38 +418,20 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 
 // ---- softcap * tanh(s scale / softcap), in log2 units
 //
-// Where a warp's scores are small against the cap, tanh(y) = z Q(z^2) with z a multiple of y and
-// Q a polynomial (a least-squares fit of the relative error on Chebyshev nodes, reweighted
-// towards equal ripple), on the FMA pipe:
-//   kNear: |y| < 3/4,  z = 8/3 y, 5 coefficients, relative error 5.7e-7 (7.3e-7 in FP32)
-//   kMid:  |y| < 8/5,  z = 5/4 y, 9 coefficients, 2.5e-7 (6.5e-7 in FP32)
-// Both limits are |z| < 2, one bit of the exponent, so testing a row is an OR over it. Elsewhere
-// tanh(y) = 1 - 2 / (1 + e^2y), which is 1 and -1 where the exponential is infinite or 0: two MUFU
-// operations a score beside the softmax's own. 2 x 32 heads on 2 x 8, causal, 4096 x 128, softcap 50: 599 us
-// with that form everywhere, 346 with these, 257 without a cap.
-enum CapRange { kNear, kMid, kFar };
-
-template <CapRange kRange>
-struct CapPoly {
-    static constexpr int kTerms = kRange == kNear ? 5 : 9;
-    float2 co[kTerms];
-    __device__ __forceinline__ explicit CapPoly(float out) {
-        constexpr float near[5] = {3.74999791e-1f, -1.75754447e-2f, 9.83255915e-4f, -5.22008486e-5f, 1.89612661e-6f};
-        constexpr float mid[9] = {7.99999774e-1f, -1.70658499e-1f, 4.36336249e-2f, -1.11605870e-2f, 2.70939758e-3f, -5.68044372e-4f, 8.98020517e-5f, -8.98356757e-6f, 4.12556517e-7f};
-#pragma unroll
-        for (int n = 0; n < kTerms; ++n) {
-            const float c = (kRange == kNear ? near[n < 5 ? n : 0] : mid[n]) * out;
-            co[n] = make_float2(c, c);
-        }
-    }
-    __device__ __forceinline__ float2 operator()(float2 z) const {  // Q(z^2)
-        const float2 u = mul2(z, z);
-        float2 q = fma2(co[kTerms - 1], u, co[kTerms - 2]);
-#pragma unroll
-        for (int n = kTerms - 3; n >= 0; --n) q = fma2(q, u, co[n]);
-        return q;
-    }
-};
+// With z = 8/3 y, y = s scale / softcap:
+//   kNear: where all scores of a warp have |y| < 3/4, tanh(y) = z Q(z^2) on the FMA pipe, Q a
+//     polynomial of 5 coefficients (a least-squares fit of the relative error on Chebyshev nodes,
+//     reweighted towards equal ripple; 5.7e-7, 7.3e-7 in FP32). The limit is |z| < 2, one bit of the
+//     exponent, so testing a row is an OR over it.
+//   kFar: elsewhere 1 - 2 / (1 + e^2y), four scores to one reciprocal (of the product of their
+//     denominators): 1.25 MUFU operations a score beside the softmax's own. e^2y is cut at 2^30, where
+//     tanh is 1 in FP32, so that the product stays below 2^121.
+// The range is a warp's, for its 128 keys: taken for each 32 keys it was slower wherever one range held
+// throughout (384 and 495 us for the next two figures). 2 x 32 heads on 2 x 8, causal, 4096 x 128: no cap 246 us; cap 50,
+// standard deviation of the scores 6, near: 348; cap 10, far: 465 (617 with a reciprocal a score in a pass
+// of its own; 450 with a second polynomial where |y| < 8/5 suffices, which leaves 617 beyond it); cap 30,
+// both ranges along a row: 553, since the two loops share an instruction cache that holds one.
+enum CapRange { kNear, kFar };
 
 // r *= k; whether all of the warp's |r| are below 2 then.
 __device__ __forceinline__ bool scale_row(uint32_t (&r)[128], float k) {
@@ -467,54 +449,108 @@ __device__ __forceinline__ bool scale_row(uint32_t (&r)[128], float k) {
 
 // Scores to z, and the range the warp's lie in. over = scale / softcap.
 __device__ __forceinline__ CapRange cap_range(uint32_t (&r)[128], float over) {
-    if (scale_row(r, 8.0f / 3.0f * over)) return kNear;
-    return scale_row(r, 15.0f / 32.0f) ? kMid : kFar;
+    return scale_row(r, 8.0f / 3.0f * over) ? kNear : kFar;
 }
 
-// The capped score of one value in the scale of kMid and kFar (z = 5/4 y); out = softcap * log2(e).
-__device__ __forceinline__ float cap_far(float z, float out) {
-    return fmaf(-2.0f * out, rcp_approx(1.0f + ex2(z * (1.6f * kLog2e))), out);
+constexpr float kCapArg = 0.75f * kLog2e;  // e^2y = 2^(kCapArg z)
+
+// The capped score of one value; out = softcap * log2(e).
+__device__ __forceinline__ float cap_one(float z, float out) {
+    return fmaf(-2.0f * out, rcp_approx(1.0f + ex2(z * kCapArg)), out);
 }
 
-// z to capped scores, in place.
+// Capped scores plus a of four values at a time.
+template <CapRange kRange>
+struct Cap4;
+
+template <>
+struct Cap4<kNear> {
+    float2 co[5], a2;
+    __device__ __forceinline__ Cap4(float out, float a) : a2(make_float2(a, a)) {
+        constexpr float near[5] = {3.74999791e-1f, -1.75754447e-2f, 9.83255915e-4f, -5.22008486e-5f, 1.89612661e-6f};
+#pragma unroll
+        for (int n = 0; n < 5; ++n) co[n] = make_float2(near[n] * out, near[n] * out);
+    }
+    __device__ __forceinline__ void operator()(float2& z0, float2& z1) const {
+        z0 = one(z0);
+        z1 = one(z1);
+    }
+    __device__ __forceinline__ float2 one(float2 z) const {
+        const float2 u = mul2(z, z);
+        float2 q = fma2(co[4], u, co[3]);
+#pragma unroll
+        for (int n = 2; n >= 0; --n) q = fma2(q, u, co[n]);
+        return fma2(q, z, a2);
+    }
+};
+
+template <>
+struct Cap4<kFar> {
+    float2 twice, a2;
+    __device__ __forceinline__ Cap4(float out, float a) : twice(make_float2(-2.0f * out, -2.0f * out)), a2(make_float2(out + a, out + a)) {}
+    static __device__ __forceinline__ float cut(float t) {  // NaN stays NaN
+        float r;
+        asm("min.NaN.f32 %0, %1, 0f41F00000;" : "=f"(r) : "f"(t));
+        return r;
+    }
+    __device__ __forceinline__ float2 denominators(float2 z) const {
+        const float2 t = mul2(z, make_float2(kCapArg, kCapArg));
+        return attn::add2(make_float2(ex2(cut(t.x)), ex2(cut(t.y))), make_float2(1.0f, 1.0f));
+    }
+    __device__ __forceinline__ void operator()(float2& z0, float2& z1) const {
+        const float2 d0 = denominators(z0), d1 = denominators(z1);
+        const float2 d = mul2(d0, d1);
+        const float r = rcp_approx(d.x * d.y);
+        const float2 pairs = make_float2(r * d.y, r * d.x);  // 1 / (d0 d1)
+        z0 = fma2(mul2(pairs, d1), twice, a2);
+        z1 = fma2(mul2(pairs, d0), twice, a2);
+    }
+};
+
+// z to capped scores, in place. kFar takes a reciprocal a score: a NaN that a mask will hide must
+// not reach others.
 template <CapRange kRange>
 __device__ __forceinline__ void cap_row(uint32_t (&r)[128], float out) {
-    if constexpr (kRange == kFar) {
+    const Cap4<kNear> near(out, 0.0f);
+    const float2 twice = make_float2(-2.0f * out, -2.0f * out), out2 = make_float2(out, out);
 #pragma unroll
-        for (int i = 0; i < 128; ++i) r[i] = __float_as_uint(cap_far(__uint_as_float(r[i]), out));
-    } else {
-        const CapPoly<kRange> poly(out);
-#pragma unroll
-        for (int i = 0; i < 64; ++i) {
-            const float2 z = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-            const float2 x = mul2(poly(z), z);
-            r[2 * i] = __float_as_uint(x.x);
-            r[2 * i + 1] = __float_as_uint(x.y);
+    for (int i = 0; i < 128; i += 2) {
+        const float2 z = make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+        float2 x;
+        if constexpr (kRange == kNear) {
+            x = near.one(z);
+        } else {
+            const float2 t = mul2(z, make_float2(kCapArg, kCapArg));
+            const float2 d = attn::add2(make_float2(ex2(t.x), ex2(t.y)), make_float2(1.0f, 1.0f));
+            x = fma2(make_float2(rcp_approx(d.x), rcp_approx(d.y)), twice, out2);
         }
+        r[i] = __float_as_uint(x.x);
+        r[i + 1] = __float_as_uint(x.y);
     }
 }
 
-// exp_store of capped scores straight from z: the argument's own multiply-add takes the last
-// product of the polynomial.
+// exp_store of capped scores straight from z. kNear: -inf becomes a weight of 0.
 template <bool kBf16, CapRange kRange, class Mid>
 __device__ __forceinline__ float cap_exp_store(uint32_t p_addr, const uint32_t (&r)[128], float out, float a, Mid&& mid) {
-    const CapPoly<kRange> poly(out);
+    const Cap4<kRange> cap(out, a);
     float2 acc[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) acc[t] = make_float2(0.0f, 0.0f);
-    const float2 a2 = make_float2(a, a);
 #pragma unroll
     for (int chunk = 0; chunk < 4; ++chunk) {
         if (chunk == 2) mid();
         uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < 16; i += 2) {
             const int idx = 32 * chunk + 2 * i;
-            const float2 z = make_float2(__uint_as_float(r[idx]), __uint_as_float(r[idx + 1]));
-            const float2 x = fma2(z, poly(z), a2);
-            const float2 e = make_float2(ex2(x.x), ex2(x.y));
-            acc[i & 3] = attn::add2(acc[i & 3], e);
-            pk[i] = pack2<kBf16>(e.x, e.y);
+            float2 z0 = make_float2(__uint_as_float(r[idx]), __uint_as_float(r[idx + 1]));
+            float2 z1 = make_float2(__uint_as_float(r[idx + 2]), __uint_as_float(r[idx + 3]));
+            cap(z0, z1);
+            const float2 e0 = make_float2(ex2(z0.x), ex2(z0.y)), e1 = make_float2(ex2(z1.x), ex2(z1.y));
+            acc[i & 3] = attn::add2(acc[i & 3], e0);
+            acc[(i + 1) & 3] = attn::add2(acc[(i + 1) & 3], e1);
+            pk[i] = pack2<kBf16>(e0.x, e0.y);
+            pk[i + 1] = pack2<kBf16>(e1.x, e1.y);
         }
         tmem_st_32x32b_x16(p_addr + 16 * chunk, pk);
     }
@@ -550,7 +586,7 @@ enum Kind {
     kPlain,        // a positive scale, folded into the exponent
     kCap,
     kBias,         // slopes, or a non-positive scale
-    kCapBias,
+    kCapBias,      // a cap of great size too
 };
 
 template <int kDPad, bool kBf16, Kind kKind, bool kDocs>
@@ -967,17 +1003,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // Scores in log2 units are r * c + base.
                 float c = p.scale_log2, base = 0.0f;
                 const float cap_out = p.softcap * kLog2e;
-                // Capped scores without a mask or bias go from z to P in one pass: capping keeps
-                // the order, so the row's max is found on z.
+                // The chunks are worked out before the bias (122 against 128 us with documents and slopes,
+                // 8192 x 64), but after a cap (348 against 352 us).
+                constexpr bool kCapped = kKind == kCap || kKind == kCapBias;
+                Chunks chunks{0, 15};
+                if (!kCapped && need_mask) chunks = chunks_of(lo - kv0, hi - kv0);
+                // Capped scores without a bias go from z to P in one pass, where a masked z of -inf ends as a
+                // weight of 0 (kNear) or none is masked. Capping keeps the order, so the row's max is found on z.
                 CapRange range = kFar;
                 bool fused = false;
-                if constexpr (kKind == kCap || kKind == kCapBias) {
+                if constexpr (kCapped) {
                     range = cap_range(r, p.scale / p.softcap);
-                    fused = kKind == kCap && !need_mask && range != kFar;
-                    if (!fused) {
-                        if (range == kNear) cap_row<kNear>(r, cap_out);
-                        else if (range == kMid) cap_row<kMid>(r, cap_out);
-                        else cap_row<kFar>(r, cap_out);
+                    fused = kKind == kCap && (range == kNear || !need_mask);
+                    if (kKind == kCapBias && range == kNear) {
+                        cap_row<kNear>(r, cap_out);
+                    } else if (!fused) {
+                        cap_row<kFar>(r, cap_out);
                     }
                     c = 1.0f;
                 }
@@ -987,13 +1028,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const bool right = __all_sync(0xffffffffu, kv0 >= pos);
                     bias_row(r, c, base, slope, pos - kv0, left, right);
                 }
-                Chunks chunks{0, 15};
                 if (need_mask) {
-                    chunks = chunks_of(lo - kv0, hi - kv0);
+                    if (kCapped) chunks = chunks_of(lo - kv0, hi - kv0);
                     mask_row(r, chunks, lo - kv0, hi - kv0);
                 }
                 const float r_max = attn::row_max128(r);
-                const float m_blk = kKind == kCap && fused ? cap_far(range == kNear ? 15.0f / 32.0f * r_max : r_max, cap_out) : fmaf(r_max, c, base);
+                const float m_blk = kKind == kCap && fused ? cap_one(r_max, cap_out) : fmaf(r_max, c, base);
                 // The point moves only when the max grows by more than 8, so P <= 2^(8 + kLift).
                 const float m_new = fmaxf(m_run, m_blk);
                 const float m_use = m_new > m_run + 8.0f ? m_new : m_run;
@@ -1035,9 +1075,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float e_sum;
                 if (kKind == kCap && fused) {
                     e_sum = range == kNear ? cap_exp_store<kBf16, kNear>(s_addr + C::kPOffset, r, cap_out, a, mid)
-                                           : cap_exp_store<kBf16, kMid>(s_addr + C::kPOffset, r, cap_out, a, mid);
+                                           : cap_exp_store<kBf16, kFar>(s_addr + C::kPOffset, r, cap_out, a, mid);
                 } else {
-                    constexpr bool kSkip = kDocs || kKind == kCap || kKind == kCapBias;
+                    constexpr bool kSkip = kDocs || kCapped;
                     e_sum = exp_store<kBf16, kSkip>(s_addr + C::kPOffset, r, c, base + a, chunks.live, mid);
                 }
                 if constexpr (!kEarly) rescale();
@@ -1155,7 +1195,9 @@ cudaError_t launch_kind(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
 template <int kDPad, bool kBf16>
 cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int device,
                    int grid, cudaStream_t stream) {
-    const bool bias = p.slopes != nullptr || (p.softcap == 0.0f && !(p.scale > 0.0f));
+    // kCap takes a row's reference point from cap_one, which is off by up to softcap * 2^-20: above this it
+    // would no longer bound the row's weights, and kCapBias takes it from the capped scores.
+    const bool bias = p.slopes != nullptr || (p.softcap == 0.0f && !(p.scale > 0.0f)) || p.softcap > 1e5f;
     if (p.softcap > 0.0f)
         return bias ? launch_kind<kDPad, kBf16, kCapBias>(mq, mk, mv, p, device, grid, stream)
                     : launch_kind<kDPad, kBf16, kCap>(mq, mk, mv, p, device, grid, stream);
