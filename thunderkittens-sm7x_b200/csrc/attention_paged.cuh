@@ -25,7 +25,7 @@
 //  - V: lane holds dims [D/8 g, D/8 (g + 1)) of tokens 2t, 2t + 1, 2t + 8, 2t + 9; byte
 //    pairs of two tokens are one register of V^T. Output dims are permuted alike.
 //  - P^T as B operand is the transpose of the S^T accumulator: one movmatrix per 8 x 8.
-// Bytes go through shared memory, a ring of kStages x 16 tokens for each warp alone
+// Bytes go through shared memory, a ring of kStages x 4 KB for each warp alone
 // (cp.async and __syncwarp, no CTA barrier): what HBM needs in flight, some 100 KB an SM,
 // does not fit the registers. The ring's 16-byte pieces are swizzled so that both the
 // K reads (rows g, pieces 2t) and the V reads (rows 2t, pieces g) hit distinct banks.
@@ -39,7 +39,7 @@
 // measured copy bandwidth); 3 of 30001 to 65536, capped scores, 88 us (92 %). With direct loads to
 // registers instead of the ring 137 us for the first. One request of 2048 tokens 6.8 us: a launch
 // and the latencies of lengths, pages, cache and the join. Heads of 64 have twice the tokens, so
-// twice the softmax, for the same bytes, and reach 42 % (ragged, 5 drafted tokens, slopes) to 67 %.
+// twice the softmax, for the same bytes, and reach 47 % (ragged, 5 drafted tokens, slopes) to 70 %.
 #pragma once
 
 #include <atomic>
@@ -61,7 +61,10 @@ template <int D>
 constexpr int kStep = 16 * kSub<D>;
 template <int D>
 constexpr int kStageBytes = kStep<D> * 2 * D;
-constexpr int kStages = 3;
+// Heads of 64 are bound by instructions, and the loop is unrolled over the stages: 376 requests of 572 to
+// 1143 tokens, 4 key heads of 64, 36 us with 2 stages, 39 with 3; 64 of up to 8192, 8 key heads, 63 and 70.
+template <int D>
+constexpr int kStages = D == 64 ? 2 : 3;
 constexpr int kMaxCluster = 8;
 constexpr long long kMostTokens = 1LL << 30;  // of a context: positions and steps stay far below 2^31
 // CTAs wanted where contexts are ragged, in rounds of 4 for each SM. 64 requests of 1 to 8192 tokens, 8
@@ -254,7 +257,7 @@ struct Smem {
     static constexpr int kCtaO = kMl + kWarps * kRows * 8;
     static constexpr int kCtaMl = kCtaO + kRows * D * 4;
     static constexpr int kAfter = kCtaMl + kRows * 8;
-    static constexpr int kRings = kWarps * kStages * kStageBytes<D>;
+    static constexpr int kRings = kWarps * kStages<D> * kStageBytes<D>;
     static constexpr int kBytes = kRings > kAfter ? kRings : kAfter;
 };
 
@@ -284,10 +287,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
     constexpr int kStride = kWarps * kStep<D>;
     const int begin = split * p.chunk;
     const int* table = p.table + static_cast<long long>(r) * p.width;
-    int page_of[kStages][kB];
+    int page_of[kStages<D>][kB];
     grid_wait();
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kStages<D>; ++i) {
 #pragma unroll
         for (int u = 0; u < kB; ++u) {
             const int col = (begin + (i * kWarps + warp) * kStep<D> + 16 * u) >> p.page_shift;
@@ -304,8 +307,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
     if (begin >= end && split > 0 && !p.cluster) return;
 
     // Warp w takes steps w, w + 4, ... of the chunk; kStages - 1 of them are in flight.
-    const uint32_t ring = smem_u32(smem) + warp * (kStages * kStageBytes<D>);
-    Block blocks[kStages][kB];
+    const uint32_t ring = smem_u32(smem) + warp * (kStages<D> * kStageBytes<D>);
+    Block blocks[kStages<D>][kB];
     int token = begin + warp * kStep<D>;
     int load_token = token;
     int next_page[kB];
@@ -320,9 +323,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
         load_token += kStride;
     };
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) load_pages(blocks[i], page_of[i], i);
+    for (int i = 0; i < kStages<D> - 1; ++i) load_pages(blocks[i], page_of[i], i);
 #pragma unroll
-    for (int u = 0; u < kB; ++u) next_page[u] = page_of[kStages - 1][u];
+    for (int u = 0; u < kB; ++u) next_page[u] = page_of[kStages<D> - 1][u];
 
     // Q as B operand: row g of each 8, dims [D/4 t, D/4 (t + 1)).
     uint32_t q[NT][2 * kM];
@@ -535,18 +538,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
 
     while (token < end) {
 #pragma unroll
-        for (int i = 0; i < kStages; ++i) {
+        for (int i = 0; i < kStages<D>; ++i) {
             if (token < end) {
-                cp_async_wait<kStages - 2>();
+                cp_async_wait<kStages<D> - 2>();
                 __syncwarp();  // every lane's copies of this step have landed, and the step before is read
-                constexpr int kAhead = kStages - 1;
+                constexpr int kAhead = kStages<D> - 1;
                 int pages[kB];
 #pragma unroll
                 for (int u = 0; u < kB; ++u) {
                     pages[u] = next_page[u];
                     next_page[u] = page_at(load_token + kStride + 16 * u);
                 }
-                load_pages(blocks[(i + kAhead) % kStages], pages, (i + kAhead) % kStages);
+                load_pages(blocks[(i + kAhead) % kStages<D>], pages, (i + kAhead) % kStages<D>);
                 compute(blocks[i], ring + i * kStageBytes<D>, token);
                 token += kStride;
             }
@@ -803,11 +806,14 @@ inline cudaError_t paged_entry(bool bf16, const void* q, long long q_stride, voi
         // hold its SMs until its longest chunk ends), each of at least 1024 tokens, or 64 KB of
         // cache where one request has to fill the GPU. 512 or 2048 tokens instead of 1024: 16
         // requests of 17 to 4096 tokens, 16 heads of 64, 32.4 or 33.6 us against 31.5; 32 of up to
-        // 1024, 8 heads of 128, 16.5 or 15.3 against 15.3.
+        // 1024, 8 heads of 128, 16.5 or 15.3 against 15.3. Chunks of less than that only where even
+        // their CTAs are all resident: 148 requests of 1143 tokens, 4 heads of 64, in one chunk each 17.6
+        // us, in two 20; 37 of them 11.0 and 9.2.
         const long long least = n_requests == 1 ? 32768 / dim : 1024;
         const long long rounds = n_requests < kRounds ? n_requests : kRounds;
         const long long want = rounds * 4LL * sm_count / items;
-        const long long most = (max_seq_len + least - 1) / least;
+        long long most = max_seq_len / least;
+        if (most <= 1) most = 2 * items <= 4LL * sm_count && max_seq_len > least ? 2 : 1;
         const long long splits = want < most ? want : most;
         cut(splits < 1 ? 1 : splits);
     }
