@@ -197,7 +197,7 @@ __device__ __forceinline__ int block_running(int v, int* warp_values, int& all) 
     return warp == (kMax ? 0 : 31) ? x : extreme<kMax>(x, outer);
 }
 
-__global__ void __launch_bounds__(kRunThreads) runs_kernel(const int* __restrict__ ids, int seq, int n_tiles, int causal,
+__global__ void __launch_bounds__(kRunThreads) runs_kernel(const int* ids, int seq, int n_tiles, int causal,
                                                            int2* rows, int4* tiles, int* next_item) {
     __shared__ int warp_values[32];
     grid_release();
@@ -316,14 +316,14 @@ __device__ __forceinline__ Item make_item(int w, const Params& p) {
         int lo = 0, hi = 0;
         if (g < it.tiles) {
             if (p.tiles != nullptr) {
-                const int4 t = __ldg(p.tiles + (static_cast<long long>(it.batch) * p.tile_stride + part * p.item_tiles + g));
+                const int4 t = p.tiles[static_cast<long long>(it.batch) * p.tile_stride + part * p.item_tiles + g];
                 lo = t.x;
                 hi = t.y;
             } else {
                 hi = p.seq_kv;
                 if (p.causal) {
                     hi = min(r0 + kBlockQ, p.seq_q) + (p.seq_kv - p.seq_q);
-                    if (p.prefix != nullptr) hi = max(hi, __ldg(p.prefix + it.batch));
+                    if (p.prefix != nullptr) hi = max(hi, p.prefix[it.batch]);
                     hi = min(max(hi, 0), p.seq_kv);
                 }
             }
@@ -920,14 +920,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         break;
                     }
                     // Documents have seq_kv = seq_q: key block j holds the rows of tile j.
-                    if (__ldg(p.tiles + (static_cast<long long>(it.batch) * p.tile_stride + j)).z != 0) {
+                    if (p.tiles[static_cast<long long>(it.batch) * p.tile_stride + j].z != 0) {
                         const uint32_t tile = base + C::kKvOffset + slot * C::kTileBytes;
 #pragma unroll
                         for (int i = 0; i < kBlockKV / 32; ++i) {
                             const int row = i * 32 + static_cast<int>(lane);
                             const int key = j * kBlockKV + row;
                             if (key >= p.seq_kv) continue;  // zero already
-                            const int2 r = __ldg(p.rows + (static_cast<long long>(it.batch) * p.seq_kv + key));
+                            const int2 r = p.rows[static_cast<long long>(it.batch) * p.seq_kv + key];
                             if (r.x < r.y) continue;
                             for (int x = 0; x < C::kBoxes; ++x)
 #pragma unroll
@@ -972,16 +972,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 lo = 0;
                 hi = p.seq_kv;
                 if constexpr (kDocs) {
-                    const int2 r = __ldg(p.rows + (static_cast<long long>(batch) * p.seq_q + q_row));
+                    const int2 r = p.rows[static_cast<long long>(batch) * p.seq_q + q_row];
                     lo = r.x;
                     hi = r.y;
                 } else if (p.causal) {
                     hi = pos + 1;
-                    if (p.prefix != nullptr) hi = min(max(hi, __ldg(p.prefix + batch)), p.seq_kv);
+                    if (p.prefix != nullptr) hi = min(max(hi, p.prefix[batch]), p.seq_kv);
                 }
             }
             float slope = 0.0f;
-            if ((kKind == kBias || kKind == kCapBias) && p.slopes != nullptr) slope = __ldg(p.slopes + head) * kLog2e;
+            if ((kKind == kBias || kKind == kCapBias) && p.slopes != nullptr) slope = p.slopes[head] * kLog2e;
             float m_run = -INFINITY;  // reference point, log2 units
             float l_run = 0.0f;       // running sum of 2^(x - m_run + kLift)
             for (int j = b0; j < b1; ++j) {

@@ -188,8 +188,8 @@ __device__ __forceinline__ void load_block(Block& bl, uint32_t stage, const Para
         for (int i = 0; i < 16 / kRows; ++i) cp_async_16(stage + piece_at<D, false>(r + i * kRows, c), k + i * 512);
 #pragma unroll
         for (int i = 0; i < 16 / kRows; ++i) cp_async_16(stage + 16 * D + piece_at<D, true>(r + i * kRows, c), v + i * 512);
-        bl.ks = __ldg(p.k_scale + tile);
-        bl.vs = __ldg(p.v_scale + tile);
+        bl.ks = p.k_scale[tile];
+        bl.vs = p.v_scale[tile];
     }
 }
 
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
 #pragma unroll
         for (int u = 0; u < kB; ++u) {
             const int col = (begin + (i * kWarps + warp) * kStep<D> + 16 * u) >> p.page_shift;
-            page_of[i][u] = col < p.width ? __ldg(table + col) : -1;
+            page_of[i][u] = col < p.width ? table[col] : -1;
         }
     }
     const Request rq = request_of(p, r);
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
     int token = begin + warp * kStep<D>;
     int load_token = token;
     int next_page[kB];
-    auto page_at = [&](int at) { return at < end ? __ldg(table + (at >> p.page_shift)) : -1; };
+    auto page_at = [&](int at) { return at < end ? table[at >> p.page_shift] : -1; };
     auto load_pages = [&](Block (&bl)[kB], const int (&pages)[kB], int stage) {
 #pragma unroll
         for (int u = 0; u < kB; ++u) {
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
         const uint16_t* at = p.q + (rq.first + row / p.group) * p.q_stride + (head * p.group + row % p.group) * D + t * (D / 4);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
-            const uint4 v = there ? __ldg(reinterpret_cast<const uint4*>(at) + i) : make_uint4(0, 0, 0, 0);
+            const uint4 v = there ? reinterpret_cast<const uint4*>(at)[i] : make_uint4(0, 0, 0, 0);
             q[nt][4 * i] = v.x;
             q[nt][4 * i + 1] = v.y;
             q[nt][4 * i + 2] = v.z;
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
             rows.factor[nt][c] = p.scale * own * (kChange ? 1.0f : kLog2e);
             rows.pos[nt][c] = in_tile < n_rows ? rq.len - rq.n + row / p.group : -1;
             rows.slope[nt][c] = kChange && p.slopes != nullptr && in_tile < n_rows
-                                    ? __ldg(p.slopes + head * p.group + row % p.group) * kLog2e : 0.0f;
+                                    ? p.slopes[head * p.group + row % p.group] * kLog2e : 0.0f;
             rows.m[nt][c] = -INFINITY;
             rows.off[nt][c] = 0.0f;
             rows.l[nt][c] = 0.0f;

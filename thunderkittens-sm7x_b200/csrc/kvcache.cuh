@@ -148,7 +148,7 @@ __device__ __forceinline__ void plan_fill(const PlanParams& p, const PlanPart& p
     for (long long k = pages + rank * kPlanThreads + tid; k < last_page; k += ctas * kPlanThreads) {
         const int i = upper_bound(part.upto, here, static_cast<int>(k));
         if (i < here && part.taken[i])
-            p.table[static_cast<long long>(r0 + i) * p.width + (k - part.base[i])] = __ldg(p.free_pages + (n_free - 1 - k));
+            p.table[static_cast<long long>(r0 + i) * p.width + (k - part.base[i])] = p.free_pages[n_free - 1 - k];
     }
     const long long last_token = min(tokens + sum, static_cast<long long>(p.max_tokens));
     const int warps = ctas * (kPlanThreads / 32);
@@ -173,7 +173,7 @@ __device__ __forceinline__ void plan_fill(const PlanParams& p, const PlanPart& p
             const int col = pow2 ? pos >> shift : pos / p.page;
             place[u] = pos - col * p.page;
             owner[u] = col < part.have[q] ? p.table[static_cast<long long>(r0 + q) * p.width + col]
-                                          : __ldg(p.free_pages + (n_free - 1 - (col + part.base[q])));
+                                          : p.free_pages[n_free - 1 - (col + part.base[q])];
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kAppendThreads, kCta ? 8 : 1) append_kernel(co
     // s_slots[1 + i]: slot of token t0 + i, -1 where there is no such token or place.
     for (int i = tid; i < 1 + count + p.page; i += kAppendThreads) {
         const long long t = static_cast<long long>(t0) + i - 1;
-        long long s = t >= 0 && t < p.n_tokens ? __ldg(p.slots + t) : -1;
+        long long s = t >= 0 && t < p.n_tokens ? p.slots[t] : -1;
         if (s < 0 || s >= n_slots) s = -1;
         s_slots[i] = s;
     }
@@ -514,11 +514,11 @@ __global__ void __launch_bounds__(kAppendThreads, kCta ? 8 : 1) append_kernel(co
                 const uint16_t* at = rows + (j0 + sub) * stride;
                 if (j0 + kRows * kHeld <= n) {
 #pragma unroll
-                    for (int u = 0; u < kHeld; ++u) held[u] = __ldg(reinterpret_cast<const uint4*>(at + u * step));
+                    for (int u = 0; u < kHeld; ++u) held[u] = *(reinterpret_cast<const uint4*>(at + u * step));
                 } else {
 #pragma unroll
                     for (int u = 0; u < kHeld; ++u)
-                        held[u] = j0 + u * kRows + sub < n ? __ldg(reinterpret_cast<const uint4*>(at + u * step)) : make_uint4(0, 0, 0, 0);
+                        held[u] = j0 + u * kRows + sub < n ? *(reinterpret_cast<const uint4*>(at + u * step)) : make_uint4(0, 0, 0, 0);
                 }
             };
             // Largest magnitudes of the even and the odd elements.
