@@ -35,7 +35,7 @@
 // distributed shared memory; more of them leave theirs in scratch, and a second kernel
 // joins those. Either way in chunk order: results do not depend on timing.
 //
-// Measured on B200: 64 requests of 1 to 8192 tokens, 32 heads on 8 of 128, 96 us = 5.98 TB/s (91 % of the
+// Measured on B200: 64 requests of 1 to 8192 tokens, 32 heads on 8 of 128, 96 us = 6.03 TB/s (92 % of the
 // measured copy bandwidth); 3 of 30001 to 65536, capped scores, 88 us (92 %). With direct loads to
 // registers instead of the ring 137 us for the first. One request of 2048 tokens 6.8 us: a launch
 // and the latencies of lengths, pages, cache and the join. Heads of 64 have twice the tokens, so

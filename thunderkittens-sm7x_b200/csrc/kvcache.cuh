@@ -203,7 +203,7 @@ __device__ __forceinline__ void plan_rest(const PlanParams& p, long long tokens,
 // outputs alone, so that no scratch is passed between the two.
 // What bounds both: the launches and the chain lengths -> sums -> entries; the bytes are a
 // few MB at most (8 a slot). 1024 requests with 385,000 tokens: 39 us when one cluster of
-// 8 CTAs did all of it (8 SMs wait for their page numbers), 12.4 us in two kernels, 8.6 in one.
+// 8 CTAs did all of it (8 SMs wait for their page numbers), 12.4 us in two kernels, 8.5 in one.
 template <bool kFill>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
     __shared__ PlanPart part;
@@ -441,8 +441,8 @@ __device__ __forceinline__ bool exact_reciprocal(float s) {
 // so the CTA looks at one slot before its chunk and a page's worth behind it.
 //
 // What bounds it: 2 bytes read and 1 written per element; at a few tokens, the chain
-// slots -> values -> scale -> bytes (64 tokens x 8 heads x 128: 3.1 us). 28,000 tokens of prompts x 8 x
-// 128, pages of 64: 35 us = 4.9 TB/s, 76 % of the measured copy bandwidth; each CTA waits for its slots
+// slots -> values -> scale -> bytes (64 tokens x 8 heads x 128: 2.9 us). 28,000 tokens of prompts x 8 x
+// 128, pages of 64: 34.4 us = 5.0 TB/s, 77 % of the measured copy bandwidth; each CTA waits for its slots
 // before its values, and 8 CTAs an SM (64 registers) cover most of that. A warp for each run
 // took 68 us there.
 template <int kDim, bool kBf16, bool kCta>
