@@ -804,9 +804,9 @@ inline cudaError_t paged_entry(bool bf16, const void* q, long long q_stride, voi
     } else {
         // Enough CTAs for several rounds of the GPU (contexts are ragged, and a cluster would
         // hold its SMs until its longest chunk ends), each of at least 1024 tokens, or 64 KB of
-        // cache where one request has to fill the GPU. 512 or 2048 tokens instead of 1024: 16
-        // requests of 17 to 4096 tokens, 16 heads of 64, 32.4 or 33.6 us against 31.5; 32 of up to
-        // 1024, 8 heads of 128, 16.5 or 15.3 against 15.3. Chunks of less than that only where even
+        // cache where one request has to fill the GPU. 512 or 1536 tokens instead of 1024, on heads of 64: 16
+        // requests of 17 to 4096 tokens, 16 heads, 25.9 or 25.1 us against 24.9, with 5 drafted tokens 28.1
+        // or 31.2 against 28.1; 376 of 572 to 1143, 4 heads, 46 or 36 against 36. Chunks of less than that only where even
         // their CTAs are all resident: 148 requests of 1143 tokens, 4 heads of 64, in one chunk each 17.6
         // us, in two 20; 37 of them 11.0 and 9.2.
         const long long least = n_requests == 1 ? 32768 / dim : 1024;
