@@ -641,15 +641,13 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     rest /= p.tiles;
     const int head = rest % p.heads_kv;
     const int r = rest / p.heads_kv;
+    grid_wait();
     const Request rq = request_of(p, r);
     const int n_rows = min(kRows, rq.n * p.group - tile * kRows);
     const int runs = p.join_runs;
     const int slot = static_cast<int>(threadIdx.x) / kQuads, quad = static_cast<int>(threadIdx.x) % kQuads;
     const int run = slot % runs, row = part * (kJoinThreads / kQuads / runs) + slot / runs;
-    if (part * (kJoinThreads / kQuads / runs) >= n_rows) {
-        grid_wait();  // also where there is nothing to do: this grid must not end before the one it follows
-        return;
-    }
+    if (part * (kJoinThreads / kQuads / runs) >= n_rows) return;
     const int kv_end = max(rq.len - rq.n + (tile * kRows + n_rows - 1) / p.group + 1, 0);
     const int used = max(min((kv_end + p.chunk - 1) / p.chunk, p.splits), 1);
     const long long item = item_of(p, r, head, tile, 0);
@@ -657,7 +655,6 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     const int last = row < n_rows ? min((run + 1) * each, used) : 0;
     const float2* ml_at = p.part_ml + item * kRows + row;
     const float* o_at = p.part_o + (item * kRows + row) * D + quad * 4;
-    grid_wait();
     Merged x;
     for (int s = run * each; s < last; s += 4) {
         float2 ml[4];

@@ -153,10 +153,10 @@ inline cudaError_t scratch_pool_bytes(int device, uint64_t* reserved, uint64_t* 
 }
 
 // Launches a kernel that begins with griddepcontrol.wait as a programmatic dependent of what is
-// before it on the stream: its launch then overlaps the end of that kernel. The wait comes before
-// the first access to global memory in every thread that makes one, so the order of the stream
-// holds as for any launch. Such a kernel makes no read-only loads (__ldg, const __restrict__): its
-// inputs may still be written when it starts.
+// before it on the stream: its launch then overlaps the end of that kernel. Every thread waits, before
+// its first access to global memory and before it may return, so the order of the stream holds as for
+// any launch, whatever the kernel before does ahead of its own wait. Such a kernel makes no read-only
+// loads (__ldg, const __restrict__): its inputs may still be written when it starts.
 template <class... P, class... A>
 cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, A... args) {
     cudaLaunchConfig_t cfg{};
