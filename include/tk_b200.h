@@ -251,7 +251,8 @@ TK_API cudaError_t tk_attention_forward_gqa_f16(const void* q, const void* k, co
  * Operands whose base or strides are not multiples of 16 bytes are first copied into
  * stream-ordered scratch, which the documents' row intervals (8 bytes a row) and the
  * work counter come from too. Except for padding, V must be finite: a masked key in a
- * block of 128 that other rows see is multiplied by 0. */
+ * block of 128 that other rows see is multiplied by 0. A pointer that is not aligned to
+ * its elements is refused. */
 TK_API cudaError_t tk_attention_masked_f16(const void* q, const void* k, const void* v, void* out,
                                            const int64_t* strides, int batch, int heads_q,
                                            int heads_kv, int seq_q, int seq_kv, int head_dim,
@@ -270,7 +271,8 @@ TK_API cudaError_t tk_attention_masked_bf16(const void* q, const void* k, const 
  * [n_pages, heads_kv, page_size, head_dim] e4m3 bytes, k_scale and v_scale
  * [n_pages, heads_kv] FP32: a byte stands for scale * e4m3. Slot s is place
  * s % page_size of page s / page_size. A request's tokens lie, in order, in the
- * pages of its row of the block table (int32 [n_requests, max_pages]). */
+ * pages of its row of the block table (int32 [n_requests, max_pages]). Pointers that are
+ * not aligned to their elements are refused. */
 
 /* Places for the new tokens of a step, from request lengths, on the GPU. Request r
  * holds cached_lens[r] tokens and adds new_lens[r] (negative values count as 0).

@@ -1,0 +1,34 @@
+"""More refusals of the prompt and serving operators, on the CPU: no GPU is touched by a call that is refused."""
+
+import pytest
+import torch
+
+from test_serving_cpu import INVALID, MB, append, masked, paged, plan
+
+# Pointers off their element's alignment: a kernel would fault on them.
+MISALIGNED = (
+    [(masked, {k: n * MB + 1}) for k, n in (("q", 1), ("k", 2), ("v", 3), ("out", 4))]
+    + [(masked, over) for over in (dict(slopes=5 * MB + 2), dict(ids=5 * MB + 1), dict(prefix=5 * MB + 2))]
+    + [(plan, {k: n * MB + off}) for k, n in (("cached", 1), ("new", 2), ("table", 3), ("free", 4), ("n_free", 5), ("lens", 6), ("seq", 7),
+                                             ("starts", 8), ("left", 10)) for off in (1, 2)]
+    + [(plan, dict(slots=9 * MB + 4))]
+    + [(append, dict(ksc=6 * MB + 1)), (append, dict(vsc=7 * MB + 2)), (append, dict(slots=3 * MB + 4))]
+    + [(paged, {k: n * MB + 2}) for k, n in (("ksc", 5), ("vsc", 6), ("table", 7), ("lens", 8), ("starts", 9), ("slopes", 10))]
+)
+
+
+@pytest.mark.parametrize("call,over", MISALIGNED, ids=[f"{c.__name__}-{k}+{v % MB}" for c, o in MISALIGNED for k, v in o.items()])
+def test_misaligned_pointers(call, over):
+    assert call(**over) == INVALID
+
+
+def test_aligned_pointers_are_not_refused():
+    """The same calls with the pointers on their element's alignment, and no more."""
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is present")
+    good = [masked(q=MB + 2, k=2 * MB + 2, v=3 * MB + 2, out=4 * MB + 2, slopes=5 * MB + 4), masked(ids=5 * MB + 4), masked(prefix=5 * MB + 4),
+            plan(cached=MB + 4, new=2 * MB + 4, table=3 * MB + 4, free=4 * MB + 4, n_free=5 * MB + 4, lens=6 * MB + 4, seq=7 * MB + 4,
+                 starts=8 * MB + 4, slots=9 * MB + 8, left=10 * MB + 4),
+            append(ksc=6 * MB + 4, vsc=7 * MB + 4, slots=3 * MB + 8),
+            paged(ksc=5 * MB + 4, vsc=6 * MB + 4, table=7 * MB + 4, lens=8 * MB + 4, starts=9 * MB + 4, slopes=10 * MB + 4)]
+    assert INVALID not in good

@@ -1263,6 +1263,10 @@ inline cudaError_t masked_entry(bool bf16, const void* q, const void* k, const v
         (doc_ids != nullptr && (prefix != nullptr || seq_q != seq_kv || batch > 65535)) || (prefix != nullptr && causal == 0)) {
         return cudaErrorInvalidValue;
     }
+    if (host::misaligned(q, 2) || host::misaligned(k, 2) || host::misaligned(v, 2) || host::misaligned(out, 2) || host::misaligned(slopes, 4) ||
+        host::misaligned(doc_ids, 4) || host::misaligned(prefix, 4)) {
+        return cudaErrorInvalidValue;
+    }
     const long long bh = static_cast<long long>(batch) * heads;
     const int pairs = static_cast<int>((seq_q + 255LL) / 256);
     // Positions and the last tile's ends stay below 2^31.

@@ -729,9 +729,9 @@ inline cudaError_t paged_entry(bool bf16, const void* q, long long q_stride, voi
         return cudaErrorInvalidValue;
     }
     const long long row = static_cast<long long>(heads_q) * dim;
-    auto off = [](const void* x, uintptr_t a) { return (reinterpret_cast<uintptr_t>(x) & (a - 1)) != 0; };
-    if (q_stride < row || out_stride < row || q_stride % 8 != 0 || out_stride % 8 != 0 || off(q, 16) || off(out, 16) ||
-        off(k_cache, 32) || off(v_cache, 32) ||
+    if (q_stride < row || out_stride < row || q_stride % 8 != 0 || out_stride % 8 != 0 || host::misaligned(q, 16) || host::misaligned(out, 16) ||
+        host::misaligned(k_cache, 32) || host::misaligned(v_cache, 32) || host::misaligned(k_scale, 4) || host::misaligned(v_scale, 4) ||
+        host::misaligned(table, 4) || host::misaligned(seq_lens, 4) || host::misaligned(starts, 4) || host::misaligned(slopes, 4) ||
         (n_tokens > 0 && (q_stride > LLONG_MAX / 4 / n_tokens || out_stride > LLONG_MAX / 4 / n_tokens)))
         return cudaErrorInvalidValue;
     const size_t tokens = n_tokens > 0 ? static_cast<size_t>(n_tokens - 1) : 0;

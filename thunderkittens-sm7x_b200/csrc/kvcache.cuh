@@ -325,6 +325,11 @@ inline cudaError_t plan_entry(const int* cached, const int* fresh, int n_request
         (slots == nullptr && max_tokens > 0)) {
         return cudaErrorInvalidValue;
     }
+    for (const void* p : {static_cast<const void*>(cached), static_cast<const void*>(fresh), static_cast<const void*>(table),
+                          static_cast<const void*>(free_pages), static_cast<const void*>(n_free), static_cast<const void*>(lens_out),
+                          static_cast<const void*>(seq_lens), static_cast<const void*>(starts), static_cast<const void*>(n_free_out)})
+        if (host::misaligned(p, 4)) return cudaErrorInvalidValue;
+    if (host::misaligned(slots, 8)) return cudaErrorInvalidValue;
     const size_t bytes = static_cast<size_t>(n_requests) * 4;
     const size_t table_bytes = bytes * static_cast<size_t>(width);
     struct Range { const void* p; size_t n; };
@@ -609,9 +614,9 @@ inline cudaError_t append_entry(bool bf16, const void* k, const void* v, long lo
         return cudaErrorInvalidValue;
     }
     const long long row = static_cast<long long>(heads) * dim;
-    auto off = [](const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; };
-    if (k_stride < row || v_stride < row || k_stride % 8 != 0 || v_stride % 8 != 0 || off(k, 16) || off(v, 16) ||
-        off(k_cache, 16) || off(v_cache, 16) || off(k_scale, 4) || off(v_scale, 4) || off(slots, 8) ||
+    if (k_stride < row || v_stride < row || k_stride % 8 != 0 || v_stride % 8 != 0 || host::misaligned(k, 16) ||
+        host::misaligned(v, 16) || host::misaligned(k_cache, 16) || host::misaligned(v_cache, 16) || host::misaligned(k_scale, 4) ||
+        host::misaligned(v_scale, 4) || host::misaligned(slots, 8) ||
         n_pages > LLONG_MAX / page / row || (n_tokens > 0 && (k_stride > LLONG_MAX / 2 / n_tokens || v_stride > LLONG_MAX / 2 / n_tokens))) {
         return cudaErrorInvalidValue;
     }

@@ -180,6 +180,9 @@ inline bool scores_ok(float scale, float softcap) {
     return scale_ok && (softcap == 0.0f || (softcap >= 1e-6f && softcap <= 1e30f));
 }
 
+// Whether p is off a multiple of `a` (a power of two); null is not.
+inline bool misaligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+
 inline bool ranges_overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
     const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
     return a0 < b0 + b_bytes && b0 < a0 + a_bytes;
