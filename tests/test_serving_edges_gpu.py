@@ -1,0 +1,132 @@
+"""Calls that the documentation of the prompt and serving operators allows and that ordinary sizes and
+values do not make, against 64 bits."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import plain64
+import tk_b200
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def ints(x, kind=torch.int32):
+    return torch.tensor(np.asarray(x), dtype=kind, device="cuda")
+
+
+def rows_of(q, k, v, allowed, *, scale, cap, half_p, half_out, far=None, slope=0.0):
+    """(out, bound) of one head as plain64.attend gives them, but with the error of a capped score following
+    the score: tanh is a contraction, so the raw score's error stays as it is, and the capped one is off
+    by 2^-20 of itself at most (argument, polynomial or exponential and reciprocal, product)."""
+    d, m = q.shape[1], k.shape[0]
+    x = q @ k.T * scale
+    off = (d + 8) * 2.0 ** -23 * (np.abs(q) @ np.abs(k).T * abs(scale))
+    if cap:
+        x = cap * np.tanh(x / cap)
+        off = off + np.abs(x) * 2.0 ** -20
+    if slope:
+        x = x - slope * far
+        off = off + slope * far * 2.0 ** -22
+    off = off + np.abs(x) * 2.0 ** -22 + 2.0 ** -21  # to log2 units, minus the reference point, 2^x
+    x = np.where(allowed, x, -np.inf)
+    some = allowed.any(1)
+    top = np.where(some, x.max(1, initial=-np.inf), 0.0)
+    w = np.where(allowed, np.exp(np.where(allowed, x - top[:, None], 0.0)), 0.0)
+    p = w / np.where(some, w.sum(1), 1.0)[:, None]
+    out = p @ v
+    worst = np.where(allowed & (p > 1e-12), off, 0.0).max(1, initial=0.0)
+    rel = 2.2 * worst + half_p + (m + 64) * 2.0 ** -23
+    bound = p @ np.abs(v) * rel[:, None] + np.abs(v).sum(0)[None] * 2.0 ** -32
+    return out, bound + half_out * (np.abs(out) + bound) + 2.0 ** -25
+
+
+class Paged:
+    """Requests over a cache with given K and V values (held exactly), in pages of random order."""
+
+    def __init__(self, lens, heads, kv_heads, page, dim, seed=0, v_scales=None, width=None):
+        g = np.random.default_rng(seed)
+        self.lens, self.heads, self.kv_heads, self.page, self.dim = lens, heads, kv_heads, page, dim
+        counts = [-(-n // page) for n in lens]
+        pages = sum(counts) + 2
+        order = g.permutation(pages).astype(np.int32)
+        self.table = np.full((len(lens), width or max(counts + [1])), -1, np.int32)
+        at = 0
+        for r, c in enumerate(counts):
+            self.table[r, :c] = order[at:at + c]
+            at += c
+        gen = torch.Generator().manual_seed(seed)
+        self.k, self.v = (torch.randn(pages, kv_heads, page, dim, generator=gen).to(torch.float8_e4m3fn) for _ in range(2))
+        self.k_scale = torch.ones(pages, kv_heads)
+        self.v_scale = torch.ones(pages, kv_heads) if v_scales is None else v_scales(g, pages, kv_heads, self.table)
+
+    def values(self, r, h):
+        """float64 K and V of request r for query head h."""
+        key = np.arange(self.lens[r])
+        own, g = self.table[r, key // self.page], h * self.kv_heads // self.heads
+        return tuple(c.float().double().numpy()[own, g, key % self.page] * s.double().numpy()[own, g][:, None]
+                     for c, s in ((self.k, self.k_scale), (self.v, self.v_scale)))
+
+    def call(self, q, news, *, scale, cap=0.0, slopes=None, most=None, hint=None, out=None):
+        starts = np.concatenate([[0], np.cumsum(news)])
+        return tk_b200.attention_paged(q, self.k.cuda(), self.v.cuda(), self.k_scale.cuda(), self.v_scale.cuda(), ints(self.table),
+                                       ints(self.lens), ints(starts), scale=scale, softcap=cap, alibi_slopes=slopes,
+                                       max_query_len=max(news) if most is None else most, max_seq_len=hint, out=out)
+
+    def held(self, q, news, out, *, scale, cap=0.0, keys=None, rows=None):
+        """Each row within its bound; only `keys` of a request, if given, may carry weight; only the first `rows`."""
+        o64, q64 = out.cpu().double().numpy(), q.cpu().double().numpy()
+        first = 0
+        for r, n in enumerate(news):
+            pos = np.arange(self.lens[r] - n, self.lens[r])[:rows]
+            key = np.arange(self.lens[r])
+            allowed = key[None] <= pos[:, None]
+            at = slice(first, first + len(pos))
+            first += n
+            for h in range(self.heads):
+                k, v = self.values(r, h)
+                pick = np.ones(len(key), bool) if keys is None else keys(r)
+                want, bound = rows_of(q64[at, h], k[pick], v[pick], allowed[:, pick], scale=scale, cap=cap, half_p=2.0 ** -11,
+                                      half_out=plain64.HALF[q.dtype])
+                err = np.abs(o64[at, h] - want)
+                assert np.all(err <= bound), (r, h, float((err / bound).max()))
+
+
+def queries(n, heads, dim, kind, seed, spread=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(n, heads, dim, generator=gen) * spread).to(kind)
+
+
+# ---- caps of any size over the cache -----------------------------------------------------------
+
+@pytest.mark.parametrize("kind", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("cap", [1e-5, 0.7, 30.0, 1e3, 1e4, 1e6, 1e7, 1e9, 1e25, 1e30])
+def test_paged_softcap_of_any_size(cap, dim, kind):
+    """A cap far above the scores changes nothing, one far below them leaves their signs; the last head's
+    scores are large beside the others', in the same tile of rows."""
+    c = Paged([1, 70, 1300], 4, 1, 16, dim, seed=1)
+    q = queries(4, 4, dim, kind, 2, 4.0)
+    q[:, 3] *= min(cap, 4000.0)
+    q = q.cuda()
+    for hint in (70, 1300, 100000):
+        out = c.call(q, [1, 2, 1], scale=0.09, cap=cap, hint=hint)
+        c.held(q, [1, 2, 1], out, scale=0.09, cap=cap)
+
+
+@pytest.mark.parametrize("cap", [1e7, 1e30])
+def test_paged_softcap_with_slopes(cap):
+    """As without a cap, slopes applied."""
+    slopes = torch.tensor([0.5, 0.25], device="cuda")
+    c = Paged([300], 2, 1, 32, 128, seed=3)
+    q = queries(1, 2, 128, F16, 4, 4.0).cuda()
+    out = c.call(q, [1], scale=0.09, cap=cap, slopes=slopes).cpu().double().numpy()
+    far = 299.0 - np.arange(300)[None]
+    for h in range(2):
+        k, v = c.values(0, h)
+        want, bound = rows_of(q[:, h].cpu().double().numpy(), k, v, np.ones((1, 300), bool), scale=0.09, cap=cap, half_p=2.0 ** -11,
+                              half_out=2.0 ** -11, far=far, slope=float(slopes[h]))
+        assert np.all(np.abs(out[:, h] - want) <= bound)
