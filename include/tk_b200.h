@@ -329,7 +329,8 @@ TK_API cudaError_t tk_kv_append_e4m3_bf16(const void* k, const void* v, int64_t 
  * and out has q's type. A row without a key (seq_lens[r] = 0, or all its pages outside
  * [0, n_pages)) is 0; tokens of pages outside that range are as if they were not there;
  * tokens behind starts[n_requests] are left as they were. Bytes behind a request's
- * last token may hold anything.
+ * last token may hold anything. A row that sees a NaN score is NaN. V of a request's tokens
+ * must be finite: a later new token is multiplied by 0 for the earlier ones of its tile.
  * max_query_len: at least the largest number of query tokens of a request (rows past it
  * are left as they were). max_seq_len only sets how the work is split and should be near
  * the largest seq_lens; results are right for any. head_dim 64 or 128; page_size 16, 32,

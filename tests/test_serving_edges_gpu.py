@@ -130,3 +130,63 @@ def test_paged_softcap_with_slopes(cap):
         want, bound = rows_of(q[:, h].cpu().double().numpy(), k, v, np.ones((1, 300), bool), scale=0.09, cap=cap, half_p=2.0 ** -11,
                               half_out=2.0 ** -11, far=far, slope=float(slopes[h]))
         assert np.all(np.abs(out[:, h] - want) <= bound)
+
+
+# ---- NaN over the cache ------------------------------------------------------------------------
+
+SPLITS = [1, 700, 9001, 100000]  # one chunk, a cluster, scratch: what max_seq_len makes of the same context
+
+
+@pytest.mark.parametrize("kind", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("hint", SPLITS)
+def test_paged_nan_query(hint, cap, dim, kind):
+    """A query row with a NaN is NaN, in the rows beside it nothing changes; a row that sees no key is 0 all the same."""
+    c = Paged([17, 2500, 1], 4, 2, 16, dim, seed=5, width=700)
+    q = queries(4, 4, dim, kind, 6)
+    bad = q.clone()
+    bad[0, 1, 5] = float("nan")
+    bad[2, 0] = float("nan")  # one of two queries of the second request
+    bad[3, 3, 0] = float("nan")
+    out = c.call(bad.cuda(), [1, 2, 1], scale=0.1, cap=cap, hint=hint)
+    hit = bad.isnan().any(-1).cuda()
+    assert out[hit].isnan().all()
+    clean = torch.where(hit[..., None], 0.0, out)
+    fine = torch.where(hit.cpu()[..., None], 0.0, q)
+    o64 = clean.cpu().double().numpy()
+    assert np.isfinite(o64).all()
+    first = 0
+    for r, n in enumerate([1, 2, 1]):
+        pos = np.arange(c.lens[r] - n, c.lens[r])
+        for h in range(4):
+            k, v = c.values(r, h)
+            want, bound = rows_of(fine[first:first + n, h].double().numpy(), k, v, np.arange(c.lens[r])[None] <= pos[:, None], scale=0.1,
+                                  cap=cap, half_p=2.0 ** -11, half_out=plain64.HALF[kind])
+            ok = ~hit[first:first + n, h].cpu().numpy()
+            assert np.all(np.abs(o64[first:first + n, h] - want)[ok] <= bound[ok]), (r, h)
+        first += n
+    c.lens = [0, 2500, 0]  # two requests without a token, their queries NaN or not
+    out = c.call(bad.cuda(), [1, 2, 1], scale=0.1, cap=cap, hint=hint)
+    assert torch.count_nonzero(out[[0, 3]]) == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("hint", SPLITS)
+@pytest.mark.parametrize("length,key", [(1, 0), (17, 16), (17, 3), (65, 64), (2500, 0), (2500, 1040), (2500, 2499), (2500, 2498)])
+def test_paged_nan_key(length, key, hint, cap, dim):
+    """A NaN K token: rows that see it are NaN wherever it stands; an earlier one of the new tokens is as without it."""
+    c = Paged([length], 4, 2, 16, dim, seed=7, width=700)
+    n = min(length, 2)
+    q = queries(n, 4, dim, F16, 8).cuda()
+    where = int(c.table[0, key // 16]), key % 16
+    fine = c.k.clone()
+    c.k.view(torch.uint8)[where[0], 0, where[1], 9] = 0x7f  # for query heads 0 and 1
+    out = c.call(q, [n], scale=0.1, cap=cap, hint=hint)
+    c.k = fine
+    sees = torch.arange(length - n, length) >= key
+    assert out[sees.cuda()][:, :2].isnan().all()
+    clean = out.clone()
+    clean[sees.cuda(), :2] = c.call(q, [n], scale=0.1, cap=cap, hint=hint)[sees.cuda(), :2]
+    c.held(q, [n], clean, scale=0.1, cap=cap)

@@ -228,12 +228,13 @@ __device__ __forceinline__ uint16_t out_bits(float x) {
     }
 }
 
-// (point, sum, O) of a row, merged one by one in a fixed order.
+// (point, sum, O) of a row, merged one by one in a fixed order. A part without a point has met no key, or
+// NaN scores alone, which no max finds: then its sum is NaN, and the row's becomes so.
 struct Merged {
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     __device__ __forceinline__ void add(float2 ml, float4 v) {
-        if (ml.x == -INFINITY) return;
+        if (ml.x == -INFINITY && ml.y == 0.0f) return;
         const float now = fmaxf(m, ml.x);
         const float a = ex2(m - now), b = ex2(ml.x - now);  // 0 for the first: m is -inf
         m = now;
@@ -247,7 +248,7 @@ struct Merged {
 
 template <int D, bool kBf16>
 __device__ __forceinline__ void write_out(const Params& p, const Request& rq, int head, int row, int col, const Merged& x) {
-    const float inv = x.l > 0.0f ? __frcp_rn(x.l) : 0.0f;  // a row without a key is 0
+    const float inv = x.l == 0.0f ? 0.0f : __frcp_rn(x.l);  // a row without a key is 0
     uint16_t* dst = p.out + (rq.first + row / p.group) * p.out_stride + (head * p.group + row % p.group) * D + col;
     uint2 w;
     w.x = out_bits<kBf16>(x.o.x * inv) | static_cast<uint32_t>(out_bits<kBf16>(x.o.y * inv)) << 16;
