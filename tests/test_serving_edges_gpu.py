@@ -190,3 +190,25 @@ def test_paged_nan_key(length, key, hint, cap, dim):
     clean = out.clone()
     clean[sees.cuda(), :2] = c.call(q, [n], scale=0.1, cap=cap, hint=hint)[sees.cuda(), :2]
     c.held(q, [n], clean, scale=0.1, cap=cap)
+
+
+# ---- rows past max_query_len ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (3, 1), (12, 2), (7, 1)])
+@pytest.mark.parametrize("hint", [1, 700, 9001, 100000])
+@pytest.mark.parametrize("most", [0, 1, 2, 3])
+def test_paged_rows_past_the_most(most, hint, heads, kv_heads, kind):
+    """Query tokens past max_query_len are left as they were; those before it stand where they stand."""
+    news = [1, 5, 3, 4]
+    c = Paged([40, 2600, 3, 900], heads, kv_heads, 16, 64, seed=9, width=700)
+    q = queries(sum(news), heads, 64, kind, 10).cuda()
+    out = torch.full_like(q, 7.0)
+    c.call(q, news, scale=0.125, most=most, hint=hint, out=out)
+    whole = c.call(q, news, scale=0.125, hint=hint)
+    first = 0
+    for n in news:
+        assert torch.all(out[first + min(n, most):first + n] == 7.0)
+        whole[first:first + min(n, most)] = out[first:first + min(n, most)]
+        first += n
+    c.held(q, news, whole, scale=0.125)

@@ -96,6 +96,7 @@ struct Params {
     const int* seq_lens;
     const int* starts;
     int n_requests, heads_q, heads_kv, group;
+    int rows;           // most rows of a (request, key head): max_query_len * group
     int tiles;          // row tiles per (request, key head)
     int splits, chunk;  // chunks per (request, key head, tile), and tokens in each (the last takes the rest)
     float scale, softcap;
@@ -118,6 +119,12 @@ __device__ __forceinline__ Request request_of(const Params& p, int r) {
     q.first = a;
     q.n = max(b - a, 0);
     return q;
+}
+
+// Rows of a tile; those past max_query_len are left out.
+template <int kRows>
+__device__ __forceinline__ int rows_of(const Params& p, const Request& rq, int tile) {
+    return min(kRows, min(rq.n * p.group, p.rows) - tile * kRows);
 }
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -307,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
         }
     }
     const Request rq = request_of(p, r);
-    const int n_rows = min(kRows, rq.n * p.group - tile * kRows);  // of this tile
+    const int n_rows = rows_of<kRows>(p, rq, tile);
     if (n_rows <= 0) return;
     // Keys up to the last row's position.
     const int last_pos = rq.len - rq.n + (tile * kRows + n_rows - 1) / p.group;
@@ -652,7 +659,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     const int r = rest / p.heads_kv;
     grid_wait();
     const Request rq = request_of(p, r);
-    const int n_rows = min(kRows, rq.n * p.group - tile * kRows);
+    const int n_rows = rows_of<kRows>(p, rq, tile);
     const int runs = p.join_runs;
     const int slot = static_cast<int>(threadIdx.x) / kQuads, quad = static_cast<int>(threadIdx.x) % kQuads;
     const int run = slot % runs, row = part * (kJoinThreads / kQuads / runs) + slot / runs;
@@ -790,6 +797,7 @@ inline cudaError_t paged_entry(bool bf16, const void* q, long long q_stride, voi
     p.heads_q = heads_q;
     p.heads_kv = heads_kv;
     p.group = group;
+    p.rows = static_cast<int>(rows);
     p.tiles = static_cast<int>(tiles);
     p.scale = scale;
     p.softcap = softcap;
