@@ -325,8 +325,10 @@ TK_API cudaError_t tk_kv_append_e4m3_bf16(const void* k, const void* v, int64_t 
  * elements, q_stride and out_stride elements apart; tokens starts[r] .. starts[r + 1]
  * are the last positions of request r, whose cache holds seq_lens[r] tokens. Query at
  * position pos sees positions 0 .. pos. Scores as for tk_attention_masked (scale,
- * softcap, alibi_slopes); the softmax is FP32, probabilities are rounded to binary16,
- * and out has q's type. A row without a key (seq_lens[r] = 0, or all its pages outside
+ * softcap, alibi_slopes); the softmax is FP32, probabilities are rounded to binary16
+ * (those below 2^-13 of a row's largest to 2^-24 of it), and out has q's type. Scales are
+ * factors of either sign, up to 2^126; bits are lost of pages whose V scale is more than
+ * 2^68 below the largest one of their context. A row without a key (seq_lens[r] = 0, or all its pages outside
  * [0, n_pages)) is 0; tokens of pages outside that range are as if they were not there;
  * tokens behind starts[n_requests] are left as they were. Bytes behind a request's
  * last token may hold anything. A row that sees a NaN score is NaN. V of a request's tokens

@@ -212,3 +212,69 @@ def test_paged_rows_past_the_most(most, hint, heads, kv_heads, kind):
         whole[first:first + min(n, most)] = out[first:first + min(n, most)]
         first += n
     c.held(q, news, whole, scale=0.125)
+
+
+# ---- scales of V -----------------------------------------------------------------------------------
+
+def two_scales(ratio, negative=False):
+    def make(g, pages, kv_heads, table):
+        s = torch.from_numpy(2.0 ** g.uniform(-1, 1, (pages, kv_heads))).float()
+        for row in table:
+            s[torch.from_numpy(row[::2][row[::2] >= 0].astype(np.int64))] *= ratio
+        if negative:
+            s = s * torch.from_numpy(g.choice([-1.0, 1.0], (pages, kv_heads))).float()
+        return s
+    return make
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("ratio", [2.0 ** 12, 2.0 ** 24, 2.0 ** 40, 2.0 ** 55, 2.0 ** -40])
+@pytest.mark.parametrize("hint", [1, 700, 9001, 100000])
+def test_paged_small_scales_with_all_the_weight(hint, ratio, page, dim):
+    """Pages of large and small V scales in turn, and the weight on the small ones: the scores of the others
+    are 60 and more below. What those add is below 2^-86 * 2^55 of a small page's values, nothing in bfloat16."""
+    lens = [page * 2, 100, 3000]
+    c = Paged(lens, 4, 2, page, dim, seed=11, v_scales=two_scales(ratio))
+    small = 0 if ratio < 1 else 1  # which pages of two in turn
+    ramp = torch.linspace(1.0, 2.0, dim)
+    for r, row in enumerate(c.table):
+        for col, own in enumerate(row[:-(-lens[r] // page)]):
+            noise = 1 + 0.125 * torch.rand(c.kv_heads, page, dim, generator=torch.Generator().manual_seed(int(own)))
+            c.k[int(own)] = ((1.0 if col % 2 == small else -1.0) * noise * ramp).to(torch.float8_e4m3fn)
+    q = (ramp * (1 + 0.1 * torch.rand(3, 4, dim, generator=torch.Generator().manual_seed(12)))).to(BF16).cuda()
+    # q.k is 7/3 dim at least (the mean square of the ramp); 30 on each side of 0.
+    scale = 30.0 / (7 / 3 * dim)
+    out = c.call(q, [1, 1, 1], scale=scale, hint=hint)
+    c.held(q, [1, 1, 1], out, scale=scale, keys=lambda r: np.arange(lens[r]) // page % 2 == small)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("ratio", [1.0, 2.0 ** 9])
+@pytest.mark.parametrize("kind", [F16, BF16], ids=["f16", "bf16"])
+def test_paged_negative_scales(kind, ratio, dim):
+    """A scale is a factor like another: pages of negative ones among the others, and alone."""
+    c = Paged([5, 90, 1400], 4, 2, 16, dim, seed=13, v_scales=two_scales(ratio, negative=True))
+    c.k_scale = c.k_scale * torch.from_numpy(np.random.default_rng(14).choice([-1.0, 1.0], tuple(c.k_scale.shape))).float()
+    q = queries(3, 4, dim, kind, 15).cuda()
+    for hint in (1, 1400, 50000):
+        c.held(q, [1, 1, 1], c.call(q, [1, 1, 1], scale=0.1, hint=hint), scale=0.1)
+    c.v_scale = -c.v_scale.abs()
+    c.held(q, [1, 1, 1], c.call(q, [1, 1, 1], scale=0.1), scale=0.1)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("zero", [0.0, 2.0 ** -100])
+def test_paged_pages_of_zeros(zero, dim):
+    """Pages whose V are zeros carry the append's least scale (or 0): among others, first, last, and alone."""
+    c = Paged([16, 64, 900], 4, 2, 16, dim, seed=16)
+    for row in c.table:
+        for own in row[::3]:
+            if own >= 0:
+                c.v.view(torch.uint8)[int(own)] = 0
+                c.v_scale[int(own)] = zero
+    q = queries(3, 4, dim, F16, 17).cuda()
+    for hint in (1, 900, 50000):
+        out = c.call(q, [1, 1, 1], scale=0.1, hint=hint)
+        assert torch.count_nonzero(out[0]) == 0
+        c.held(q, [1, 1, 1], out, scale=0.1)

@@ -174,6 +174,9 @@ __device__ __forceinline__ float tanh_of(float x) {
     return fabsf(x) < 0.625f ? q * x : far;
 }
 
+// 1 / x of a power of two from 2^-126 to 2^126; 2^127 of 0.
+__device__ __forceinline__ float inverse_of(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+
 // 16 tokens of one key head in a warp's ring: K, then V, 16 D bytes each, in lines of 128
 // bytes (a token, or two of head_dim 64). Piece c of token r stands at piece_at.
 template <int D, bool kV>
@@ -409,9 +412,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
         for (int i = 0; i < kM; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) o[nt][i][c] = 0.0f;
-    // O is held in units of v_unit, a power of two not below any page scale met so far,
-    // so that probabilities times page scale / unit stay in binary16's range.
-    float v_unit = 0.0f, v_over = 0.0f;
+    // O is held in units of v_unit, a power of two, so that probabilities times page scale / unit stay in
+    // binary16's range: not below the page's scale, and at most 2^8 above it, so that they keep their 11 bits
+    // down to 2^-13 of the largest weight wherever that lies. Pages more than 2^60 below the largest scale met
+    // are left at that (v_floor): O may be that much larger than what it is made of, and stays in FP32's range.
+    float v_unit = 0.0f, v_floor = 0.0f;
 
     auto compute = [&](const Block (&bl)[kB], uint32_t stage, int token) {
         float s[kB][NT][4];
@@ -442,7 +447,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
 #pragma unroll
         for (int u = 0; u < kB; ++u) partial = partial || !bl[u].on;
         bool grow = false;
-        float unit = v_unit;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float top[2] = {-INFINITY, -INFINITY};
@@ -491,24 +495,24 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) paged_kernel(const 
             }
         }
 #pragma unroll
-        for (int u = 0; u < kB; ++u)
-            if (bl[u].on && bl[u].vs > unit)  // the next power of two
-                unit = __uint_as_float((__float_as_uint(bl[u].vs) + 0x7fffffu) & 0xff800000u);
-        if (unit > v_unit) {
-            const float alpha = v_unit > 0.0f ? __fdiv_rn(v_unit, unit) : 1.0f;
-            v_unit = unit;
-            v_over = __fdiv_rn(1.0f, unit);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < kM; ++i)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) o[nt][i][c] *= alpha;
-        }
-#pragma unroll
         for (int u = 0; u < kB; ++u) {
             if (!bl[u].on) continue;
-            const float vr = bl[u].vs * v_over;
+            const float vs = fabsf(bl[u].vs);
+            if (vs > v_unit || (vs < v_unit * 0x1p-8f && v_unit > v_floor)) {
+                // To the next power of two.
+                const float to = __uint_as_float((__float_as_uint(vs) + 0x7fffffu) & 0xff800000u);
+                v_floor = fmaxf(v_floor, fmaxf(to * 0x1p-60f, 0x1p-126f));
+                const float unit = fminf(fmaxf(to, v_floor), 0x1p126f);
+                const float alpha = v_unit * inverse_of(unit);
+                v_unit = unit;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < kM; ++i)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) o[nt][i][c] *= alpha;
+            }
+            const float vr = bl[u].vs * inverse_of(v_unit);
             uint32_t b[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
