@@ -278,3 +278,32 @@ def test_paged_pages_of_zeros(zero, dim):
         out = c.call(q, [1, 1, 1], scale=0.1, hint=hint)
         assert torch.count_nonzero(out[0]) == 0
         c.held(q, [1, 1, 1], out, scale=0.1)
+
+
+# ---- capped scores of very different rows ------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("slopes", [False, True], ids=["plain", "slopes"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("cap", [30.0, 200.0, 1e3, 1e4, 1e5, 1e6, 1e7])
+def test_masked_softcap_beside_large_rows(cap, dim, slopes, kind):
+    """Rows with scores of a few, beside rows of the same 32 whose scores are far beyond the cap."""
+    n, h = 300, 2
+    if kind == F16 and cap > 1e6:
+        pytest.skip("queries that large are not binary16")
+    gen = torch.Generator().manual_seed(20)
+    small = 2.0 ** -9
+    size = torch.where(torch.arange(n) % 3 == 1, small * cap, small)
+    q = (torch.randn(1, h, n, dim, generator=gen) * size[:, None]).to(kind).cuda()
+    k, v = (torch.randn(1, 1, n, dim, generator=gen).to(kind).cuda() for _ in range(2))
+    scale = 3.0 / (small * math.sqrt(dim))
+    s = torch.tensor([0.5, 0.125]) if slopes else None
+    out = tk_b200.attention_masked(q, k, v, scale=scale, causal=True, softcap=cap, alibi_slopes=None if s is None else s.cuda())
+    pos = np.arange(n)
+    for j in range(h):
+        want, bound = rows_of(q[0, j].cpu().double().numpy(), k[0, 0].cpu().double().numpy(), v[0, 0].cpu().double().numpy(),
+                              pos[None] <= pos[:, None], scale=scale, cap=cap, half_p=plain64.HALF[kind], half_out=plain64.HALF[kind],
+                              far=np.abs(pos[:, None] - pos[None]), slope=0.0 if s is None else float(s[j]))
+        err = np.abs(out[0, j].cpu().double().numpy() - want)
+        assert np.all(err <= bound), (j, float((err / bound).max()))
+    assert tk_b200.device_status() == 0

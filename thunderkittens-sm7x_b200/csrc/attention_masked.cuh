@@ -431,7 +431,10 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 // standard deviation of the scores 6, near: 348; cap 10, far: 465 (617 with a reciprocal a score in a pass
 // of its own; 450 with a second polynomial where |y| < 8/5 suffices, which leaves 617 beyond it); cap 30,
 // both ranges along a row: 553, since the two loops share an instruction cache that holds one.
-enum CapRange { kNear, kFar };
+//   kBoth: each value as its own size asks, for caps above kFineCap: kFar is off by softcap * 2^-22 however small
+//     the score, and a row of small scores may share a warp with one of large scores.
+enum CapRange { kNear, kFar, kBoth };
+constexpr float kFineCap = 256.0f;  // kFar is off by 2^-14 at most up to here
 
 // r *= k; whether all of the warp's |r| are below 2 then.
 __device__ __forceinline__ bool scale_row(uint32_t (&r)[128], float k) {
@@ -507,8 +510,8 @@ struct Cap4<kFar> {
     }
 };
 
-// z to capped scores, in place. kFar takes a reciprocal a score: a NaN that a mask will hide must
-// not reach others.
+// z to capped scores, in place. kFar and kBoth take a reciprocal a score: a NaN that a mask will hide
+// must not reach others.
 template <CapRange kRange>
 __device__ __forceinline__ void cap_row(uint32_t (&r)[128], float out) {
     const Cap4<kNear> near(out, 0.0f);
@@ -523,6 +526,11 @@ __device__ __forceinline__ void cap_row(uint32_t (&r)[128], float out) {
             const float2 t = mul2(z, make_float2(kCapArg, kCapArg));
             const float2 d = attn::add2(make_float2(ex2(t.x), ex2(t.y)), make_float2(1.0f, 1.0f));
             x = fma2(make_float2(rcp_approx(d.x), rcp_approx(d.y)), twice, out2);
+            if constexpr (kRange == kBoth) {
+                const float2 small = near.one(z);
+                if (fabsf(z.x) < 2.0f) x.x = small.x;
+                if (fabsf(z.y) < 2.0f) x.y = small.y;
+            }
         }
         r[i] = __float_as_uint(x.x);
         r[i + 1] = __float_as_uint(x.y);
@@ -586,7 +594,8 @@ enum Kind {
     kPlain,        // a positive scale, folded into the exponent
     kCap,
     kBias,         // slopes, or a non-positive scale
-    kCapBias,      // a cap of great size too
+    kCapBias,
+    kCapFine,      // a cap above kFineCap, with slopes or without
 };
 
 template <int kDPad, bool kBf16, Kind kKind, bool kDocs>
@@ -981,7 +990,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             float slope = 0.0f;
-            if ((kKind == kBias || kKind == kCapBias) && p.slopes != nullptr) slope = p.slopes[head] * kLog2e;
+            if ((kKind == kBias || kKind == kCapBias || kKind == kCapFine) && p.slopes != nullptr) slope = p.slopes[head] * kLog2e;
             float m_run = -INFINITY;  // reference point, log2 units
             float l_run = 0.0f;       // running sum of 2^(x - m_run + kLift)
             for (int j = b0; j < b1; ++j) {
@@ -1005,7 +1014,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float cap_out = p.softcap * kLog2e;
                 // The chunks are worked out before the bias (122 against 128 us with documents and slopes,
                 // 8192 x 64), but after a cap (348 against 352 us).
-                constexpr bool kCapped = kKind == kCap || kKind == kCapBias;
+                constexpr bool kCapped = kKind == kCap || kKind == kCapBias || kKind == kCapFine;
                 Chunks chunks{0, 15};
                 if (!kCapped && need_mask) chunks = chunks_of(lo - kv0, hi - kv0);
                 // Capped scores without a bias go from z to P in one pass, where a masked z of -inf ends as a
@@ -1015,14 +1024,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if constexpr (kCapped) {
                     range = cap_range(r, p.scale / p.softcap);
                     fused = kKind == kCap && (range == kNear || !need_mask);
-                    if (kKind == kCapBias && range == kNear) {
+                    if (kKind != kCap && range == kNear) {
                         cap_row<kNear>(r, cap_out);
+                    } else if (kKind == kCapFine) {
+                        cap_row<kBoth>(r, cap_out);
                     } else if (!fused) {
                         cap_row<kFar>(r, cap_out);
                     }
                     c = 1.0f;
                 }
-                if constexpr (kKind == kBias || kKind == kCapBias) {
+                if (kKind == kBias || kKind == kCapBias || (kKind == kCapFine && p.slopes != nullptr)) {
                     // Keys behind the row's position are masked, unless all of them are seen.
                     const bool left = (p.causal && p.prefix == nullptr) || __all_sync(0xffffffffu, kv0 + kBlockKV - 1 <= pos);
                     const bool right = __all_sync(0xffffffffu, kv0 >= pos);
@@ -1195,9 +1206,11 @@ cudaError_t launch_kind(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
 template <int kDPad, bool kBf16>
 cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int device,
                    int grid, cudaStream_t stream) {
-    // kCap takes a row's reference point from cap_one, which is off by up to softcap * 2^-20: above this it
-    // would no longer bound the row's weights, and kCapBias takes it from the capped scores.
-    const bool bias = p.slopes != nullptr || (p.softcap == 0.0f && !(p.scale > 0.0f)) || p.softcap > 1e5f;
+    const bool bias = p.slopes != nullptr || (p.softcap == 0.0f && !(p.scale > 0.0f));
+    // kCap takes a row's reference point from cap_one and large scores from kFar, both off by softcap * 2^-22 and
+    // more; kCapFine takes the point from the capped scores, and those from kBoth. With kBoth in kCapBias, that
+    // lost 2 to 8 % for ordinary caps (causal, 2 x 32 heads, 4096 x 128, cap 50, 10: 441, 605 us against 451, 636).
+    if (p.softcap > kFineCap) return launch_kind<kDPad, kBf16, kCapFine>(mq, mk, mv, p, device, grid, stream);
     if (p.softcap > 0.0f)
         return bias ? launch_kind<kDPad, kBf16, kCapBias>(mq, mk, mv, p, device, grid, stream)
                     : launch_kind<kDPad, kBf16, kCap>(mq, mk, mv, p, device, grid, stream);
