@@ -244,7 +244,8 @@ TK_API cudaError_t tk_attention_forward_gqa_f16(const void* q, const void* k, co
  * Elements are binary16 (_f16) or bfloat16 (_bf16), out alike. Probabilities are
  * rounded to that type before the PV product, everything between is FP32.
  * head_dim in {16, 32, 64, 128}; seq_q, seq_kv >= 1; |scale| <= 1e30; softcap 0 (none)
- * or 1e-6 to 1e30; with doc_ids, batch at most 65535.
+ * or 1e-6 to 1e30 (up to 256, |scale| is 0 or at least softcap * 2^-125); with doc_ids,
+ * batch at most 65535.
  * strides (host): 12 values in elements, (batch, head, row) of Q, K, V and out in
  * turn, or NULL for contiguous tensors; the elements of a row are adjacent. Strides of
  * dimensions larger than 1 must be positive, and out's rows must not share elements.
@@ -337,8 +338,8 @@ TK_API cudaError_t tk_kv_append_e4m3_bf16(const void* k, const void* v, int64_t 
  * are left as they were). max_seq_len only sets how the work is split and should be near
  * the largest seq_lens; results are right for any. head_dim 64 or 128; page_size 16, 32,
  * 64 or 128; q and out 16-byte aligned with strides that are multiples of 8, caches
- * 32-byte aligned; max_pages * page_size at most 2^30; scale and softcap as for
- * tk_attention_masked; n_requests * heads_kv * ceil(max_query_len * heads_q / heads_kv
+ * 32-byte aligned; max_pages * page_size at most 2^30; |scale| <= 1e30; softcap 0
+ * (none) or 1e-6 to 1e30; n_requests * heads_kv * ceil(max_query_len * heads_q / heads_kv
  * / 16) at most 2^24. Long contexts take scratch for their chunks' partial sums. */
 TK_API cudaError_t tk_attention_paged_e4m3_f16(
     const void* q, int64_t q_stride, void* out, int64_t out_stride, int n_tokens, const void* k_cache,

@@ -32,3 +32,16 @@ def test_aligned_pointers_are_not_refused():
             append(ksc=6 * MB + 4, vsc=7 * MB + 4, slots=3 * MB + 8),
             paged(ksc=5 * MB + 4, vsc=6 * MB + 4, table=7 * MB + 4, lens=8 * MB + 4, starts=9 * MB + 4, slopes=10 * MB + 4)]
     assert INVALID not in good
+
+
+# scale / softcap below FP32's normal range would lose the scores' bits or all of them.
+@pytest.mark.parametrize("scale,cap", [(1e-38, 1.0), (-1e-38, 30.0), (1e-45, 1e-6), (2e-36, 256.0)])
+def test_scale_far_below_the_cap(scale, cap):
+    assert masked(scale=scale, cap=cap) == INVALID
+
+
+@pytest.mark.parametrize("scale,cap", [(0.0, 30.0), (1e-35, 30.0), (1e-37, 1.0), (1e-38, 0.0), (1e-38, 257.0), (1e-45, 1e30)])
+def test_scale_above_that_is_not_refused(scale, cap):
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is present")
+    assert masked(scale=scale, cap=cap) != INVALID

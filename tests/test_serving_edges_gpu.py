@@ -307,3 +307,20 @@ def test_masked_softcap_beside_large_rows(cap, dim, slopes, kind):
         err = np.abs(out[0, j].cpu().double().numpy() - want)
         assert np.all(err <= bound), (j, float((err / bound).max()))
     assert tk_b200.device_status() == 0
+
+
+@pytest.mark.parametrize("cap", [300.0, 1e9, 1e25, 1e30])
+@pytest.mark.parametrize("scale", [1e-6, 1e-12, 1e-20, 1e-30, 1e-37])
+def test_masked_small_scale_under_a_large_cap(scale, cap):
+    """Large values and a small scale: the scores are a few, scale / softcap is below what FP32 holds."""
+    gen = torch.Generator().manual_seed(21)
+    size = math.sqrt(3.0 / (scale * 8.0))
+    q, k = (torch.randn(1, 1, 200, 64, generator=gen).mul(size).to(BF16).cuda() for _ in range(2))
+    v = torch.randn(1, 1, 200, 64, generator=gen).to(BF16).cuda()
+    pos = np.arange(200)
+    for s in (None, torch.tensor([0.25])):
+        out = tk_b200.attention_masked(q, k, v, scale=scale, causal=True, softcap=cap, alibi_slopes=None if s is None else s.cuda())
+        want, bound = rows_of(q[0, 0].cpu().double().numpy(), k[0, 0].cpu().double().numpy(), v[0, 0].cpu().double().numpy(),
+                              pos[None] <= pos[:, None], scale=float(np.float32(scale)), cap=cap, half_p=2.0 ** -8, half_out=2.0 ** -8,
+                              far=np.abs(pos[:, None] - pos[None]), slope=0.0 if s is None else 0.25)
+        assert np.all(np.abs(out[0, 0].cpu().double().numpy() - want) <= bound)

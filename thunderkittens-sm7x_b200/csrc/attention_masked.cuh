@@ -450,9 +450,16 @@ __device__ __forceinline__ bool scale_row(uint32_t (&r)[128], float k) {
     return !__any_sync(0xffffffffu, ((any[0] | any[1]) | (any[2] | any[3])) & 0x40000000u);
 }
 
-// Scores to z, and the range the warp's lie in. over = scale / softcap.
-__device__ __forceinline__ CapRange cap_range(uint32_t (&r)[128], float over) {
-    return scale_row(r, 8.0f / 3.0f * over) ? kNear : kFar;
+// Scores to z, and the range the warp's lie in. kSteps: scale, then cap, where their quotient is below what
+// FP32 holds.
+template <bool kSteps>
+__device__ __forceinline__ CapRange cap_range(uint32_t (&r)[128], float scale, float softcap) {
+    if (kSteps && fabsf(scale) < softcap * 0x1p-125f) {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * scale);
+        scale = 1.0f;
+    }
+    return scale_row(r, 8.0f / 3.0f * (scale / softcap)) ? kNear : kFar;
 }
 
 constexpr float kCapArg = 0.75f * kLog2e;  // e^2y = 2^(kCapArg z)
@@ -1022,7 +1029,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 CapRange range = kFar;
                 bool fused = false;
                 if constexpr (kCapped) {
-                    range = cap_range(r, p.scale / p.softcap);
+                    range = cap_range<kKind == kCapFine>(r, p.scale, p.softcap);
                     fused = kKind == kCap && (range == kNear || !need_mask);
                     if (kKind != kCap && range == kNear) {
                         cap_row<kNear>(r, cap_out);
@@ -1280,6 +1287,9 @@ inline cudaError_t masked_entry(bool bf16, const void* q, const void* k, const v
         host::misaligned(doc_ids, 4) || host::misaligned(prefix, 4)) {
         return cudaErrorInvalidValue;
     }
+    // A normal scale / softcap; above kFineCap the kernel divides the scores instead.
+    const float size = scale < 0.0f ? -scale : scale;
+    if (softcap > 0.0f && softcap <= kFineCap && scale != 0.0f && size < softcap * 0x1p-125f) return cudaErrorInvalidValue;
     const long long bh = static_cast<long long>(batch) * heads;
     const int pairs = static_cast<int>((seq_q + 255LL) / 256);
     // Positions and the last tile's ends stay below 2^31.

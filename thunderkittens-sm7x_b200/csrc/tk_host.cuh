@@ -173,8 +173,8 @@ cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, unsigned threads,
 }
 
 // Softmax scale and score cap of the attention entry points with score changes: a finite
-// scale (in log2 units too), and a cap that is 0 (none) or leaves the factors scale / cap
-// and cap * log2(e) finite and normal.
+// scale (in log2 units too), and a cap that is 0 (none) or leaves 1 / cap and cap * log2(e)
+// finite and normal, and scale / cap finite.
 inline bool scores_ok(float scale, float softcap) {
     const bool scale_ok = scale >= -1e30f && scale <= 1e30f;
     return scale_ok && (softcap == 0.0f || (softcap >= 1e-6f && softcap <= 1e30f));
