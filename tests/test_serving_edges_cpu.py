@@ -3,6 +3,8 @@
 import pytest
 import torch
 
+import tk_b200
+
 from test_serving_cpu import INVALID, MB, append, masked, paged, plan
 
 # Pointers off their element's alignment: a kernel would fault on them.
@@ -45,3 +47,30 @@ def test_scale_above_that_is_not_refused(scale, cap):
     if torch.cuda.is_available():
         pytest.skip("a GPU is present")
     assert masked(scale=scale, cap=cap) != INVALID
+
+
+OTHER_BYTES = [torch.int8, torch.bool, torch.float8_e5m2, torch.float8_e4m3fnuz, torch.float8_e5m2fnuz]
+
+
+@pytest.mark.parametrize("kinds", [(t, t) for t in OTHER_BYTES] + [(torch.uint8, t) for t in OTHER_BYTES],
+                         ids=lambda p: "-".join(str(t).split(".")[1] for t in p))
+def test_helpers_refuse_caches_of_other_bytes(kinds):
+    """Bytes of another format would be read as e4m3. (All on the CPU: right types are refused for that.)"""
+    k, v = (torch.zeros(3, 2, 16, 64, dtype=torch.uint8).view(t) for t in kinds)
+    scale = torch.zeros(3, 2)
+    x = torch.zeros(5, 2, 64, dtype=torch.float16)
+    i = torch.int32
+    with pytest.raises(ValueError, match="_cache"):
+        tk_b200.kv_append(x, x, torch.zeros(5, dtype=torch.int64), k, v, scale, scale)
+    with pytest.raises(ValueError, match="_cache"):
+        tk_b200.attention_paged(x, k, v, scale, scale, torch.zeros(3, 4, dtype=i), torch.zeros(3, dtype=i), torch.zeros(4, dtype=i), scale=1.0)
+
+
+@pytest.mark.parametrize("k_kind", [torch.uint8, torch.float8_e4m3fn], ids=["uint8", "e4m3fn"])
+@pytest.mark.parametrize("v_kind", [torch.uint8, torch.float8_e4m3fn], ids=["uint8", "e4m3fn"])
+def test_helpers_take_e4m3_bytes(v_kind, k_kind):
+    k, v = (torch.zeros(3, 2, 16, 64, dtype=torch.uint8).view(t) for t in (k_kind, v_kind))
+    scale = torch.zeros(3, 2)
+    x = torch.zeros(5, 2, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="CUDA device"):  # all that is left to refuse
+        tk_b200.kv_append(x, x, torch.zeros(5, dtype=torch.int64), k, v, scale, scale)

@@ -254,7 +254,8 @@ struct Cache {
 Cache cache_of(PyObject* const* a, const at::Tensor& as) {
     const at::Tensor &k = tensor(a[0], "k_cache"), &v = tensor(a[1], "v_cache"), &ks = tensor(a[2], "k_scale"), &vs = tensor(a[3], "v_scale");
     if (k.dim() != 4) refuse("k_cache must be [pages, Hkv, page_size, D]");
-    if (k.element_size() != 1 || v.element_size() != 1) refuse("k_cache and v_cache must hold bytes (uint8 or float8_e4m3fn)");
+    for (const at::Tensor* t : {&k, &v})
+        if (t->scalar_type() != at::kByte && t->scalar_type() != at::kFloat8_e4m3fn) refuse("k_cache and v_cache must be uint8 or float8_e4m3fn");
     vector(k, as, "k_cache", k.scalar_type(), k.sizes());
     vector(v, as, "v_cache", v.scalar_type(), k.sizes());
     vector(ks, as, "k_scale", at::kFloat, k.sizes().slice(0, 2));
