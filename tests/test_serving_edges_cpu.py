@@ -74,3 +74,12 @@ def test_helpers_take_e4m3_bytes(v_kind, k_kind):
     x = torch.zeros(5, 2, 64, dtype=torch.float16)
     with pytest.raises(ValueError, match="CUDA device"):  # all that is left to refuse
         tk_b200.kv_append(x, x, torch.zeros(5, dtype=torch.int64), k, v, scale, scale)
+
+
+def test_plan_of_no_requests_takes_null():
+    """Arrays without an element may be null; the others may not."""
+    empty = dict(r=0, cached=None, new=None, table=None, lens=None, seq=None)
+    for over in (dict(n_free=None), dict(starts=None), dict(left=None), dict(slots=None), dict(free=None), dict(width=0), dict(left=8 * MB)):
+        assert plan(**{**empty, **over}) == INVALID
+    if not torch.cuda.is_available():
+        assert plan(**empty) != INVALID and plan(**empty, free=None, cap=0, slots=None, tokens=0) != INVALID

@@ -324,3 +324,23 @@ def test_masked_small_scale_under_a_large_cap(scale, cap):
                               pos[None] <= pos[:, None], scale=float(np.float32(scale)), cap=cap, half_p=2.0 ** -8, half_out=2.0 ** -8,
                               far=np.abs(pos[:, None] - pos[None]), slope=0.0 if s is None else 0.25)
         assert np.all(np.abs(out[0, 0].cpu().double().numpy() - want) <= bound)
+
+
+# ---- an idle step ----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("max_tokens", [0, 7, 9000])
+def test_plan_of_no_requests(max_tokens, in_place):
+    """The helper's call with empty tensors: the slots stand for nothing, the free pages stay; and the rest of the step."""
+    none, table, n_free = ints([]), torch.empty(0, 4, dtype=torch.int32, device="cuda"), ints([3])
+    out = dict(lens_out=none, n_free_out=n_free) if in_place else {}
+    lens, seq, starts, slots, left = tk_b200.kv_plan(none, ints([]), table, ints([4, 5, 6]), n_free, page_size=16, max_tokens=max_tokens, **out)
+    assert lens.numel() == 0 and seq.numel() == 0 and starts.tolist() == [0] and left.tolist() == [3]
+    assert slots.tolist() == [-1] * max_tokens
+    cache, scale = torch.zeros(9, 2, 16, 64, dtype=torch.uint8, device="cuda"), torch.ones(9, 2, device="cuda")
+    x = torch.ones(max_tokens, 2, 64, dtype=F16, device="cuda")
+    tk_b200.kv_append(x, x, slots, cache, cache.clone(), scale, scale.clone())
+    assert torch.count_nonzero(cache) == 0 and torch.all(scale == 1)
+    q = torch.ones(max_tokens, 4, 64, dtype=F16, device="cuda")
+    keep = torch.full_like(q, 3.0)
+    assert torch.all(tk_b200.attention_paged(q, cache, cache, scale, scale, table, seq, starts, scale=0.1, out=keep) == 3.0)

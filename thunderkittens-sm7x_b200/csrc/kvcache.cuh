@@ -319,8 +319,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_fill_kernel(const PlanParam
 inline cudaError_t plan_entry(const int* cached, const int* fresh, int n_requests, int page, int* table, int width,
                               const int* free_pages, int free_capacity, const int* n_free, int* lens_out, int* seq_lens,
                               int* starts, int64_t* slots, int max_tokens, int* n_free_out, cudaStream_t stream) {
-    if (cached == nullptr || fresh == nullptr || n_free == nullptr || lens_out == nullptr || seq_lens == nullptr ||
-        starts == nullptr || n_free_out == nullptr || table == nullptr || n_requests < 0 || width <= 0 || page <= 0 ||
+    // Arrays without an element may be null.
+    const bool none = n_requests == 0;
+    if ((!none && (cached == nullptr || fresh == nullptr || lens_out == nullptr || seq_lens == nullptr || table == nullptr)) ||
+        n_free == nullptr || starts == nullptr || n_free_out == nullptr || n_requests < 0 || width <= 0 || page <= 0 ||
         free_capacity < 0 || max_tokens < 0 || (free_pages == nullptr && free_capacity > 0) ||
         (slots == nullptr && max_tokens > 0)) {
         return cudaErrorInvalidValue;
