@@ -83,3 +83,16 @@ def test_plan_of_no_requests_takes_null():
         assert plan(**{**empty, **over}) == INVALID
     if not torch.cuda.is_available():
         assert plan(**empty) != INVALID and plan(**empty, free=None, cap=0, slots=None, tokens=0) != INVALID
+
+
+@pytest.mark.parametrize("cap", [1e-50, 1e-46, -1e-50])
+def test_helpers_refuse_caps_that_are_no_float(cap):
+    """A cap that is 0 only in 32 bits is not 'none': refused, as the entry points refuse others below 1e-6."""
+    q = torch.zeros(1, 2, 8, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="softcap"):
+        tk_b200.attention_masked(q, q, q, scale=1.0, softcap=cap)
+    cache, scale = torch.zeros(3, 2, 16, 64, dtype=torch.uint8), torch.ones(3, 2)
+    i = torch.int32
+    with pytest.raises(ValueError, match="softcap"):
+        tk_b200.attention_paged(torch.zeros(5, 2, 64, dtype=torch.float16), cache, cache, scale, scale, torch.zeros(3, 4, dtype=i),
+                                torch.zeros(3, dtype=i), torch.zeros(4, dtype=i), scale=1.0, softcap=cap)

@@ -59,6 +59,14 @@ double number(PyObject* o, const char* name) {
     return v;
 }
 
+// A cap in 32 bits; 0 means none, so what only becomes 0 there is not that.
+float cap_of(PyObject* o) {
+    const double v = number(o, "softcap");
+    const float cap = static_cast<float>(v);
+    if (cap == 0.0f && v != 0.0) refuse("softcap must be 0 (none) or from 1e-6 to 1e30");
+    return cap;
+}
+
 int whole(PyObject* o, const char* name) {
     int overflow = 0;
     const long v = PyLong_AsLongAndOverflow(o, &overflow);
@@ -153,7 +161,7 @@ PyObject* attention_masked(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const float scale = static_cast<float>(number(a[3], "scale"));
         const int causal = PyObject_IsTrue(a[4]);
         if (causal < 0) return nullptr;
-        const float cap = static_cast<float>(number(a[5], "softcap"));
+        const float cap = cap_of(a[5]);
         const auto slopes = maybe(a[6], "alibi_slopes"), ids = maybe(a[7], "doc_ids"), prefix = maybe(a[8], "prefix_lens");
         auto out = maybe(a[9], "out");
         if (slopes) vector(*slopes, q, "alibi_slopes", at::kFloat, {h});
@@ -312,7 +320,7 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
         vector(table, q, "block_table", at::kInt, table.sizes());
         vector(lens, q, "seq_lens", at::kInt, {r});
         vector(starts, q, "starts", at::kInt, {static_cast<int64_t>(r) + 1});
-        const float scale = static_cast<float>(number(a[8], "scale")), cap = static_cast<float>(number(a[9], "softcap"));
+        const float scale = static_cast<float>(number(a[8], "scale")), cap = cap_of(a[9]);
         const auto slopes = maybe(a[10], "alibi_slopes");
         if (slopes) vector(*slopes, q, "alibi_slopes", at::kFloat, {heads});
         const int most_queries = whole(a[11], "max_query_len");
