@@ -344,3 +344,93 @@ def test_plan_of_no_requests(max_tokens, in_place):
     q = torch.ones(max_tokens, 4, 64, dtype=F16, device="cuda")
     keep = torch.full_like(q, 3.0)
     assert torch.all(tk_b200.attention_paged(q, cache, cache, scale, scale, table, seq, starts, scale=0.1, out=keep) == 3.0)
+
+
+# ---- autograd ------------------------------------------------------------------------------------
+
+def attention_calls():
+    """(call, tensors by name) of both attentions; any float tensor may be replaced."""
+    gen = torch.Generator().manual_seed(30)
+    q, k, v = (torch.randn(1, h, 40, 64, generator=gen).half().cuda() for h in (4, 2, 2))
+    slopes = torch.rand(4, generator=gen).cuda()
+    masked = dict(q=q, k=k, v=v, slopes=slopes)
+    c = Paged([40], 4, 2, 16, 64, seed=31)
+    paged = dict(q=queries(1, 4, 64, F16, 32).cuda(), ks=c.k_scale.cuda(), vs=c.v_scale.cuda(), slopes=slopes)
+    kc, vc = c.k.cuda(), c.v.cuda()
+    table, lens, starts = ints(c.table), ints([40]), ints([0, 1])
+
+    def call_masked(q, k, v, slopes, out=None):
+        return tk_b200.attention_masked(q, k, v, scale=0.1, causal=True, alibi_slopes=slopes, out=out)
+
+    def call_paged(q, ks, vs, slopes, out=None):
+        return tk_b200.attention_paged(q, kc, vc, ks, vs, table, lens, starts, scale=0.1, alibi_slopes=slopes, out=out)
+
+    return [(call_masked, masked), (call_paged, paged)]
+
+
+@pytest.mark.parametrize("which", [0, 1], ids=["masked", "paged"])
+def test_backward_raises(which):
+    """There is no gradient: an output of inputs that require one says so in backward, and is right otherwise."""
+    call, given = attention_calls()[which]
+    want = call(**given)
+    assert not want.requires_grad
+    for name in given:
+        leaf = given[name].clone().requires_grad_()
+        for x in (leaf, leaf * 1):
+            args = {**given, name: x}
+            out = call(**args)
+            assert torch.equal(out, want) and out.requires_grad
+            with pytest.raises(RuntimeError, match="not implemented"):
+                out.float().sum().backward()
+            assert leaf.grad is None
+            with torch.no_grad():
+                assert not call(**args).requires_grad
+            with pytest.raises(ValueError, match="out"):
+                call(**args, out=torch.empty_like(want))
+            with torch.no_grad():
+                out = torch.empty_like(want)
+                call(**args, out=out)
+                assert torch.equal(out, want)
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(given[name], torch.ones_like(given[name]))
+            with pytest.raises(ValueError, match="forward-mode"):
+                call(**{**given, name: dual})
+    with torch.inference_mode():
+        inner = {k: v.clone() for k, v in given.items()}
+        assert torch.equal(call(**inner), want)
+        out = torch.empty_like(want)
+    call(**inner, out=out)  # inference tensors have no version
+    assert torch.equal(out, want)
+
+
+def test_written_tensors_have_new_versions():
+    """What a call writes in place counts as changed: a backward pass that saved it before raises."""
+    for call, given in attention_calls():
+        out = torch.empty_like(given["q"])
+        version = out._version
+        call(**given, out=out)
+        assert out._version > version
+        weight = torch.ones_like(out, requires_grad=True)
+        loss = (out * weight).float().sum()
+        call(**given, out=out)
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+        with pytest.raises(ValueError, match="out"):
+            call(**given, out=torch.empty_like(out).requires_grad_())
+    lens, new, table, free, n_free = ints([3]), ints([4]), ints([[0, -1]]), ints([1, 2]), ints([2])
+    slots = torch.empty(4, dtype=torch.int64, device="cuda")
+    before = [t._version for t in (lens, table, n_free, slots, new, free)]
+    tk_b200.kv_plan(lens, new, table, free, n_free, page_size=4, max_tokens=4, lens_out=lens, n_free_out=n_free, slots=slots)
+    after = [t._version for t in (lens, table, n_free, slots, new, free)]
+    assert all(a > b for a, b in zip(after[:4], before[:4])) and after[4:] == before[4:]
+    cache, scales = [torch.zeros(3, 2, 16, 64, dtype=torch.uint8, device="cuda") for _ in range(2)], [torch.ones(3, 2, device="cuda") for _ in range(2)]
+    x = torch.ones(4, 2, 64, dtype=F16, device="cuda")
+    before = [t._version for t in cache + scales]
+    tk_b200.kv_append(x, x, slots, *cache, *scales)
+    assert all(t._version > b for t, b in zip(cache + scales, before))
+    tk_b200.kv_append(x.clone().requires_grad_(), x, slots, *cache, *scales)  # 8 bits carry no gradient
+    for i in range(2):
+        bad = list(scales)
+        bad[i] = scales[i].clone().requires_grad_()
+        with pytest.raises(ValueError, match="_scale"):
+            tk_b200.kv_append(x, x, slots, *cache, *bad)

@@ -2,7 +2,8 @@
 // operators (include/tk_b200.h): takes torch tensors, checks them, allocates what is not
 // given, and calls the entry point on the tensors' device and its current stream.
 //
-// It computes nothing. It exists because the smallest of these calls take a few
+// It computes nothing, and no gradients: an output of inputs that require them carries a node that raises in
+// backward, tangents of forward mode are refused, and tensors written in place get a new version. It exists because the smallest of these calls take a few
 // microseconds on the GPU, and looking at a dozen tensors from Python takes longer than
 // that (kv_append of 64 tokens: 11 us in Python with ctypes, 4.9 us here).
 //
@@ -15,10 +16,17 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/forward_grad.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <initializer_list>
+#include <memory>
 #include <optional>
 #include <string>
+#include <utility>
 
 #include "tk_b200.h"
 
@@ -110,6 +118,45 @@ T* data(const std::optional<at::Tensor>& t) {
     return t ? static_cast<T*>(t->data_ptr()) : nullptr;
 }
 
+// ---- autograd
+
+// Whether forward mode is in use at all; only then are tensors asked for tangents.
+bool forward_mode() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
+
+// What a call reads: whether gradients have to reach any of it.
+bool tracked(std::initializer_list<const at::Tensor*> reads) {
+    bool some = false;
+    const bool forward = forward_mode();
+    for (const at::Tensor* t : reads) {
+        if (t == nullptr) continue;
+        some = some || t->requires_grad();
+        if (forward && t->_fw_grad(0).defined()) refuse("there is no forward-mode derivative");
+    }
+    return some && at::GradMode::is_enabled();
+}
+
+// Before a call writes a tensor of the caller's.
+void writable(const at::Tensor& t, const char* name) {
+    if (at::GradMode::is_enabled() && t.requires_grad()) refuse(std::string(name) + " is written in place and must not require gradients");
+    if (forward_mode() && t._fw_grad(0).defined()) refuse("there is no forward-mode derivative");
+}
+
+// After it has.
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// Backward through `out` raises instead of leaving gradients out.
+void no_backward(const at::Tensor& out, const char* name, std::initializer_list<const at::Tensor*> reads) {
+    torch::autograd::edge_list edges;
+    for (const at::Tensor* t : reads)
+        if (t != nullptr && t->requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(*t));
+    std::shared_ptr<torch::autograd::Node> node(new torch::autograd::NotImplemented(name, std::move(edges)), torch::autograd::deleteNode);
+    torch::autograd::set_history(out, node);
+}
+
+const at::Tensor* if_given(const std::optional<at::Tensor>& t) { return t ? &*t : nullptr; }
+
 struct Failed {
     const char* name;
     int code;
@@ -168,6 +215,12 @@ PyObject* attention_masked(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (ids) vector(*ids, q, "doc_ids", at::kInt, {b, sq});
         if (prefix) vector(*prefix, q, "prefix_lens", at::kInt, {b});
         if (out && (out->scalar_type() != q.scalar_type() || out->sizes() != q.sizes())) refuse("out must have q's type and shape");
+        const bool grad = tracked({&q, &k, &v, if_given(slopes)});
+        const bool given = out.has_value();
+        if (given) {
+            writable(*out, "out");
+            if (grad) refuse("out cannot be given where an input requires gradients");
+        }
         if (d > 1 && (q.stride(3) != 1 || k.stride(3) != 1 || v.stride(3) != 1 || (out && out->stride(3) != 1)))
             refuse("the last strides of q, k, v and out must be 1");
         on_cuda(q, "q");
@@ -185,6 +238,8 @@ PyObject* attention_masked(PyObject*, PyObject* const* a, Py_ssize_t n) {
               (bf16 ? tk_attention_masked_bf16 : tk_attention_masked_f16)(
                   q.data_ptr(), k.data_ptr(), v.data_ptr(), out->data_ptr(), strides, b, h, hkv, sq, skv, d, scale, cap,
                   data<float>(slopes), data<int32_t>(ids), data<int32_t>(prefix), causal, scope.stream));
+        if (given) written(*out);
+        if (grad) no_backward(*out, "tk_b200.attention_masked", {&q, &k, &v, if_given(slopes)});
         return THPVariable_Wrap(*out);
     });
 }
@@ -247,6 +302,9 @@ PyObject* kv_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
               tk_kv_plan(cached.data_ptr<int>(), fresh.data_ptr<int>(), r, page, table.data_ptr<int>(), width, free.data_ptr<int>(),
                          fits_int(free.numel(), "free_pages"), n_free.data_ptr<int>(), outs[0].data_ptr<int>(), outs[1].data_ptr<int>(),
                          outs[2].data_ptr<int>(), outs[3].data_ptr<int64_t>(), max_tokens, outs[4].data_ptr<int>(), scope.stream));
+        written(table);
+        for (int i = 0; i < 5; ++i)
+            if (a[7 + i] != Py_None) written(outs[i]);
         PyObject* result = PyTuple_New(5);
         for (int i = 0; i < 5 && result != nullptr; ++i) PyTuple_SET_ITEM(result, i, THPVariable_Wrap(outs[i]));
         return result;
@@ -290,6 +348,10 @@ PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (v.scalar_type() != k.scalar_type() || v.sizes() != k.sizes()) refuse("k and v must have one type and shape");
         same_device(v, k, "v");
         vector(slots, k, "slots", at::kLong, {k.size(0)});
+        writable(c.k, "k_cache");
+        writable(c.v, "v_cache");
+        writable(c.ks, "k_scale");
+        writable(c.vs, "v_scale");
         on_cuda(k, "k");
         const int tokens = fits_int(k.size(0), "k");
         if (tokens > 0) {
@@ -300,6 +362,7 @@ PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
                   (bf16 ? tk_kv_append_e4m3_bf16 : tk_kv_append_e4m3_f16)(
                       k.data_ptr(), v.data_ptr(), k_stride, v_stride, slots.data_ptr<int64_t>(), tokens, c.heads, c.dim, c.k.data_ptr(),
                       c.v.data_ptr(), c.ks.data_ptr<float>(), c.vs.data_ptr<float>(), c.pages, c.page, scope.stream));
+            for (const at::Tensor* t : {&c.k, &c.v, &c.ks, &c.vs}) written(*t);
         }
         Py_RETURN_NONE;
     });
@@ -329,6 +392,12 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
         auto out = maybe(a[13], "out");
         if (out && (out->scalar_type() != q.scalar_type() || out->sizes() != q.sizes())) refuse("out must have q's type and shape");
         const int64_t q_stride = token_stride(q, "q");
+        const bool grad = tracked({&q, &c.k, &c.v, &c.ks, &c.vs, if_given(slopes)});
+        const bool given = out.has_value();
+        if (given) {
+            writable(*out, "out");
+            if (grad) refuse("out cannot be given where an input requires gradients");
+        }
         on_cuda(q, "q");
         if (out) same_device(*out, q, "out");
         const Scope scope(q);
@@ -341,7 +410,9 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
                       q.data_ptr(), q_stride, out->data_ptr(), out_stride, tokens, c.k.data_ptr(), c.v.data_ptr(), c.ks.data_ptr<float>(),
                       c.vs.data_ptr<float>(), c.pages, c.page, table.data_ptr<int>(), width, lens.data_ptr<int>(), starts.data_ptr<int>(), r,
                       heads, c.heads, c.dim, most_queries, most_keys, scale, cap, data<float>(slopes), scope.stream));
+            if (given) written(*out);
         }
+        if (grad) no_backward(*out, "tk_b200.attention_paged", {&q, &c.k, &c.v, &c.ks, &c.vs, if_given(slopes)});
         return THPVariable_Wrap(*out);
     });
 }
