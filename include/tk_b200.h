@@ -290,7 +290,8 @@ TK_API cudaError_t tk_attention_masked_bf16(const void* q, const void* k, const 
  * token; -1 for tokens of requests not taken, behind a negative table entry, and
  * behind the last token), n_free_out (may be n_free). free_pages is not changed. To
  * give pages back, a caller writes them at free_pages[*n_free ...] and raises *n_free.
- * Any page_size >= 1; *n_free is taken as at most n_free_capacity. One launch, no scratch. */
+ * Any page_size >= 1; *n_free is taken as at most n_free_capacity. One launch, or two where
+ * lens_out or n_free_out is the input itself and max_tokens is over 4096; no scratch. */
 TK_API cudaError_t tk_kv_plan(const int32_t* cached_lens, const int32_t* new_lens, int n_requests,
                               int page_size, int32_t* block_table, int max_pages,
                               const int32_t* free_pages, int n_free_capacity, const int32_t* n_free,

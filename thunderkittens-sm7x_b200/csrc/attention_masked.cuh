@@ -30,8 +30,8 @@
 // What bounds it: the softmax, as in attention.cuh. A block of 128 keys takes a warp 1024 MUFU
 // cycles for its exponentials, two warps share each MUFU, and of the rest (loads from tensor
 // memory, max, sums, packing, masks, biases, caps) only part overlaps. Measured on B200, causal,
-// burst clocks: 2 x 32 heads on 2 x 8, 4096 x 128, no change of scores 246 us (1,120 TFLOP/s), softcap
-// 348 us (MUFU floor 115); 11 documents with slopes, 32 heads, 8192 x 64, 122 us (floor 32: 6 blocks an
+// burst clocks: 2 x 32 heads on 2 x 8, 4096 x 128, no change of scores 245 us (1,120 TFLOP/s), softcap
+// 347 us (MUFU floor 115); 11 documents with slopes, 32 heads, 8192 x 64, 122 us (floor 32: 6 blocks an
 // item leave its start and end in sight); 64 heads, a prefix, 1001 rows on 2777 keys, 88 us (256
 // items on 148 SMs: two rounds).
 #pragma once
@@ -66,7 +66,8 @@ constexpr float kLift = 7.0f;  // P <= 2^(8 + kLift) = 2^15 < 65504
 // so the next S is ready when it has finished with this one, and waits for PV_{j-1} (pv_done)
 // only before it writes P and rescales O. Otherwise P overwrites S, PV_j has to complete
 // before S_{j+1}, and each tile's chain S -> softmax -> PV -> S is serial. 2 x 32 heads, unmasked,
-// 4096 x 64: 412 us with P over S, 326 apart.
+// 4096 x 64: 412 us with P over S, 326 apart. head_dim 16 and 32 run in 64 columns too, which TMA fills with zeros: their
+// exponentials bound them all the same (causal, 2 x 32 heads, 4096, head_dim 64 / 32 / 16: 183 / 181 / 181 us, MUFU 115).
 template <int kDPad, bool kBf16>
 struct Cfg {
     static constexpr bool kApart = kDPad == 64;
@@ -430,7 +431,7 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 // throughout (384 and 495 us for the next two figures). 2 x 32 heads on 2 x 8, causal, 4096 x 128: no cap 246 us; cap 50,
 // standard deviation of the scores 6, near: 348; cap 10, far: 465 (617 with a reciprocal a score in a pass
 // of its own; 450 with a second polynomial where |y| < 8/5 suffices, which leaves 617 beyond it); cap 30,
-// both ranges along a row: 553, since the two loops share an instruction cache that holds one.
+// both ranges along a row: 560, since the two loops share an instruction cache that holds one.
 //   kBoth: each value as its own size asks, for caps above kFineCap: kFar is off by softcap * 2^-22 however small
 //     the score, and a row of small scores may share a warp with one of large scores.
 enum CapRange { kNear, kFar, kBoth };

@@ -35,9 +35,9 @@
 // distributed shared memory; more of them leave theirs in scratch, and a second kernel
 // joins those. Either way in chunk order: results do not depend on timing.
 //
-// Measured on B200: 64 requests of 1 to 8192 tokens, 32 heads on 8 of 128, 96 us = 6.03 TB/s (92 % of the
-// measured copy bandwidth); 3 of 30001 to 65536, capped scores, 88 us (92 %). With direct loads to
-// registers instead of the ring 137 us for the first. One request of 2048 tokens 6.8 us: a launch
+// Measured on B200, in a graph: 64 requests of 1 to 8192 tokens, 32 heads on 8 of 128, 96 us = 6.0 TB/s (92 % of the
+// measured copy bandwidth; 99 to 104 us as a pass among others on a stream, 85 to 88 %); 3 of 30001 to 65536, capped
+// scores, 89 us (91 %). With direct loads to registers instead of the ring 137 us for the first. One request of 2048 tokens 6.8 us: a launch
 // and the latencies of lengths, pages, cache and the join. Heads of 64 have twice the tokens, so
 // twice the softmax, for the same bytes, and reach 47 % (ragged, 5 drafted tokens, slopes) to 70 %.
 #pragma once
@@ -826,7 +826,8 @@ inline cudaError_t paged_entry(bool bf16, const void* q, long long q_stride, voi
         // requests of 17 to 4096 tokens, 16 heads, 25.9 or 25.1 us against 24.9, with 5 drafted tokens 28.1
         // or 31.2 against 28.1; 376 of 572 to 1143, 4 heads, 46 or 36 against 36. Chunks of less than that only where even
         // their CTAs are all resident: 148 requests of 1143 tokens, 4 heads of 64, in one chunk each 17.6
-        // us, in two 20; 37 of them 11.0 and 9.2.
+        // us, in two 20; 37 of them 11.0 and 9.2. Few requests pay for it, heads of 128, 8192 tokens, 1 / 2 / 8 requests: one
+        // key head 8.4 / 14.3 / 14.4 us, eight key heads 9.3 / 14.5 / 28.1 (their bytes: 2.6 / 5.1 / 20.5).
         const long long least = n_requests == 1 ? 32768 / dim : 1024;
         const long long rounds = n_requests < kRounds ? n_requests : kRounds;
         const long long want = rounds * 4LL * sm_count / items;
