@@ -96,3 +96,35 @@ def test_helpers_refuse_caps_that_are_no_float(cap):
     with pytest.raises(ValueError, match="softcap"):
         tk_b200.attention_paged(torch.zeros(5, 2, 64, dtype=torch.float16), cache, cache, scale, scale, torch.zeros(3, 4, dtype=i),
                                 torch.zeros(3, dtype=i), torch.zeros(4, dtype=i), scale=1.0, softcap=cap)
+
+
+class Handles:
+    """Stands in for torch.cuda: which stream a handle becomes."""
+
+    class Stream:
+        def __init__(self, name, device):
+            self.name, self.device = name, device
+
+    def __init__(self, monkeypatch):
+        monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: self.Stream("default", device))
+        monkeypatch.setattr(torch.cuda, "ExternalStream", lambda handle, device=None: self.Stream(handle, device))
+        monkeypatch.setattr(torch.cuda, "stream", lambda stream: stream)
+
+
+class OnCuda:
+    device = torch.device("cuda:0")
+
+
+@pytest.mark.parametrize("handle,want", [(0, "default"), (1, "default"), (0x7f00, 0x7f00)])
+def test_stream_handles(handle, want, monkeypatch):
+    """0 and 1 are handles of the default stream, for which ExternalStream makes a stream of its own."""
+    Handles(monkeypatch)
+    stream = tk_b200._on(handle, OnCuda)
+    assert stream.name == want and stream.device == OnCuda.device
+
+
+def test_stream_handle_of_the_thread(monkeypatch):
+    """The per-thread default stream has no counterpart among torch's."""
+    Handles(monkeypatch)
+    with pytest.raises(ValueError, match="stream"):
+        tk_b200._on(2, OnCuda)

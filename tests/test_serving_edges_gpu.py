@@ -434,3 +434,20 @@ def test_written_tensors_have_new_versions():
         bad[i] = scales[i].clone().requires_grad_()
         with pytest.raises(ValueError, match="_scale"):
             tk_b200.kv_append(x, x, slots, *cache, *bad)
+
+
+# ---- stream handles --------------------------------------------------------------------------------
+
+def test_stream_handles():
+    """A call on handle 0 runs on the default stream, on another stream's handle on that one."""
+    call, given = attention_calls()[0]
+    args = (given["q"], given["k"], given["v"])
+    want = tk_b200.attention_masked(*args, scale=0.1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for handle, stream in ((0, torch.cuda.default_stream()), (side.cuda_stream, side)):
+        with tk_b200._on(handle, given["q"]):
+            assert torch.cuda.current_stream().cuda_stream == stream.cuda_stream == handle
+        out = tk_b200.attention_masked(*args, scale=0.1, stream=handle)
+        stream.synchronize()
+        assert torch.equal(out, want)

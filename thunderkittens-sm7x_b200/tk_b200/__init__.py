@@ -316,7 +316,10 @@ def _on(stream, t):
     """Makes a call's stream current, with its device, while the call allocates and launches."""
     import torch
     if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device=t.device)
+        # 0 and 1 are handles of the default stream; ExternalStream(0) would be a new stream.
+        if stream == 2:
+            raise ValueError("the per-thread default stream (handle 2) is none of torch's streams")
+        stream = torch.cuda.default_stream(t.device) if stream in (0, 1) else torch.cuda.ExternalStream(stream, device=t.device)
     if stream.device != t.device:
         raise ValueError(f"stream is on {stream.device}, tensors on {t.device}")
     return torch.cuda.stream(stream)
