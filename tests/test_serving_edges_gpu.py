@@ -451,3 +451,52 @@ def test_stream_handles():
         out = tk_b200.attention_masked(*args, scale=0.1, stream=handle)
         stream.synchronize()
         assert torch.equal(out, want)
+
+
+# ---- large caps under masks -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("dim", [16, 64, 128])
+@pytest.mark.parametrize("cap", [300.0, 1e6])
+@pytest.mark.parametrize("mask", ["documents", "documents_causal", "prefix", "few_keys", "nan_key"])
+def test_masked_large_caps_under_masks(mask, cap, dim, kind):
+    """Caps above 256: padding that holds NaN, a prefix, rows before the first key, a NaN key; rows of a few beside large ones."""
+    n, h = 400, 2
+    gen = torch.Generator().manual_seed(40)
+    size = torch.where(torch.arange(n) % 3 == 1, 0.01 * cap if cap < 1e4 else 3000.0, 2.0)
+    q = (torch.randn(1, h, n, dim, generator=gen) * size[:, None]).to(kind)
+    m = 150 if mask == "few_keys" else n
+    k, v = (torch.randn(1, 1, m, dim, generator=gen).to(kind) for _ in range(2))
+    scale, slopes = 1 / math.sqrt(dim), torch.tensor([0.5, 0.0625])
+    pos, key = np.arange(n) + m - n, np.arange(m)
+    allowed = key[None] <= pos[:, None] if mask != "documents" else np.ones((n, m), bool)
+    kw, clean = dict(causal=mask != "documents"), [x.double().numpy() for x in (q, k, v)]
+    if mask.startswith("documents"):
+        ids = np.searchsorted([3, 100, 131, 260, 390], key, side="right").astype(np.int32)
+        ids[100:131], ids[200:250] = -1, -5
+        allowed = allowed & np.array([[a <= j < b for j in key] for a, b in plain64.runs_of(ids)])
+        kw["doc_ids"] = ints(ids[None])
+        pad = torch.from_numpy(ids < 0)
+        for x in (q, k, v):
+            x[:, :, pad] = float("nan")
+        clean = [np.where((ids < 0)[None, None, :, None], 0.0, x) for x in clean]
+    if mask == "prefix":
+        allowed = allowed | (key < 170)[None]
+        kw["prefix_lens"] = ints([170])
+    if mask == "nan_key":
+        k[:, :, 333] = float("nan")
+    for s in (None, slopes):
+        out = tk_b200.attention_masked(q.cuda(), k.cuda(), v.cuda(), scale=scale, softcap=cap, alibi_slopes=None if s is None else s.cuda(), **kw)
+        o64 = out.cpu().double().numpy()
+        rows = n
+        if mask == "nan_key":
+            assert out[:, :, 333:].isnan().all()
+            rows = 333
+        for j in range(h):
+            want, bound = rows_of(clean[0][0, j][:rows], clean[1][0, 0], clean[2][0, 0], allowed[:rows], scale=scale, cap=cap,
+                                  half_p=plain64.HALF[kind], half_out=plain64.HALF[kind], far=np.abs(pos[:rows, None] - key[None]),
+                                  slope=0.0 if s is None else float(s[j]))
+            err = np.abs(o64[0, j][:rows] - want)
+            assert np.all(err <= bound), (j, float((err / bound).max()))
+            assert np.all(o64[0, j][:rows][~allowed[:rows].any(1)] == 0)
+    assert tk_b200.device_status() == 0
