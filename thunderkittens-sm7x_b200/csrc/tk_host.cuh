@@ -123,14 +123,23 @@ inline cudaError_t scratch_alloc(void** ptr, size_t bytes, int device, cudaStrea
             props.allocType = cudaMemAllocationTypePinned;
             props.location.type = cudaMemLocationTypeDevice;
             props.location.id = device;
-            cudaMemPool_t created = nullptr;
-            cudaError_t err = cudaMemPoolCreate(&created, &props);
+            // Creating a pool is not an operation of any stream, but while this thread captures one it is
+            // only allowed in the relaxed mode.
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            cudaError_t err = cudaThreadExchangeStreamCaptureMode(&mode);
             if (err != cudaSuccess) return err;
+            cudaMemPool_t created = nullptr;
+            err = cudaMemPoolCreate(&created, &props);
             uint64_t keep = UINT64_MAX;
-            err = cudaMemPoolSetAttribute(created, cudaMemPoolAttrReleaseThreshold, &keep);
-            if (err != cudaSuccess) {
+            if (err == cudaSuccess) {
+                err = cudaMemPoolSetAttribute(created, cudaMemPoolAttrReleaseThreshold, &keep);
+                if (err != cudaSuccess) static_cast<void>(cudaMemPoolDestroy(created));
+            }
+            const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+            if (err != cudaSuccess) return err;
+            if (back != cudaSuccess) {
                 static_cast<void>(cudaMemPoolDestroy(created));
-                return err;
+                return back;
             }
             sp.pools[device] = created;
         }
