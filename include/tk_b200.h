@@ -306,7 +306,8 @@ TK_API cudaError_t tk_kv_plan(const int32_t* cached_lens, const int32_t* new_len
  *   least 2^-100; if the page held tokens before (its first new place is not 0), not
  *   below its scale, and where that grows the places before the first new one become
  *   e4m3(old value * old scale / new scale);
- *   new bytes = e4m3(x / scale), nearest even, infinities as 448, NaN as NaN.
+ *   new bytes = e4m3(x / scale), nearest even, infinities as 448, NaN as NaN (x / scale is
+ *   rounded to FP32 first where an older scale that is no power of two stays).
  * Tokens of one page must be adjacent, with consecutive slots, as tk_kv_plan gives
  * them; what a page holds that is named in two separate stretches is not defined.
  * Other places keep their bytes. head_dim 64 or 128, page_size 16, 32, 64 or 128; k, v

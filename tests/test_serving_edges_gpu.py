@@ -500,3 +500,33 @@ def test_masked_large_caps_under_masks(mask, cap, dim, kind):
             assert np.all(err <= bound), (j, float((err / bound).max()))
             assert np.all(o64[0, j][:rows][~allowed[:rows].any(1)] == 0)
     assert tk_b200.device_status() == 0
+
+
+# ---- rescaled pages ---------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tokens", [1, 1500], ids=["warp", "cta"])
+def test_append_rescales_with_one_rounding(tokens, dim):
+    """14 * 2.7142856 / 4 = 9.4999996 is nearer to 9 than to 10; FP32 holds it as 9.5, a tie that goes to 10. All bytes, and
+    scales that bring their products next to the ties of the format."""
+    page, heads = 16, 2
+    every = torch.arange(256, dtype=torch.uint8)
+    every[(every & 0x7f) == 0x7f] = 0
+    factors = [np.float32(t / v) for v in (14.0, 13.0, 11.0, 9.0, 15.0, 7.0) for t in (9.5, 8.5, 10.5, 4.75, 5.25)]
+    factors = [f for f in factors if 0.5 < f < 1] + [np.nextafter(f, np.float32(s)) for f in factors if 0.5 < f < 1 for s in (0, 1)]
+    pages = max(len(factors), -(-tokens // page)) + 1
+    k_cache = every.repeat(pages * heads * page * dim // 256).view(pages, heads, page, dim).clone().cuda()
+    k_scale = torch.ones(pages, heads)
+    for p, f in enumerate(factors):
+        k_scale[p] = 4.0 * float(f)  # from there to 4
+    k_scale = k_scale.cuda()
+    v_cache, v_scale = k_cache.clone(), k_scale.clone()
+    slots = [p * page + 3 for p in range(len(factors))]
+    slots += [-1] * max(0, tokens - len(slots))
+    x = torch.full((len(slots), heads, dim), 1500.0, dtype=F16).cuda()  # needs a scale of 4
+    values, scales = plain64.cache_values(k_cache), k_scale.cpu().double().numpy()
+    plain64.append(x.cpu().double().numpy(), slots, values, scales, page)
+    tk_b200.kv_append(x, x, ints(slots, torch.int64), k_cache, v_cache, k_scale, v_scale)
+    for c, s in ((k_cache, k_scale), (v_cache, v_scale)):
+        assert np.array_equal(s.cpu().double().numpy(), scales)
+        assert np.array_equal(plain64.cache_values(c), values)

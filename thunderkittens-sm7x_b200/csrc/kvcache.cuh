@@ -433,6 +433,13 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
+// a * b rounded to odd: rounded once more, to e4m3's 4 bits, it is the exact product rounded once (a product next to
+// a tie of e4m3 would become that tie in FP32).
+__device__ __forceinline__ float product_to_odd(float a, float b) {
+    const float p = __fmul_rz(a, b);
+    return fmaf(a, b, -p) == 0.0f ? p : __uint_as_float(__float_as_uint(p) | 1u);
+}
+
 // Whether x * (1 / s) is x / s: s a power of two with a normal reciprocal.
 __device__ __forceinline__ bool exact_reciprocal(float s) {
     return (__float_as_uint(s) & 0x7fffffu) == 0 && s >= 7.9e-31f && s < 1.7e38f;
@@ -571,7 +578,8 @@ __global__ void __launch_bounds__(kAppendThreads, kCta ? 8 : 1) append_kernel(co
                     for (int c = 0; c < 4; ++c) {
                         const float2 lo = half2_bits_to_float2(from_e4m3x2(w[c] & 0xffffu));
                         const float2 hi = half2_bits_to_float2(from_e4m3x2(w[c] >> 16));
-                        w[c] = to_e4m3x2(lo.x * factor, lo.y * factor) | to_e4m3x2(hi.x * factor, hi.y * factor) << 16;
+                        w[c] = to_e4m3x2(product_to_odd(lo.x, factor), product_to_odd(lo.y, factor)) |
+                               to_e4m3x2(product_to_odd(hi.x, factor), product_to_odd(hi.y, factor)) << 16;
                     }
                     *reinterpret_cast<uint4*>(bytes + b) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
