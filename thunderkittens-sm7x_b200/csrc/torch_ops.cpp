@@ -135,10 +135,18 @@ bool tracked(std::initializer_list<const at::Tensor*> reads) {
     return some && at::GradMode::is_enabled();
 }
 
-// Before a call writes a tensor of the caller's.
-void writable(const at::Tensor& t, const char* name) {
-    if (at::GradMode::is_enabled() && t.requires_grad()) refuse(std::string(name) + " is written in place and must not require gradients");
-    if (forward_mode() && t._fw_grad(0).defined()) refuse("there is no forward-mode derivative");
+// Before a call writes tensors of the caller's.
+struct Target {
+    const at::Tensor* t;
+    const char* name;
+};
+
+void writable(std::initializer_list<Target> targets) {
+    const bool grads = at::GradMode::is_enabled(), forward = forward_mode();
+    for (const Target& x : targets) {
+        if (grads && x.t->requires_grad()) refuse(std::string(x.name) + " is written in place and must not require gradients");
+        if (forward && x.t->_fw_grad(0).defined()) refuse("there is no forward-mode derivative");
+    }
 }
 
 // After it has.
@@ -218,7 +226,7 @@ PyObject* attention_masked(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const bool grad = tracked({&q, &k, &v, if_given(slopes)});
         const bool given = out.has_value();
         if (given) {
-            writable(*out, "out");
+            writable({{&*out, "out"}});
             if (grad) refuse("out cannot be given where an input requires gradients");
         }
         if (d > 1 && (q.stride(3) != 1 || k.stride(3) != 1 || v.stride(3) != 1 || (out && out->stride(3) != 1)))
@@ -348,10 +356,7 @@ PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (v.scalar_type() != k.scalar_type() || v.sizes() != k.sizes()) refuse("k and v must have one type and shape");
         same_device(v, k, "v");
         vector(slots, k, "slots", at::kLong, {k.size(0)});
-        writable(c.k, "k_cache");
-        writable(c.v, "v_cache");
-        writable(c.ks, "k_scale");
-        writable(c.vs, "v_scale");
+        writable({{&c.k, "k_cache"}, {&c.v, "v_cache"}, {&c.ks, "k_scale"}, {&c.vs, "v_scale"}});
         on_cuda(k, "k");
         const int tokens = fits_int(k.size(0), "k");
         if (tokens > 0) {
@@ -395,7 +400,7 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const bool grad = tracked({&q, &c.k, &c.v, &c.ks, &c.vs, if_given(slopes)});
         const bool given = out.has_value();
         if (given) {
-            writable(*out, "out");
+            writable({{&*out, "out"}});
             if (grad) refuse("out cannot be given where an input requires gradients");
         }
         on_cuda(q, "q");
